@@ -54,6 +54,7 @@ extern "C" {
 /* device status word bits */
 #define SMLM_FLAG_INDEX_RANGE 1
 #define SMLM_FLAG_TIMEOUT 4 /* a bounded wait inside a kernel gave up; that call's outputs are invalid */
+#define SMLM_FLAG_NO_PAGES 8 /* a paged cache ran out of free pages, or a token has no page to be written to */
 
 /* flags of smlm_bag_backward_rows: rows whose touched byte is 0 are written, not accumulated (the caller
  * guarantees such rows count as zero, e.g. a RowStore whose untouched rows are never read as data) */
@@ -472,6 +473,90 @@ SMLM_API int smlm_rows_rowwise_step(float *param, int64_t table_rows, const int6
 SMLM_API int smlm_ngram_rows(const int64_t *c, int64_t batch, int64_t t_len, int history, const int64_t *mult,
                              const int *orders, int n_orders, int heads, int max_order, int64_t rows, int64_t *out,
                              void *stream);
+
+/* ---------------------------------------------------------------------------------- paged key-value cache
+ * No counterpart in the reference (its decoding loop concatenates one growing cache per layer, model.py:91-104).
+ * A layer's keys and values lie in pages of page_size tokens (a power of two up to 4096) of a pool of n_pages pages;
+ * row b of the table (int32, table_rows x max_blocks, table_stride elements apart) lists the pages of sequence b in
+ * order, -1 where it has none, and lengths[b] (int32) counts its tokens. strides: six host integers, the elements
+ * between pages, heads and tokens of k_pages and then of v_pages (multiples of 16 bytes; the head dimension d, a
+ * multiple of 16 up to 256, is contiguous), so that any order of pages, heads and tokens serves. dtype: F32, BF16 or
+ * F16, the same for the cache and the activations. Page numbers outside the pool and lengths outside the table set
+ * SMLM_FLAG_INDEX_RANGE and are left out. */
+
+/* Scratch bytes of smlm_paged_attention. */
+SMLM_API size_t smlm_paged_attention_workspace(int64_t batch, int64_t hq, int64_t d);
+
+/* Attention of one new token per sequence: q and out (batch, hq, d); query head i reads key head i / (hq / hkv).
+ * Token j of sequence b is visible if j < lengths[b], its table entry is not -1, and, with window > 0, if
+ * j >= lengths[b] - window or j < sinks. out = sum_j p_j v_j with p the softmax over the visible tokens of
+ * scale * <q, k_j> (scores, sums and the output's sum in fp32); a row with no visible token (or only scores of
+ * -inf) gives 0. lse: NULL, or fp32 (batch, hq) for the logarithm of the softmax's sum (-inf for such a row).
+ * Nothing of a token that is not visible enters, whatever its bits. */
+SMLM_API int smlm_paged_attention(const void *q, const void *k_pages, const void *v_pages, int dtype,
+                                  const int64_t *strides, const int32_t *table, int64_t table_stride,
+                                  const int32_t *lengths, int64_t batch, int64_t hq, int64_t hkv, int64_t d,
+                                  int64_t n_pages, int64_t page_size, int64_t max_blocks, float scale, int64_t window,
+                                  int64_t sinks, void *out, float *lse, void *workspace, size_t workspace_bytes,
+                                  int *status, void *stream);
+
+/* The last `tokens` tokens of every sequence from a fused projection: qkv (batch, tokens, (hq + 2 hkv) d), queries,
+ * then keys, then values. Token t of sequence b has position lengths[b] - tokens + t. Queries and keys are turned by
+ * the half-split rotary embedding with cos / sin (fp32, max_pos x d / 2; both NULL: not turned), computed in fp32 and
+ * rounded once; keys and values go to their pages, queries to q_out (batch, tokens, hq, d). A negative position is
+ * padding before a shorter chunk: its queries are 0 and it is not stored. A token whose page is missing sets
+ * SMLM_FLAG_NO_PAGES, a position beyond max_pos SMLM_FLAG_INDEX_RANGE; both are skipped. */
+SMLM_API int smlm_paged_append(const void *qkv, void *k_pages, void *v_pages, int dtype, const int64_t *strides,
+                               const int32_t *table, int64_t table_stride, const int32_t *lengths, int64_t batch,
+                               int64_t tokens, int64_t hq, int64_t hkv, int64_t d, int64_t n_pages, int64_t page_size,
+                               int64_t max_blocks, const float *cos, const float *sin, int64_t max_pos, void *q_out,
+                               int *status, void *stream);
+
+/* ------------------------------------------------------------------------------- pages of a paged cache
+ * No counterpart in the reference. refcount (int32, n_pages): how many table entries hold each page, 0 = free; this
+ * is the whole state of the allocator, and the lowest free page is always taken first. rows, parents, children:
+ * device int32 row numbers; rows listed twice and rows outside the table set SMLM_FLAG_INDEX_RANGE. A sequence of n
+ * tokens has ceil(n / page_size) entries, the later ones of its row being -1 (entries that smlm_pages_trim dropped
+ * are -1 too). */
+
+/* The rows' pages are released, their entries become -1 and their lengths 0. */
+SMLM_API int smlm_pages_free(int32_t *table, int64_t table_stride, int64_t table_rows, int64_t max_blocks,
+                             int32_t *lengths, int32_t *refcount, int64_t n_pages, const int32_t *rows, int64_t n,
+                             int *status, void *stream);
+
+/* The rows' pages that hold only tokens in [sinks, length - window) are released; their entries become -1. */
+SMLM_API int smlm_pages_trim(int32_t *table, int64_t table_stride, int64_t table_rows, int64_t max_blocks,
+                             int32_t *lengths, int32_t *refcount, int64_t n_pages, int64_t page_size,
+                             const int32_t *rows, int64_t n, int64_t window, int64_t sinks, int *status, void *stream);
+
+/* lengths[r] += n_new for every listed row, with new pages where its last page is full. A row whose pages are not
+ * free any more keeps its length (SMLM_FLAG_NO_PAGES), and so does one that the table is too narrow for
+ * (SMLM_FLAG_INDEX_RANGE). At most 65535 rows a call. */
+SMLM_API size_t smlm_pages_extend_workspace(int64_t n, int64_t n_pages);
+SMLM_API int smlm_pages_extend(int32_t *table, int64_t table_stride, int64_t table_rows, int64_t max_blocks,
+                               int32_t *lengths, int32_t *refcount, int64_t n_pages, int64_t page_size,
+                               const int32_t *rows, int64_t n, int64_t n_new, void *workspace, size_t workspace_bytes,
+                               int *status, void *stream);
+
+/* Row children[i] becomes a copy of row parents[i] as it was before the call, for all i at once (a row may be both);
+ * what the children held is released. Whole pages are shared, the tokens of a partly filled last page are copied to a
+ * page of the child's own, in all planes of the pool: pool (planes, n_pages, heads, page_size, token_bytes) with
+ * planes = layers x 2 and token_bytes = the bytes of one head's token (a multiple of 16 up to 4096). children
+ * distinct; at most 65535 pairs. Without a free page for it the child's last entry is -1 (SMLM_FLAG_NO_PAGES). */
+SMLM_API size_t smlm_pages_fork_workspace(int64_t n, int64_t table_rows, int64_t max_blocks, int64_t n_pages);
+SMLM_API int smlm_pages_fork(void *pool, int64_t planes, int64_t heads, int64_t token_bytes, int32_t *table,
+                             int64_t table_stride, int64_t table_rows, int64_t max_blocks, int32_t *lengths,
+                             int32_t *refcount, int64_t n_pages, int64_t page_size, const int32_t *parents,
+                             const int32_t *children, int64_t n, void *workspace, size_t workspace_bytes, int *status,
+                             void *stream);
+
+/* Moves the pages in use to the lowest numbers: with L pages in use, the k-th used page numbered L or above goes to
+ * the k-th free page below L, in the pool, the counts and the table. */
+SMLM_API size_t smlm_pages_compact_workspace(int64_t n_pages);
+SMLM_API int smlm_pages_compact(void *pool, int64_t planes, int64_t heads, int64_t token_bytes, int32_t *table,
+                                int64_t table_stride, int64_t table_rows, int64_t max_blocks, int32_t *refcount,
+                                int64_t n_pages, int64_t page_size, void *workspace, size_t workspace_bytes,
+                                int *status, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,54 @@
+// Shared by the paged key-value cache kernels (paged_attn.cu, pages.cu): the shape of a cache as kernels see it.
+#pragma once
+
+#include "common.cuh"
+
+namespace smlm {
+
+// One layer's pages. Token t of a sequence lies in page table[row][t >> page_shift], slot t & (page - 1); its key of
+// head h starts at k + page * kp + h * kh + slot * kt (64-bit element offsets: a long cache passes 2^31 elements).
+struct PageView {
+    const void* k;
+    const void* v;
+    int64_t kp, kh, kt, vp, vh, vt;
+    const int32_t* table;
+    const int32_t* lengths;
+    int64_t table_stride;
+    int batch, hq, hkv, d, n_pages, page_shift, max_blocks;
+};
+
+// Tokens of row b that the table can hold at all (a length beyond the table is cut and flagged).
+__device__ __forceinline__ int row_length(const PageView& pv, int b, int* status) {
+    const int n = pv.lengths[b];
+    const int64_t cap = (int64_t)pv.max_blocks << pv.page_shift;
+    if (n < 0 || n > cap) {
+        flag(status, SMLM_FLAG_INDEX_RANGE);
+        return n < 0 ? 0 : (int)cap;
+    }
+    return n;
+}
+
+// The page that holds token t of row b, or -1: a hole (entry -1) or an entry outside the pool (flagged).
+__device__ __forceinline__ int page_of(const PageView& pv, int b, int t, int* status) {
+    const int p = __ldg(pv.table + b * pv.table_stride + (t >> pv.page_shift));
+    if (p >= pv.n_pages) {
+        flag(status, SMLM_FLAG_INDEX_RANGE);
+        return -1;
+    }
+    return p < 0 ? -1 : p;
+}
+
+template <typename T>
+__device__ __forceinline__ float widen(T x) {
+    if constexpr (std::is_same_v<T, float>) return x;
+    else if constexpr (std::is_same_v<T, __half>) return __half2float(x);
+    else return __bfloat162float(x);
+}
+template <typename T>
+__device__ __forceinline__ T narrow(float x) {
+    if constexpr (std::is_same_v<T, float>) return x;
+    else if constexpr (std::is_same_v<T, __half>) return __float2half_rn(x);
+    else return __float2bfloat16_rn(x);
+}
+
+}  // namespace smlm

@@ -23,6 +23,7 @@ F32, BF16, F16, Q4 = 0, 1, 2, 3
 I32, I64, I8 = 4, 5, 6
 FLAG_INDEX_RANGE = 1
 FLAG_TIMEOUT = 4
+FLAG_NO_PAGES = 8
 ROWRMS, ROWADAGRAD = 0, 1
 BWD_FIRST_TOUCH_WRITES = 1
 BWD_DEFER_ROWS = 2
@@ -99,6 +100,20 @@ SIGNATURES = {
     "smlm_host_rows_add": (_i32, [_p, _p, _p, _i64, _p, _p, _p, _i64, _i64, _p, _p]),
     "smlm_rows_rowwise_step": (_i32, [_p, _i64, _p, _p, _p, _i64, _i64, _p, _p, _i32, _f32, _f32, _f32, _p, _f32,
                                       _i32, _p, _p]),
+    "smlm_paged_attention_workspace": (_sz, [_i64, _i64, _i64]),
+    "smlm_paged_attention": (_i32, [_p, _p, _p, _i32, _p, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                                    _f32, _i64, _i64, _p, _p, _p, _sz, _p, _p]),
+    "smlm_paged_append": (_i32, [_p, _p, _p, _i32, _p, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                                 _p, _p, _i64, _p, _p, _p]),
+    "smlm_pages_free": (_i32, [_p, _i64, _i64, _i64, _p, _p, _i64, _p, _i64, _p, _p]),
+    "smlm_pages_trim": (_i32, [_p, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _i64, _i64, _p, _p]),
+    "smlm_pages_extend_workspace": (_sz, [_i64, _i64]),
+    "smlm_pages_extend": (_i32, [_p, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _i64, _p, _sz, _p, _p]),
+    "smlm_pages_fork_workspace": (_sz, [_i64, _i64, _i64, _i64]),
+    "smlm_pages_fork": (_i32, [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _i64, _p, _sz,
+                               _p, _p]),
+    "smlm_pages_compact_workspace": (_sz, [_i64]),
+    "smlm_pages_compact": (_i32, [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _p, _sz, _p, _p]),
 }
 
 _LIB = None
@@ -240,5 +255,7 @@ def after(device, what):
     flags = read_status(device)
     if flags & FLAG_TIMEOUT:
         raise RuntimeError(f"{what}: a kernel-internal wait timed out (device status {flags:#x}); outputs invalid")
+    if flags & FLAG_NO_PAGES:
+        raise RuntimeError(f"{what}: the paged cache has no free page (device status {flags:#x})")
     if flags & FLAG_INDEX_RANGE:
         raise IndexError(f"{what}: row index out of range (device status {flags:#x})")

@@ -1,0 +1,213 @@
+"""A paged key-value cache and attention over it (no counterpart in the reference, whose decoding loop concatenates one
+growing cache per layer, smlm/model.py:91-104).
+
+A layer's keys and values lie in pages of `page_size` tokens; a table row lists a sequence's pages in order (-1: none),
+`lengths` counts its tokens, and one reference count per page (0 = free) is the allocator's whole state. All of it is
+on the device, so every function here can be captured in a CUDA graph:
+
+    paged_attention     one new token per sequence over the cache, with a sliding window and first tokens that stay
+                        visible (sinks)
+    paged_append        rotary positions on a fused projection's queries and keys; keys and values into their pages
+    pages_extend / pages_fork / pages_free / pages_trim / pages_compact
+                        the pages of sequences that grow, split into several, end, slide out of a window, and the pool
+                        made dense again
+
+PagedKVCache keeps these tensors together for a model; smlm_b200.decode.PagedDecoder generates with it.
+
+The cache and the activations are fp32, bf16 or fp16, of one type; scores, softmax sums and outputs are accumulated in
+fp32 and rounded once. What a row's table and length do not cover is never used, whatever its bits. Rows of the table
+outside their range, pages outside the pool and an exhausted pool do not fault: the token or row is left out and a flag
+of the device status word is set (SMLM_B200_CHECK=1 turns it into an exception).
+"""
+import ctypes
+
+import torch
+
+from . import _lib as L
+
+
+def _int32(what, t, dim):
+    if t.dtype != torch.int32 or t.dim() != dim or (t.numel() and t.stride(-1) != 1):
+        raise ValueError(f"{what} has to be an int32 tensor of {dim} dimension(s) with contiguous rows")
+
+
+def _cache(what, x, k_pages, v_pages, table, lengths, batch):
+    """Checks a layer's pages against the activations x; returns the cache's common arguments."""
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+        raise ValueError(f"{what}: k_pages and v_pages have to be (pages, key heads, page_size, head dimension)")
+    if x.dtype != k_pages.dtype or x.dtype != v_pages.dtype:
+        raise ValueError(f"{what}: activations and pages have to be of one type, got {x.dtype}, {k_pages.dtype}, "
+                         f"{v_pages.dtype}")
+    if k_pages.stride(3) != 1 or v_pages.stride(3) != 1:
+        raise ValueError(f"{what}: the pages' head dimension has to be contiguous")
+    _int32(f"{what}: table", table, 2)
+    _int32(f"{what}: lengths", lengths, 1)
+    if table.shape[0] != batch or lengths.shape[0] != batch:
+        raise ValueError(f"{what}: {batch} sequences, but a table of {table.shape[0]} rows and {lengths.shape[0]} lengths")
+    strides = (ctypes.c_int64 * 6)(*k_pages.stride()[:3], *v_pages.stride()[:3])
+    return strides
+
+
+def paged_attention(q, k_pages, v_pages, table, lengths, *, scale=None, window=0, sinks=0, return_lse=False):
+    """Attention of one new token per sequence: q (B, query heads, d), k_pages / v_pages (pages, key heads, page_size, d)
+    with any page, head and token strides (multiples of 16 bytes), table (B, blocks) and lengths (B,) int32 -> (B,
+    query heads, d). The newest token is expected in the cache already (paged_append), so lengths counts it.
+
+    Query head i reads key head i // (query heads // key heads). Token j is visible if j < lengths[b] and its table
+    entry is not -1; with window > 0 only the last `window` tokens and the first `sinks` are. scale defaults to
+    d ** -0.5. A row that sees nothing gives 0. return_lse: also the logarithm of the softmax's sum, fp32 (B, query
+    heads), -inf for such a row."""
+    if q.dim() != 3:
+        raise ValueError(f"paged_attention: q has to be (sequences, heads, head dimension), got {tuple(q.shape)}")
+    B, HQ, D = q.shape
+    strides = _cache("paged_attention", q, k_pages, v_pages, table, lengths, B)
+    P, HKV, page, Dk = k_pages.shape
+    if D != Dk or HQ % HKV:
+        raise ValueError(f"paged_attention: {HQ} query heads of {D} over {HKV} key heads of {Dk}")
+    if window < 0 or sinks < 0:
+        raise ValueError(f"paged_attention: window {window}, sinks {sinks}")
+    dev = L.require_cuda(q, k_pages, v_pages, table, lengths)
+    q = q if q.is_contiguous() else q.contiguous()
+    out = torch.empty_like(q)
+    lse = torch.empty(B, HQ, dtype=torch.float32, device=dev) if return_lse else None
+    lib = L.lib()
+    ws = L.workspace(lib.smlm_paged_attention_workspace(B, HQ, D), dev)
+    with L.timed("paged_attention", 1):
+        rc = lib.smlm_paged_attention(L.ptr(q), L.ptr(k_pages), L.ptr(v_pages), L.dtype_code(q.dtype), strides,
+                                      L.ptr(table), table.stride(0), L.ptr(lengths), B, HQ, HKV, D, P, page,
+                                      table.shape[1], D ** -0.5 if scale is None else scale, window, sinks,
+                                      L.ptr(out), L.ptr(lse), L.ptr(ws), ws.numel(), L.status_ptr(dev), L.stream(dev))
+    L.check(rc, "paged_attention")
+    L.after(dev, "paged_attention")
+    return (out, lse) if return_lse else out
+
+
+def paged_append(qkv, k_pages, v_pages, table, lengths, cos=None, sin=None):
+    """The last T tokens of every sequence: qkv (B, T, (query heads + 2 key heads) d), queries, then keys, then values;
+    keys and values are written to their pages (positions lengths[b] - T .. lengths[b] - 1; a negative one is padding
+    before a shorter chunk and is not stored), queries are returned, (B, T, query heads, d). With cos / sin (fp32,
+    (positions, d / 2)) queries and keys are turned by the half-split rotary embedding of their position, in fp32,
+    rounded once."""
+    if qkv.dim() != 3:
+        raise ValueError(f"paged_append: qkv has to be (sequences, tokens, width), got {tuple(qkv.shape)}")
+    B, T, W = qkv.shape
+    strides = _cache("paged_append", qkv, k_pages, v_pages, table, lengths, B)
+    P, HKV, page, D = k_pages.shape
+    HQ = W // D - 2 * HKV
+    if W % D or HQ < 1 or HQ % HKV:
+        raise ValueError(f"paged_append: a projection of {W} values with {HKV} key heads of {D}")
+    max_pos = 0
+    if (cos is None) != (sin is None):
+        raise ValueError("paged_append: cos and sin come together")
+    if cos is not None:
+        for t in (cos, sin):
+            if t.dtype != torch.float32 or t.dim() != 2 or t.shape != cos.shape or 2 * t.shape[1] != D or \
+                    not t.is_contiguous():
+                raise ValueError(f"paged_append: cos and sin have to be contiguous fp32 (positions, {D // 2})")
+        max_pos = cos.shape[0]
+    dev = L.require_cuda(qkv, k_pages, v_pages, table, lengths, cos, sin)
+    qkv = qkv if qkv.is_contiguous() else qkv.contiguous()
+    q = torch.empty(B, T, HQ, D, dtype=qkv.dtype, device=dev)
+    with L.timed("paged_append", 1):
+        rc = L.lib().smlm_paged_append(L.ptr(qkv), L.ptr(k_pages), L.ptr(v_pages), L.dtype_code(qkv.dtype), strides,
+                                       L.ptr(table), table.stride(0), L.ptr(lengths), B, T, HQ, HKV, D, P, page,
+                                       table.shape[1], L.ptr(cos), L.ptr(sin), max_pos, L.ptr(q), L.status_ptr(dev),
+                                       L.stream(dev))
+    L.check(rc, "paged_append")
+    L.after(dev, "paged_append")
+    return q
+
+
+# --------------------------------------------------------------------------------------------- the pages
+def _tables(what, table, lengths, refcount, *rows):
+    _int32(f"{what}: table", table, 2)
+    _int32(f"{what}: reference counts", refcount, 1)
+    for r in rows:
+        _int32(f"{what}: row numbers", r, 1)
+    if lengths is not None:
+        _int32(f"{what}: lengths", lengths, 1)
+        if lengths.shape[0] != table.shape[0]:
+            raise ValueError(f"{what}: {table.shape[0]} table rows, {lengths.shape[0]} lengths")
+    return L.require_cuda(table, lengths, refcount, *rows)
+
+
+def _pool(what, pool, refcount):
+    """(layers, 2, pages, key heads, page_size, d), contiguous -> (planes, heads, bytes of a head's token, page_size)"""
+    if pool.dim() != 6 or pool.shape[1] != 2 or not pool.is_contiguous():
+        raise ValueError(f"{what}: the pool has to be a contiguous (layers, 2, pages, key heads, page_size, head "
+                         f"dimension) tensor, got {tuple(pool.shape)}")
+    if pool.shape[2] != refcount.shape[0]:
+        raise ValueError(f"{what}: {pool.shape[2]} pages, {refcount.shape[0]} reference counts")
+    L.require_cuda(pool, refcount)
+    return 2 * pool.shape[0], pool.shape[3], pool.shape[5] * pool.element_size(), pool.shape[4]
+
+
+def pages_free(table, lengths, refcount, rows):
+    """The sequences `rows` (int32) end: their pages are released, their table entries become -1, their lengths 0."""
+    dev = _tables("pages_free", table, lengths, refcount, rows)
+    with L.timed("pages_free", 1):
+        rc = L.lib().smlm_pages_free(L.ptr(table), table.stride(0), table.shape[0], table.shape[1], L.ptr(lengths),
+                                     L.ptr(refcount), refcount.shape[0], L.ptr(rows), rows.shape[0],
+                                     L.status_ptr(dev), L.stream(dev))
+    L.check(rc, "pages_free")
+    L.after(dev, "pages_free")
+
+
+def pages_trim(table, lengths, refcount, rows, page_size, window, sinks=0):
+    """Releases the pages of the sequences `rows` that paged_attention with this window and these sinks no longer reads:
+    those that hold only tokens in [sinks, length - window)."""
+    dev = _tables("pages_trim", table, lengths, refcount, rows)
+    with L.timed("pages_trim", 1):
+        rc = L.lib().smlm_pages_trim(L.ptr(table), table.stride(0), table.shape[0], table.shape[1], L.ptr(lengths),
+                                     L.ptr(refcount), refcount.shape[0], page_size, L.ptr(rows), rows.shape[0], window,
+                                     sinks, L.status_ptr(dev), L.stream(dev))
+    L.check(rc, "pages_trim")
+    L.after(dev, "pages_trim")
+
+
+def pages_extend(table, lengths, refcount, rows, n_new, page_size):
+    """Every sequence in `rows` grows by n_new tokens: lengths[r] += n_new, with the lowest free pages (row by row) where
+    its last page is full. A sequence that finds too few keeps its length."""
+    dev = _tables("pages_extend", table, lengths, refcount, rows)
+    lib = L.lib()
+    ws = L.workspace(lib.smlm_pages_extend_workspace(rows.shape[0], refcount.shape[0]), dev)
+    with L.timed("pages_extend", 1):
+        rc = lib.smlm_pages_extend(L.ptr(table), table.stride(0), table.shape[0], table.shape[1], L.ptr(lengths),
+                                   L.ptr(refcount), refcount.shape[0], page_size, L.ptr(rows), rows.shape[0], n_new,
+                                   L.ptr(ws), ws.numel(), L.status_ptr(dev), L.stream(dev))
+    L.check(rc, "pages_extend")
+    L.after(dev, "pages_extend")
+
+
+def pages_fork(pool, table, lengths, refcount, parents, children):
+    """Sequence children[i] becomes a copy of sequence parents[i] as it was before the call, for all i at once (a row may
+    be a parent and a child: a beam's reordering); what the children held is released. Whole pages are shared, the
+    tokens of a partly filled last page are copied in all layers. pool: (layers, 2, pages, key heads, page_size, d)."""
+    dev = _tables("pages_fork", table, lengths, refcount, parents, children)
+    planes, heads, token, page = _pool("pages_fork", pool, refcount)
+    if parents.shape != children.shape:
+        raise ValueError(f"pages_fork: {parents.shape[0]} parents, {children.shape[0]} children")
+    lib, n = L.lib(), parents.shape[0]
+    ws = L.workspace(lib.smlm_pages_fork_workspace(n, table.shape[0], table.shape[1], refcount.shape[0]), dev)
+    with L.timed("pages_fork", 2):
+        rc = lib.smlm_pages_fork(L.ptr(pool), planes, heads, token, L.ptr(table), table.stride(0), table.shape[0],
+                                 table.shape[1], L.ptr(lengths), L.ptr(refcount), refcount.shape[0], page,
+                                 L.ptr(parents), L.ptr(children), n, L.ptr(ws), ws.numel(), L.status_ptr(dev),
+                                 L.stream(dev))
+    L.check(rc, "pages_fork")
+    L.after(dev, "pages_fork")
+
+
+def pages_compact(pool, table, refcount):
+    """Moves the pages in use to the lowest numbers, in the pool, the table and the counts: with n in use, the k-th used
+    page numbered n or above goes to the k-th free page below n."""
+    dev = _tables("pages_compact", table, None, refcount)
+    planes, heads, token, page = _pool("pages_compact", pool, refcount)
+    lib = L.lib()
+    ws = L.workspace(lib.smlm_pages_compact_workspace(refcount.shape[0]), dev)
+    with L.timed("pages_compact", 2):
+        rc = lib.smlm_pages_compact(L.ptr(pool), planes, heads, token, L.ptr(table), table.stride(0), table.shape[0],
+                                    table.shape[1], L.ptr(refcount), refcount.shape[0], page, L.ptr(ws), ws.numel(),
+                                    L.status_ptr(dev), L.stream(dev))
+    L.check(rc, "pages_compact")
+    L.after(dev, "pages_compact")
