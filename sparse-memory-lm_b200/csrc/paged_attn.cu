@@ -3,42 +3,531 @@
 
 namespace smlm {
 
-// One warp's share of one (sequence, query head): tokens warp, warp + WARPS, ...; the four warps' running maxima,
-// sums and outputs are joined at the end.
+// ------------------------------------------------------------------------------------------------ attention
+// One query per head against len keys: 4 flops per loaded 16-bit element and head of a group, so the bytes of the
+// keys and values bound it at every group the tensor cores are not needed for, and the kernel is built to keep loads
+// in flight. Each WARP is a worker of its own with no barrier in its loop: it takes tiles of TT tokens straight from
+// global memory into registers with 16-byte loads, in the layout that mma.sync wants:
+//   S^T = K q^T     A = keys (16 tokens x k), B = queries (k x 8): a lane's 16 bytes of token lane / 4 are the A
+//                   fragments of two k-steps, because the order of k is free as long as q's is the same;
+//   O^T += V^T P^T  A = values (16 d x tokens): the 16 bytes of tokens 2t, 2t + 1 are zipped into pairs (prmt) and
+//                   feed d = 8 g + 2 i in row g, 8 g + 2 i + 1 in row g + 8; B = P^T, the transposed scores
+//                   (movmatrix).
+// With queries as the 8 columns, up to 8 query heads of one key head cost the same as one. (mma.sync is enough: the
+// tile of queries is 8 wide, and tcgen05's 128-row tiles would be 1/16 full or less.) Running maxima and sums are
+// fp32, one per column; the weights enter the second product as a sum of two 16-bit values (hi + lo), so they carry
+// 16 bits or more and rounding the output is the only loss that shows.
+// fp32 caches use the same shape with tf32 fragments, each operand split in two and three products kept (2^-21).
+//
+// The tiles of all (sequence, key head, 8 query heads) items form one list, cut evenly over all warps of the grid,
+// whatever the lengths are (they are on the device). An item cut between warps is joined by paged_join_kernel.
+
+constexpr int SPLIT_WARPS = 4, SPLIT_THREADS = SPLIT_WARPS * 32;
+constexpr int QT = 8;  // query heads per item
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint4 load16(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
 template <typename T>
-__global__ void __launch_bounds__(128) paged_attention_kernel(PageView pv, const T* q, float scale, int window,
-                                                              int sinks, T* out, float* lse, int* status) {
-    constexpr int WARPS = 4, PER = 8;  // d <= 256: at most 8 values per lane
-    const int b = blockIdx.y, hq = blockIdx.x, h = hq / (pv.hq / pv.hkv);
-    const int lane = lane_id(), warp = threadIdx.x >> 5;
-    const int n = row_length(pv, b, status);
-    const int first = window ? max(n - window, 0) : 0;
-    float qv[PER], acc[PER];
-#pragma unroll
-    for (int i = 0; i < PER; i++) {
-        const int c = lane + 32 * i;
-        qv[i] = c < pv.d ? widen(q[((int64_t)b * pv.hq + hq) * pv.d + c]) * scale : 0.f;
-        acc[i] = 0.f;
+__device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                      uint32_t b1) {
+    if constexpr (std::is_same_v<T, __half>)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// fp32 operands as tf32 hi + lo: x = hi + lo up to 2^-22 of x. fin is hi without infinities and NaN, for the products
+// with a lo, whose sign and zeros would turn an infinite product into a NaN.
+struct Split32 {
+    uint32_t hi, lo, fin;
+    __device__ __forceinline__ explicit Split32(uint32_t bits) {
+        asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(__uint_as_float(bits)));
+        const bool finite = (hi & 0x7f800000u) != 0x7f800000u;
+        lo = finite ? __float_as_uint(__uint_as_float(bits) - __uint_as_float(hi)) : 0;
+        fin = finite ? hi : 0;
     }
-    float m = -INFINITY, l = 0.f;
-    for (int t = warp; t < n; t += WARPS) {
-        if (t < first && t >= sinks) continue;
-        const int p = page_of(pv, b, t, status);
-        if (p < 0) continue;
-        const int slot = t & ((1 << pv.page_shift) - 1);
-        const T* k = static_cast<const T*>(pv.k) + p * pv.kp + h * pv.kh + slot * pv.kt;
-        const T* v = static_cast<const T*>(pv.v) + p * pv.vp + h * pv.vh + slot * pv.vt;
-        float s = 0.f;
+};
+__device__ __forceinline__ void mma8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                     uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_split32(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                            const Split32& b0, const Split32& b1) {
+    const Split32 x0(a0), x1(a1), x2(a2), x3(a3);
+    mma8(c, x0.lo, x1.lo, x2.lo, x3.lo, b0.fin, b1.fin);
+    mma8(c, x0.fin, x1.fin, x2.fin, x3.fin, b0.lo, b1.lo);
+    mma8(c, x0.hi, x1.hi, x2.hi, x3.hi, b0.hi, b1.hi);
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack16(float x, float y) {  // x in the low half
+    if constexpr (std::is_same_v<T, __half>) {
+        const __half2 h = __floats2half2_rn(x, y);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack16(uint32_t p) {
+    if constexpr (std::is_same_v<T, __half>) return __half22float2(*reinterpret_cast<const __half2*>(&p));
+    else return make_float2(bf16_bits_to_f32(p & 0xffffu), __uint_as_float(p & 0xffff0000u));
+}
+
+// The tiles of one sequence: all of [0, n), or with a window those of the first tokens and of [lo, n).
+struct Span {
+    int n, lo, sinks, head, skip, tiles;  // tiles [0, head) and, skip further on, the rest
+    __device__ __forceinline__ Span(int len, int window, int sink, int tt) : n(len) {
+        lo = window && n > window ? n - window : 0;
+        sinks = min(sink, lo);
+        head = (sinks + tt - 1) / tt;
+        skip = max(lo / tt - head, 0);
+        tiles = (n + tt - 1) / tt - skip;
+    }
+    __device__ __forceinline__ int token(int tile, int tt) const { return (tile < head ? tile : tile + skip) * tt; }
+    __device__ __forceinline__ bool sees(int t) const { return t < n && (t >= lo || t < sinks); }
+};
+
+struct SplitWork {
+    int64_t* base;   // (batch): first tile of each sequence in the list
+    int64_t* per;    // tiles per worker
+    float* m;        // (2 workers, rows): a worker's first and last piece
+    float* l;
+    float* o;        // (2 workers, rows, dp)
+    int rows, dp;    // rows = min(group, QT)
+};
+
+__device__ __forceinline__ int group_tiles(const PageView& pv) { return (pv.hq / pv.hkv + QT - 1) / QT; }
+
+template <typename T, int DP>
+struct SplitShape {
+    static constexpr int ES = sizeof(T);
+    static constexpr int CH = 16 / ES;                   // elements of a 16-byte load
+    static constexpr int TT = ES == 2 && DP <= 64 ? 32 : 16;  // tokens per tile: 64 registers of keys and values
+    static constexpr int NS = TT / 16;
+    static constexpr int KJ = DP / (4 * CH);             // loads per key row and lane
+    static constexpr int VB = DP >= 8 * CH ? DP / (8 * CH) : 1;  // loads per value row and lane
+    static constexpr int MT = ES == 2 ? 4 : 2;           // 16-row tiles of O^T per value load
+    static constexpr bool WIDE = DP * ES > 256;          // queries from shared memory, values loaded after the scores
+    static constexpr int BLOCKS = DP * ES <= 128 ? 4 : DP * ES <= 256 ? 3 : 2;  // resident per SM (registers)
+};
+
+template <typename T, int DP, bool PART>
+__global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP>::BLOCKS)
+    paged_split_kernel(PageView pv, const T* __restrict__ q, float c, int window, int sinks, T* __restrict__ out,
+                       float* __restrict__ lse, SplitWork wk, int* status) {
+    using S = SplitShape<T, DP>;
+    constexpr int CH = S::CH, TT = S::TT, NS = S::NS, KJ = S::KJ, VB = S::VB, MT = S::MT;
+    constexpr bool WIDE = S::WIDE;
+    constexpr bool F = S::ES == 4;
+    __shared__ int64_t pre[SPLIT_THREADS + 1];
+    __shared__ int64_t part[SPLIT_WARPS];
+    __shared__ uint4 qs[WIDE ? SPLIT_WARPS : 1][WIDE ? KJ : 1][WIDE ? 32 : 1];
+    asm volatile("griddepcontrol.launch_dependents;");
+
+    const int lane = lane_id(), warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
+    const int group = pv.hq / pv.hkv, gt = group_tiles(pv), items = pv.hkv * gt;
+
+    // the list's length and this thread's sequences' place in it
+    const int chunk = (pv.batch + SPLIT_THREADS - 1) / SPLIT_THREADS;
+    const int r0 = min(pv.batch, (int)threadIdx.x * chunk), r1 = min(pv.batch, r0 + chunk);
+    int64_t mine = 0;
+    for (int r = r0; r < r1; r++) mine += Span(row_length(pv, r, status), window, sinks, TT).tiles;
+    mine *= items;
+    {
+        int64_t x = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t y = __shfl_up_sync(FULL, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) part[warp] = x;
+        __syncthreads();
+        for (int w = 0; w < warp; w++) x += part[w];
+        pre[threadIdx.x + 1] = x;
+        if (threadIdx.x == 0) pre[0] = 0;
+        __syncthreads();
+    }
+    const int64_t total = pre[SPLIT_THREADS];
+    const int workers = gridDim.x * SPLIT_WARPS;
+    const int64_t per = max((total + workers - 1) / workers, (int64_t)1);
+    if (blockIdx.x == 0) {
+        if (threadIdx.x == 0) *wk.per = per;
+        int64_t x = pre[threadIdx.x];
+        for (int r = r0; r < r1; r++) {
+            wk.base[r] = x;
+            x += (int64_t)items * Span(row_length(pv, r, nullptr), window, sinks, TT).tiles;
+        }
+    }
+    const int worker = warp * gridDim.x + blockIdx.x;  // few tiles: one warp per SM first
+    int64_t left = min(per, total - worker * per);
+    if (left <= 0) return;
+
+    // the sequence, item and tile where this worker starts
+    int b, item, tile;
+    {
+        const int64_t start = worker * per;
+        int a = 0, e = SPLIT_THREADS;  // pre[a] <= start < pre[e]
+        while (e - a > 1) {
+            const int mid = (a + e) >> 1;
+            if (pre[mid] <= start) a = mid;
+            else e = mid;
+        }
+        int64_t off = start - pre[a];
+        b = a * chunk;
+        while (true) {
+            const int r = b + lane;
+            const int64_t w = r < pv.batch ? (int64_t)items * Span(row_length(pv, r, nullptr), window, sinks, TT).tiles
+                                           : 0;
+            int64_t x = w;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t y = __shfl_up_sync(FULL, x, o);
+                if (lane >= o) x += y;
+            }
+            const unsigned beyond = __ballot_sync(FULL, x > off);
+            if (beyond) {
+                const int at = __ffs(beyond) - 1;
+                off -= __shfl_sync(FULL, x - w, at);
+                b += at;
+                break;
+            }
+            off -= __shfl_sync(FULL, x, 31);
+            b += 32;
+        }
+        const int tiles = Span(row_length(pv, b, nullptr), window, sinks, TT).tiles;
+        item = (int)(off / tiles);
+        tile = (int)(off % tiles);
+    }
+
+    const int shift = pv.page_shift, slots = (1 << shift) - 1;
+    while (true) {
+        const Span span(row_length(pv, b, nullptr), window, sinks, TT);
+        if (span.tiles == 0) {  // an empty sequence (paged_join_kernel writes its output)
+            b++;
+            continue;
+        }
+        const int first = tile, last = (int)min((int64_t)span.tiles, tile + left);
+        const int h = item / gt, q0 = item % gt * QT;
+        const int qrow = q0 + g;  // this lane's column of the first product
+        const T* qp = q + ((int64_t)b * pv.hq + h * group) * pv.d;
+        uint4 qf[WIDE ? 1 : KJ];
+#pragma unroll
+        for (int j = 0; j < KJ; j++) {
+            const int d0 = (t4 + 4 * j) * CH;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (qrow < group && (!PART || d0 < pv.d)) v = load16(qp + (int64_t)qrow * pv.d + d0);
+            if constexpr (WIDE) qs[warp][j][lane] = v;
+            else qf[j] = v;
+        }
+        const T* kp = static_cast<const T*>(pv.k) + h * pv.kh;
+        const T* vp = static_cast<const T*>(pv.v) + h * pv.vh;
+        const int32_t* row = pv.table + b * pv.table_stride;
+
+        // the page of token (tile, lane), or -1 if it is not seen
+        auto pages_at = [&](int i) {
+            const int t = span.token(i, TT) + lane;
+            int p = -1;
+            if (lane < TT && span.sees(t)) {
+                p = __ldg(row + (t >> shift));
+                if (p >= pv.n_pages) {
+                    flag(status, SMLM_FLAG_INDEX_RANGE);
+                    p = -1;
+                }
+            }
+            return p;
+        };
+        uint4 kr[NS][2][KJ], vr[NS][4][VB];
+        // rows that are not seen load the query's row instead (any mapped address) and are masked after
+        auto load_keys = [&](int i, int pages) {
+            const int t0 = span.token(i, TT);
+#pragma unroll
+            for (int s = 0; s < NS; s++)
+#pragma unroll
+                for (int r = 0; r < 2; r++) {
+                    const int x = 16 * s + 8 * r + g;
+                    const int p = __shfl_sync(FULL, pages, x);
+                    const T* src = p < 0 ? qp : kp + p * pv.kp + ((t0 + x) & slots) * pv.kt;
+#pragma unroll
+                    for (int j = 0; j < KJ; j++) {
+                        const int d0 = (t4 + 4 * j) * CH;
+                        if (!PART || d0 < pv.d) kr[s][r][j] = load16(src + d0);
+                        else kr[s][r][j] = make_uint4(0, 0, 0, 0);
+                    }
+                }
+        };
+        auto value_token = [&](int s, int r) {  // token of value row r in tile order
+            return 16 * s + (F ? t4 + 4 * r : 2 * t4 + (r & 1) + 8 * (r >> 1));
+        };
+        auto load_values = [&](int i, int pages) {
+            const int t0 = span.token(i, TT);
+#pragma unroll
+            for (int s = 0; s < NS; s++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int x = value_token(s, r);
+                    const int p = __shfl_sync(FULL, pages, x);
+                    const T* src = p < 0 ? qp : vp + p * pv.vp + ((t0 + x) & slots) * pv.vt;
+#pragma unroll
+                    for (int vb = 0; vb < VB; vb++) {
+                        const int d0 = (g + 8 * vb) * CH;
+                        vr[s][r][vb] = load16(src + (d0 < pv.d ? d0 : 0));  // columns past d are not stored
+                    }
+                }
+        };
+
+        float o[VB * MT][4];
+#pragma unroll
+        for (int i = 0; i < VB * MT; i++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) o[i][x] = 0.f;
+        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;  // columns 2 t4, 2 t4 + 1
+
+        int pages = pages_at(first), pages_next = -1;
+        load_keys(first, pages);
+        if (!WIDE) load_values(first, pages);
+        if (first + 1 < last) pages_next = pages_at(first + 1);
+        for (int i = first; i < last; i++) {
+            float sc[NS][4];
+#pragma unroll
+            for (int s = 0; s < NS; s++) {
+                sc[s][0] = sc[s][1] = sc[s][2] = sc[s][3] = 0.f;
+#pragma unroll
+                for (int j = 0; j < KJ; j++) {
+                    const uint4 a = kr[s][0][j], e = kr[s][1][j];
+                    uint4 w;
+                    if constexpr (WIDE) w = qs[warp][j][lane];
+                    else w = qf[j];
+                    if constexpr (F) {
+                        mma_split32(sc[s], a.x, e.x, a.y, e.y, Split32(w.x), Split32(w.y));
+                        mma_split32(sc[s], a.z, e.z, a.w, e.w, Split32(w.z), Split32(w.w));
+                    } else {
+                        mma16<T>(sc[s], a.x, e.x, a.y, e.y, w.x, w.y);
+                        mma16<T>(sc[s], a.z, e.z, a.w, e.w, w.z, w.w);
+                    }
+                }
+            }
+            if (WIDE) load_values(i, pages);
+            const unsigned seen = __ballot_sync(FULL, pages >= 0);
+            if (!WIDE && i + 1 < last) load_keys(i + 1, pages_next);
+            float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+            for (int s = 0; s < NS; s++)
+#pragma unroll
+                for (int r = 0; r < 2; r++) {
+                    const bool on = seen >> (16 * s + 8 * r + g) & 1;
+                    sc[s][2 * r] = on ? sc[s][2 * r] * c : -INFINITY;
+                    sc[s][2 * r + 1] = on ? sc[s][2 * r + 1] * c : -INFINITY;
+                    x0 = fmaxf(x0, sc[s][2 * r]);
+                    x1 = fmaxf(x1, sc[s][2 * r + 1]);
+                }
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) {
+                x0 = fmaxf(x0, __shfl_xor_sync(FULL, x0, w));
+                x1 = fmaxf(x1, __shfl_xor_sync(FULL, x1, w));
+            }
+            if (__any_sync(FULL, x0 > m0 || x1 > m1)) {
+                const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+                const float f0 = m0 == n0 ? 1.f : ex2(m0 - n0), f1 = m1 == n1 ? 1.f : ex2(m1 - n1);
+                m0 = n0;
+                m1 = n1;
+                l0 *= f0;
+                l1 *= f1;
+#pragma unroll
+                for (int x = 0; x < VB * MT; x++) {
+                    o[x][0] *= f0;
+                    o[x][1] *= f1;
+                    o[x][2] *= f0;
+                    o[x][3] *= f1;
+                }
+            }
+            const float z0 = m0 == -INFINITY ? 0.f : m0, z1 = m1 == -INFINITY ? 0.f : m1;
+#pragma unroll
+            for (int s = 0; s < NS; s++)
+#pragma unroll
+                for (int r = 0; r < 2; r++) {
+                    sc[s][2 * r] = ex2(sc[s][2 * r] - z0);
+                    sc[s][2 * r + 1] = ex2(sc[s][2 * r + 1] - z1);
+                    l0 += sc[s][2 * r];
+                    l1 += sc[s][2 * r + 1];
+                }
+            if (seen != (TT == 32 ? FULL : 0xffffu)) {  // 0 * (a stale infinity or NaN) must not reach the sums
+#pragma unroll
+                for (int s = 0; s < NS; s++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        if (!(seen >> value_token(s, r) & 1)) {
+#pragma unroll
+                            for (int vb = 0; vb < VB; vb++) vr[s][r][vb] = make_uint4(0, 0, 0, 0);
+                        }
+            }
+#pragma unroll
+            for (int s = 0; s < NS; s++) {
+                if constexpr (F) {
+#pragma unroll
+                    for (int r = 0; r < 2; r++) {  // tokens 8 r .. 8 r + 7 of the 16
+                        // P^T: weight of token t4 (+ 4) for query g, from lane (token, query / 2)
+                        const int from = 4 * t4 + (g >> 1);
+                        const float a = __shfl_sync(FULL, sc[s][2 * r], from);
+                        const float b1 = __shfl_sync(FULL, sc[s][2 * r + 1], from);
+                        const float a4 = __shfl_sync(FULL, sc[s][2 * r], from + 16);
+                        const float b4 = __shfl_sync(FULL, sc[s][2 * r + 1], from + 16);
+                        const Split32 p0(__float_as_uint(g & 1 ? b1 : a)), p1(__float_as_uint(g & 1 ? b4 : a4));
+#pragma unroll
+                        for (int vb = 0; vb < VB; vb++) {
+                            const uint4 x = vr[s][2 * r][vb], y = vr[s][2 * r + 1][vb];
+                            mma_split32(o[vb * MT], x.x, x.y, y.x, y.y, p0, p1);
+                            mma_split32(o[vb * MT + 1], x.z, x.w, y.z, y.w, p0, p1);
+                        }
+                    }
+                } else {
+                    const uint32_t h0 = pack16<T>(sc[s][0], sc[s][1]), h1 = pack16<T>(sc[s][2], sc[s][3]);
+                    const float2 u0 = unpack16<T>(h0), u1 = unpack16<T>(h1);
+                    const uint32_t e0 = transpose8x8(pack16<T>(sc[s][0] - u0.x, sc[s][1] - u0.y));
+                    const uint32_t e1 = transpose8x8(pack16<T>(sc[s][2] - u1.x, sc[s][3] - u1.y));
+                    const uint32_t p0 = transpose8x8(h0), p1 = transpose8x8(h1);
+#pragma unroll
+                    for (int vb = 0; vb < VB; vb++) {
+                        const uint4 x = vr[s][0][vb], y = vr[s][1][vb], z = vr[s][2][vb], w = vr[s][3][vb];
+                        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+                        const uint32_t zs[4] = {z.x, z.y, z.z, z.w}, ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const uint32_t a0 = __byte_perm(xs[k], ys[k], 0x5410);
+                            const uint32_t a1 = __byte_perm(xs[k], ys[k], 0x7632);
+                            const uint32_t a2 = __byte_perm(zs[k], ws[k], 0x5410);
+                            const uint32_t a3 = __byte_perm(zs[k], ws[k], 0x7632);
+                            mma16<T>(o[vb * MT + k], a0, a1, a2, a3, e0, e1);
+                            mma16<T>(o[vb * MT + k], a0, a1, a2, a3, p0, p1);
+                        }
+                    }
+                }
+            }
+            if (i + 1 < last) {
+                if (WIDE) load_keys(i + 1, pages_next);
+                else load_values(i + 1, pages_next);
+                pages = pages_next;
+                pages_next = i + 2 < last ? pages_at(i + 2) : -1;
+            }
+        }
+#pragma unroll
+        for (int w = 4; w < 32; w <<= 1) {
+            l0 += __shfl_xor_sync(FULL, l0, w);
+            l1 += __shfl_xor_sync(FULL, l1, w);
+        }
+        // columns 2 t4 (x = 0) and 2 t4 + 1: this lane has values CH (g + 8 vb) .. + CH - 1 of them
+        const bool whole = first == 0 && last == span.tiles;
+        const int64_t slot = 2 * (int64_t)worker + (first == 0);
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            const int col = 2 * t4 + x;
+            if (q0 + col >= group) continue;
+            const float l = x ? l1 : l0, m = x ? m1 : m0;
+            const int64_t head = (int64_t)b * pv.hq + h * group + q0 + col;
+            const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+            if (g == 0) {
+                if (whole) {
+                    if (lse) lse[head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
+                } else {
+                    wk.m[slot * wk.rows + col] = m;
+                    wk.l[slot * wk.rows + col] = l;
+                }
+            }
+#pragma unroll
+            for (int vb = 0; vb < VB; vb++) {
+                const int d0 = (g + 8 * vb) * CH;
+                if (d0 >= pv.d) continue;
+                float v[CH];
+#pragma unroll
+                for (int k = 0; k < MT; k++) {
+                    v[2 * k] = o[vb * MT + k][x] * inv;
+                    v[2 * k + 1] = o[vb * MT + k][2 + x] * inv;
+                }
+                if (whole) {
+                    uint4 w;
+                    if constexpr (F)
+                        w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
+                                       __float_as_uint(v[3]));
+                    else
+                        w = make_uint4(pack16<T>(v[0], v[1]), pack16<T>(v[2], v[3]), pack16<T>(v[4], v[5]),
+                                       pack16<T>(v[6], v[7]));
+                    *reinterpret_cast<uint4*>(out + head * pv.d + d0) = w;
+                } else {
+                    float* dst = wk.o + (slot * wk.rows + col) * wk.dp + d0;
+#pragma unroll
+                    for (int k = 0; k < CH; k += 4)
+                        *reinterpret_cast<float4*>(dst + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                }
+            }
+        }
+        left -= last - first;
+        if (left == 0) return;
+        tile = 0;
+        if (++item == items) {
+            item = 0;
+            b++;
+        }
+    }
+}
+
+// One block per (query head, sequence): the pieces of an item that was cut, in the order of the tokens, each scaled
+// to the largest maximum (the same sums in the same order on every run); rows that see nothing become 0.
+template <typename T, int TT>
+__global__ void __launch_bounds__(128) paged_join_kernel(PageView pv, int window, int sinks, T* __restrict__ out,
+                                                         float* __restrict__ lse, SplitWork wk) {
+    constexpr int WARPS = 4, PER = 8;  // d <= 256: at most 8 values per lane
+    const int lane = lane_id(), warp = threadIdx.x >> 5, hq = blockIdx.x, b = blockIdx.y;
+    const int group = pv.hq / pv.hkv, gt = group_tiles(pv), qi = hq % group;
+    const int tiles = Span(row_length(pv, b, nullptr), window, sinks, TT).tiles;
+    const int64_t head = (int64_t)b * pv.hq + hq;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (tiles == 0) {
+        for (int x = threadIdx.x; x < pv.d; x += 128) out[head * pv.d + x] = narrow<T>(0.f);
+        if (lse && threadIdx.x == 0) lse[head] = -INFINITY;
+        return;
+    }
+    const int64_t per = *wk.per, at = wk.base[b] + (int64_t)(hq / group * gt + qi / QT) * tiles;
+    const int64_t w0 = at / per, w1 = (at + tiles - 1) / per;
+    if (w0 == w1) return;
+    float m = -INFINITY, l = 0.f, acc[PER];
+#pragma unroll
+    for (int i = 0; i < PER; i++) acc[i] = 0.f;
+    for (int64_t w = w0 + warp; w <= w1; w += WARPS) {
+        const int64_t r = (2 * w + (w == w0)) * wk.rows + qi % QT;
+        const float pm = wk.m[r], pl = wk.l[r];
+        const float mn = fmaxf(m, pm), base = mn == -INFINITY ? 0.f : mn;
+        const float a = ex2(m - base), e = ex2(pm - base);
+        l = l * a + pl * e;
 #pragma unroll
         for (int i = 0; i < PER; i++)
-            if (lane + 32 * i < pv.d) s += qv[i] * widen(k[lane + 32 * i]);
-        s = warp_sum(s);
-        const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.f : mn;
-        const float c = expf(m - base), e = expf(s - base);
-        l = l * c + e;
-#pragma unroll
-        for (int i = 0; i < PER; i++)
-            if (lane + 32 * i < pv.d) acc[i] = acc[i] * c + e * widen(v[lane + 32 * i]);
+            if (lane + 32 * i < pv.d) acc[i] = acc[i] * a + wk.o[r * wk.dp + lane + 32 * i] * e;
         m = mn;
     }
     __shared__ float sm[WARPS], sl[WARPS], so[WARPS][256];
@@ -52,13 +541,14 @@ __global__ void __launch_bounds__(128) paged_attention_kernel(PageView pv, const
     float mx = -INFINITY, sum = 0.f;
     for (int w = 0; w < WARPS; w++) mx = fmaxf(mx, sm[w]);
     const float base = mx == -INFINITY ? 0.f : mx;
-    for (int w = 0; w < WARPS; w++) sum += sl[w] * expf(sm[w] - base);
-    for (int c = threadIdx.x; c < pv.d; c += 128) {
-        float o = 0.f;
-        for (int w = 0; w < WARPS; w++) o += so[w][c] * expf(sm[w] - base);
-        out[((int64_t)b * pv.hq + hq) * pv.d + c] = narrow<T>(sum == 0.f ? 0.f : o / sum);
+    for (int w = 0; w < WARPS; w++) sum += sl[w] * ex2(sm[w] - base);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    for (int x = threadIdx.x; x < pv.d; x += 128) {
+        float v = 0.f;
+        for (int w = 0; w < WARPS; w++) v += so[w][x] * ex2(sm[w] - base);
+        out[head * pv.d + x] = narrow<T>(v * inv);
     }
-    if (lse && threadIdx.x == 0) lse[(int64_t)b * pv.hq + hq] = sum == 0.f ? -INFINITY : mx + logf(sum);
+    if (lse && threadIdx.x == 0) lse[head] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * 0.69314718055994530942f;
 }
 
 // Rotary positions on the queries and keys of a fused projection, keys and values into their pages. One thread per
@@ -147,11 +637,76 @@ static int by_dtype(int dtype, F f) {
     return f(__nv_bfloat16());
 }
 
+static int split_blocks(int64_t es, int64_t dp) { return es * dp <= 128 ? 4 : es * dp <= 256 ? 3 : 2; }
+static int64_t padded_d(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+
+// Carves the workspace (sizes only without one).
+template <typename W>
+static void split_work(W& ws, SplitWork& wk, int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t es) {
+    const int64_t dp = padded_d(d), slots = 2 * (int64_t)sm_count() * split_blocks(es, dp) * SPLIT_WARPS;
+    wk.rows = (int)std::min<int64_t>(hq / std::max<int64_t>(hkv, 1), QT);
+    wk.dp = (int)dp;
+    if constexpr (std::is_same_v<W, Workspace>) {
+        wk.base = ws.template take<int64_t>(batch);
+        wk.per = ws.template take<int64_t>(1);
+        wk.m = ws.template take<float>(slots * wk.rows);
+        wk.l = ws.template take<float>(slots * wk.rows);
+        wk.o = ws.template take<float>(slots * wk.rows * dp);
+    } else {
+        ws.template take<int64_t>(batch);
+        ws.template take<int64_t>(1);
+        ws.template take<float>(slots * wk.rows);
+        ws.template take<float>(slots * wk.rows);
+        ws.template take<float>(slots * wk.rows * dp);
+    }
+}
+
+template <typename T, int DP, bool PART>
+static int launch_split(const PageView& pv, const void* q, float scale, int window, int sinks, void* out, float* lse,
+                        const SplitWork& wk, int* status, cudaStream_t st) {
+    using S = SplitShape<T, DP>;
+    paged_split_kernel<T, DP, PART><<<sm_count() * S::BLOCKS, SPLIT_THREADS, 0, st>>>(
+        pv, static_cast<const T*>(q), scale * 1.4426950408889634074f, window, sinks, static_cast<T*>(out), lse, wk,
+        status);
+    SMLM_LAUNCHED("paged_attention");
+    // launched while the first kernel still runs; it waits for that kernel's end itself
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(pv.hq, pv.batch);
+    cfg.blockDim = dim3(128);
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    SMLM_CUDA(cudaLaunchKernelEx(&cfg, paged_join_kernel<T, S::TT>, pv, window, sinks, static_cast<T*>(out), lse, wk));
+    return SMLM_OK;
+}
+
+template <typename T>
+static int launch_attention(const PageView& pv, const void* q, float scale, int window, int sinks, void* out,
+                            float* lse, const SplitWork& wk, int* status, cudaStream_t st) {
+    const auto go = [&](auto dp) {
+        constexpr int DP = decltype(dp)::value;
+        return pv.d == DP ? launch_split<T, DP, false>(pv, q, scale, window, sinks, out, lse, wk, status, st)
+                          : launch_split<T, DP, true>(pv, q, scale, window, sinks, out, lse, wk, status, st);
+    };
+    if (pv.d <= 32) return go(std::integral_constant<int, 32>());
+    if (pv.d <= 64) return go(std::integral_constant<int, 64>());
+    if (pv.d <= 128) return go(std::integral_constant<int, 128>());
+    return go(std::integral_constant<int, 256>());
+}
+
 }  // namespace smlm
 
 using namespace smlm;
 
-extern "C" size_t smlm_paged_attention_workspace(int64_t batch, int64_t hq, int64_t d) { return 0; }
+extern "C" size_t smlm_paged_attention_workspace(int64_t batch, int64_t hq, int64_t hkv, int64_t d, int dtype) {
+    WorkspaceSize ws;
+    SplitWork wk;
+    split_work(ws, wk, std::max<int64_t>(batch, 0), hq, hkv, d, element_bytes(dtype));
+    return ws.used;
+}
 
 extern "C" int smlm_paged_attention(const void* q, const void* k_pages, const void* v_pages, int dtype,
                                     const int64_t* strides, const int32_t* table, int64_t table_stride,
@@ -168,13 +723,16 @@ extern "C" int smlm_paged_attention(const void* q, const void* k_pages, const vo
                    "paged_attention: q and out have to be 16-byte aligned");
     SMLM_CHECK_ARG(window >= 0 && sinks >= 0, "paged_attention: window %lld, sinks %lld", (long long)window,
                    (long long)sinks);
-    const int win = (int)std::min<int64_t>(window, INT32_MAX), snk = (int)std::min<int64_t>(sinks, INT32_MAX);
+    const int win = (int)std::min<int64_t>(window, INT32_MAX), snk = (int)std::min<int64_t>(sinks, INT32_MAX / 2);
+    Workspace ws(workspace, workspace_bytes);
+    SplitWork wk;
+    split_work(ws, wk, batch, hq, hkv, d, element_bytes(dtype));
+    if (!workspace || !ws.ok()) {
+        set_error("paged_attention: workspace of %zu bytes, %zu needed", workspace_bytes, ws.used);
+        return SMLM_ERR_WORKSPACE;
+    }
     return by_dtype(dtype, [&](auto t) {
-        using T = decltype(t);
-        paged_attention_kernel<T><<<dim3(hq, batch), 128, 0, as_stream(stream)>>>(
-            pv, static_cast<const T*>(q), scale, win, snk, static_cast<T*>(out), lse, status);
-        SMLM_LAUNCHED("paged_attention");
-        return SMLM_OK;
+        return launch_attention<decltype(t)>(pv, q, scale, win, snk, out, lse, wk, status, as_stream(stream));
     });
 }
 

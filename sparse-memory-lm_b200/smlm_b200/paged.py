@@ -71,8 +71,8 @@ def paged_attention(q, k_pages, v_pages, table, lengths, *, scale=None, window=0
     out = torch.empty_like(q)
     lse = torch.empty(B, HQ, dtype=torch.float32, device=dev) if return_lse else None
     lib = L.lib()
-    ws = L.workspace(lib.smlm_paged_attention_workspace(B, HQ, D), dev)
-    with L.timed("paged_attention", 1):
+    ws = L.workspace(lib.smlm_paged_attention_workspace(B, HQ, HKV, D, L.dtype_code(q.dtype)), dev)
+    with L.timed("paged_attention", 2):
         rc = lib.smlm_paged_attention(L.ptr(q), L.ptr(k_pages), L.ptr(v_pages), L.dtype_code(q.dtype), strides,
                                       L.ptr(table), table.stride(0), L.ptr(lengths), B, HQ, HKV, D, P, page,
                                       table.shape[1], D ** -0.5 if scale is None else scale, window, sinks,
