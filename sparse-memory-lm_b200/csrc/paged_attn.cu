@@ -23,6 +23,7 @@ namespace smlm {
 // whatever the lengths are (they are on the device). An item cut between warps is joined by paged_join_kernel.
 
 constexpr int SPLIT_WARPS = 4, SPLIT_THREADS = SPLIT_WARPS * 32;
+constexpr int JOIN_THREADS = 256;
 constexpr int QT = 8;  // query heads per item
 
 __device__ __forceinline__ float ex2(float x) {
@@ -115,9 +116,28 @@ struct Span {
     __device__ __forceinline__ bool sees(int t) const { return t < n && (t >= lo || t < sinks); }
 };
 
+// The list of `total` tiles cut into `workers` pieces: the first `extra` of `per` + 1 tiles, the others of `per`.
+struct Cut {
+    int64_t per, extra;
+    __device__ __forceinline__ Cut(int64_t total, int workers) {
+        if (total >> 31) {
+            per = total / workers;
+            extra = total % workers;
+        } else {  // 32-bit division is several times shorter
+            per = (uint32_t)total / (uint32_t)workers;
+            extra = (uint32_t)total % (uint32_t)workers;
+        }
+    }
+    __device__ __forceinline__ int64_t start(int64_t w) const { return w * per + min(w, extra); }
+    __device__ __forceinline__ int64_t worker_of(int64_t tile) const {
+        const int64_t wide = extra * (per + 1);
+        return tile < wide ? tile / (per + 1) : extra + (tile - wide) / per;
+    }
+};
+
 struct SplitWork {
     int64_t* base;   // (batch): first tile of each sequence in the list
-    int64_t* per;    // tiles per worker
+    int64_t* total;  // tiles of all
     float* m;        // (2 workers, rows): a worker's first and last piece
     float* l;
     float* o;        // (2 workers, rows, dp)
@@ -139,7 +159,8 @@ struct SplitShape {
     static constexpr int BLOCKS = DP * ES <= 128 ? 4 : DP * ES <= 256 ? 3 : 2;  // resident per SM (registers)
 };
 
-template <typename T, int DP, bool PART>
+// SMALL: pages of fewer than 16 tokens, whose tokens are looked up one by one (PART: d < DP).
+template <typename T, int DP, bool PART, bool SMALL>
 __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP>::BLOCKS)
     paged_split_kernel(PageView pv, const T* __restrict__ q, float c, int window, int sinks, T* __restrict__ out,
                        float* __restrict__ lse, SplitWork wk, int* status) {
@@ -147,6 +168,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP>::BLOCKS)
     constexpr int CH = S::CH, TT = S::TT, NS = S::NS, KJ = S::KJ, VB = S::VB, MT = S::MT;
     constexpr bool WIDE = S::WIDE;
     constexpr bool F = S::ES == 4;
+    constexpr unsigned ALL = TT == 32 ? FULL : 0xffffu;
     __shared__ int64_t pre[SPLIT_THREADS + 1];
     __shared__ int64_t part[SPLIT_WARPS];
     __shared__ uint4 qs[WIDE ? SPLIT_WARPS : 1][WIDE ? KJ : 1][WIDE ? 32 : 1];
@@ -176,10 +198,9 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP>::BLOCKS)
         __syncthreads();
     }
     const int64_t total = pre[SPLIT_THREADS];
-    const int workers = gridDim.x * SPLIT_WARPS;
-    const int64_t per = max((total + workers - 1) / workers, (int64_t)1);
+    const Cut cut(total, gridDim.x * SPLIT_WARPS);
     if (blockIdx.x == 0) {
-        if (threadIdx.x == 0) *wk.per = per;
+        if (threadIdx.x == 0) *wk.total = total;
         int64_t x = pre[threadIdx.x];
         for (int r = r0; r < r1; r++) {
             wk.base[r] = x;
@@ -187,13 +208,13 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP>::BLOCKS)
         }
     }
     const int worker = warp * gridDim.x + blockIdx.x;  // few tiles: one warp per SM first
-    int64_t left = min(per, total - worker * per);
+    int64_t left = cut.per + (worker < cut.extra);
     if (left <= 0) return;
 
     // the sequence, item and tile where this worker starts
     int b, item, tile;
     {
-        const int64_t start = worker * per;
+        const int64_t start = cut.start(worker);
         int a = 0, e = SPLIT_THREADS;  // pre[a] <= start < pre[e]
         while (e - a > 1) {
             const int mid = (a + e) >> 1;
@@ -202,32 +223,40 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP>::BLOCKS)
         }
         int64_t off = start - pre[a];
         b = a * chunk;
-        while (true) {
-            const int r = b + lane;
-            const int64_t w = r < pv.batch ? (int64_t)items * Span(row_length(pv, r, nullptr), window, sinks, TT).tiles
-                                           : 0;
-            int64_t x = w;
+        if (chunk > 1) {
+            while (true) {
+                const int r = b + lane;
+                const int64_t w =
+                    r < pv.batch ? (int64_t)items * Span(row_length(pv, r, nullptr), window, sinks, TT).tiles : 0;
+                int64_t x = w;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int64_t y = __shfl_up_sync(FULL, x, o);
-                if (lane >= o) x += y;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int64_t y = __shfl_up_sync(FULL, x, o);
+                    if (lane >= o) x += y;
+                }
+                const unsigned beyond = __ballot_sync(FULL, x > off);
+                if (beyond) {
+                    const int at = __ffs(beyond) - 1;
+                    off -= __shfl_sync(FULL, x - w, at);
+                    b += at;
+                    break;
+                }
+                off -= __shfl_sync(FULL, x, 31);
+                b += 32;
             }
-            const unsigned beyond = __ballot_sync(FULL, x > off);
-            if (beyond) {
-                const int at = __ffs(beyond) - 1;
-                off -= __shfl_sync(FULL, x - w, at);
-                b += at;
-                break;
-            }
-            off -= __shfl_sync(FULL, x, 31);
-            b += 32;
         }
         const int tiles = Span(row_length(pv, b, nullptr), window, sinks, TT).tiles;
-        item = (int)(off / tiles);
-        tile = (int)(off % tiles);
+        if (off >> 31) {
+            item = (int)(off / tiles);
+            tile = (int)(off % tiles);
+        } else {
+            item = (uint32_t)off / (uint32_t)tiles;
+            tile = (uint32_t)off % (uint32_t)tiles;
+        }
     }
 
     const int shift = pv.page_shift, slots = (1 << shift) - 1;
+    const uint32_t kpb = pv.kp * S::ES, ktb = pv.kt * S::ES, vpb = pv.vp * S::ES, vtb = pv.vt * S::ES;  // bytes
     while (true) {
         const Span span(row_length(pv, b, nullptr), window, sinks, TT);
         if (span.tiles == 0) {  // an empty sequence (paged_join_kernel writes its output)
@@ -236,6 +265,48 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP>::BLOCKS)
         }
         const int first = tile, last = (int)min((int64_t)span.tiles, tile + left);
         const int h = item / gt, q0 = item % gt * QT;
+        const int32_t* row = pv.table + b * pv.table_stride;
+        auto entry = [&](int t) {  // the page of token t, or -1 past the end, in a hole or outside the pool
+            int p = -1;
+            if (t < span.n) {
+                p = __ldg(row + (t >> shift));
+                if (p >= pv.n_pages) {
+                    flag(status, SMLM_FLAG_INDEX_RANGE);
+                    p = -1;
+                }
+            }
+            return p;
+        };
+        // the pages of a tile: SMALL: of token `lane`; else of each 16 tokens (the same in all lanes)
+        struct PagesOf {
+            int p[SMALL ? 1 : NS];
+        };
+        auto pages_at = [&](int i) {
+            const int t0 = span.token(i, TT);
+            PagesOf x;
+            if constexpr (SMALL) {
+                x.p[0] = lane < TT ? entry(t0 + lane) : -1;
+            } else {
+#pragma unroll
+                for (int s = 0; s < NS; s++) x.p[s] = entry(t0 + 16 * s);
+            }
+            return x;
+        };
+        // which of the tile's tokens are seen
+        auto seen_of = [&](int i, const PagesOf& x) {
+            const int t0 = span.token(i, TT);
+            bool whole = t0 + TT <= span.n && (t0 >= span.lo || t0 + TT <= span.sinks);
+            if constexpr (!SMALL) {
+#pragma unroll
+                for (int s = 0; s < NS; s++) whole = whole && x.p[s] >= 0;
+                if (whole) return ALL;
+                const int p = lane < 16 ? x.p[0] : x.p[NS - 1];
+                return __ballot_sync(FULL, lane < TT && p >= 0 && span.sees(t0 + lane));
+            } else {
+                return __ballot_sync(FULL, x.p[0] >= 0 && span.sees(t0 + lane));
+            }
+        };
+        PagesOf pages = pages_at(first), pages_next;
         const int qrow = q0 + g;  // this lane's column of the first product
         const T* qp = q + ((int64_t)b * pv.hq + h * group) * pv.d;
         uint4 qf[WIDE ? 1 : KJ];
@@ -247,60 +318,65 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP>::BLOCKS)
             if constexpr (WIDE) qs[warp][j][lane] = v;
             else qf[j] = v;
         }
-        const T* kp = static_cast<const T*>(pv.k) + h * pv.kh;
-        const T* vp = static_cast<const T*>(pv.v) + h * pv.vh;
-        const int32_t* row = pv.table + b * pv.table_stride;
-
-        // the page of token (tile, lane), or -1 if it is not seen
-        auto pages_at = [&](int i) {
-            const int t = span.token(i, TT) + lane;
-            int p = -1;
-            if (lane < TT && span.sees(t)) {
-                p = __ldg(row + (t >> shift));
-                if (p >= pv.n_pages) {
-                    flag(status, SMLM_FLAG_INDEX_RANGE);
-                    p = -1;
-                }
-            }
-            return p;
-        };
+        const char* kp = reinterpret_cast<const char*>(static_cast<const T*>(pv.k) + h * pv.kh + t4 * CH);
+        const char* vp = reinterpret_cast<const char*>(static_cast<const T*>(pv.v) + h * pv.vh);
         uint4 kr[NS][2][KJ], vr[NS][4][VB];
-        // rows that are not seen load the query's row instead (any mapped address) and are masked after
-        auto load_keys = [&](int i, int pages) {
+        // Tokens that are not seen are loaded all the same, from their own page or page 0 (mapped memory), and masked.
+        auto load_keys = [&](int i, const PagesOf& x) {
             const int t0 = span.token(i, TT);
 #pragma unroll
-            for (int s = 0; s < NS; s++)
+            for (int s = 0; s < NS; s++) {
+                const char* base = kp;
+                if constexpr (!SMALL)
+                    base += (uint64_t)(uint32_t)max(x.p[s], 0) * kpb + (uint64_t)(uint32_t)((t0 + 16 * s) & slots) * ktb +
+                            (uint64_t)(uint32_t)g * ktb;
 #pragma unroll
                 for (int r = 0; r < 2; r++) {
-                    const int x = 16 * s + 8 * r + g;
-                    const int p = __shfl_sync(FULL, pages, x);
-                    const T* src = p < 0 ? qp : kp + p * pv.kp + ((t0 + x) & slots) * pv.kt;
+                    const char* src;
+                    if constexpr (SMALL) {
+                        const int y = 16 * s + 8 * r + g;
+                        const int p = max(__shfl_sync(FULL, x.p[0], y), 0);
+                        src = kp + (uint64_t)(uint32_t)p * kpb + (uint64_t)(uint32_t)((t0 + y) & slots) * ktb;
+                    } else {
+                        src = base + (uint64_t)(8 * r) * ktb;
+                    }
 #pragma unroll
                     for (int j = 0; j < KJ; j++) {
-                        const int d0 = (t4 + 4 * j) * CH;
-                        if (!PART || d0 < pv.d) kr[s][r][j] = load16(src + d0);
+                        if (!PART || (t4 + 4 * j) * CH < pv.d) kr[s][r][j] = load16(src + 64 * j);
                         else kr[s][r][j] = make_uint4(0, 0, 0, 0);
                     }
                 }
+            }
         };
         auto value_token = [&](int s, int r) {  // token of value row r in tile order
             return 16 * s + (F ? t4 + 4 * r : 2 * t4 + (r & 1) + 8 * (r >> 1));
         };
-        auto load_values = [&](int i, int pages) {
+        auto load_values = [&](int i, const PagesOf& x) {
             const int t0 = span.token(i, TT);
 #pragma unroll
-            for (int s = 0; s < NS; s++)
+            for (int s = 0; s < NS; s++) {
+                const char* base = vp;
+                if constexpr (!SMALL)
+                    base += (uint64_t)(uint32_t)max(x.p[s], 0) * vpb + (uint64_t)(uint32_t)((t0 + 16 * s) & slots) * vtb +
+                            (uint64_t)(uint32_t)(F ? t4 : 2 * t4) * vtb;
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const int x = value_token(s, r);
-                    const int p = __shfl_sync(FULL, pages, x);
-                    const T* src = p < 0 ? qp : vp + p * pv.vp + ((t0 + x) & slots) * pv.vt;
+                    const char* src;
+                    if constexpr (SMALL) {
+                        const int y = value_token(s, r);
+                        const int p = max(__shfl_sync(FULL, x.p[0], y), 0);
+                        src = vp + (uint64_t)(uint32_t)p * vpb + (uint64_t)(uint32_t)((t0 + y) & slots) * vtb;
+                    } else {
+                        src = base + (uint64_t)(F ? 4 * r : (r & 1) + 8 * (r >> 1)) * vtb;
+                    }
 #pragma unroll
                     for (int vb = 0; vb < VB; vb++) {
-                        const int d0 = (g + 8 * vb) * CH;
-                        vr[s][r][vb] = load16(src + (d0 < pv.d ? d0 : 0));  // columns past d are not stored
+                        const int d0 = (g + 8 * vb) * CH;  // columns past d are not stored
+                        const bool in = (!PART && DP >= 8 * CH) || d0 < pv.d;
+                        vr[s][r][vb] = load16(src + (in ? 16 * g + 128 * vb : 0));
                     }
                 }
+            }
         };
 
         float o[VB * MT][4];
@@ -310,7 +386,6 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP>::BLOCKS)
             for (int x = 0; x < 4; x++) o[i][x] = 0.f;
         float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;  // columns 2 t4, 2 t4 + 1
 
-        int pages = pages_at(first), pages_next = -1;
         load_keys(first, pages);
         if (!WIDE) load_values(first, pages);
         if (first + 1 < last) pages_next = pages_at(first + 1);
@@ -335,16 +410,31 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP>::BLOCKS)
                 }
             }
             if (WIDE) load_values(i, pages);
-            const unsigned seen = __ballot_sync(FULL, pages >= 0);
+            const unsigned seen = seen_of(i, pages);
             if (!WIDE && i + 1 < last) load_keys(i + 1, pages_next);
+#pragma unroll
+            for (int s = 0; s < NS; s++)
+#pragma unroll
+                for (int x = 0; x < 4; x++) sc[s][x] *= c;
+            if (seen != ALL) {  // 0 * (a stale infinity or NaN) must not reach the sums either
+#pragma unroll
+                for (int s = 0; s < NS; s++) {
+#pragma unroll
+                    for (int r = 0; r < 2; r++)
+                        if (!(seen >> (16 * s + 8 * r + g) & 1)) sc[s][2 * r] = sc[s][2 * r + 1] = -INFINITY;
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        if (!WIDE && !(seen >> value_token(s, r) & 1)) {
+#pragma unroll
+                            for (int vb = 0; vb < VB; vb++) vr[s][r][vb] = make_uint4(0, 0, 0, 0);
+                        }
+                }
+            }
             float x0 = -INFINITY, x1 = -INFINITY;
 #pragma unroll
             for (int s = 0; s < NS; s++)
 #pragma unroll
                 for (int r = 0; r < 2; r++) {
-                    const bool on = seen >> (16 * s + 8 * r + g) & 1;
-                    sc[s][2 * r] = on ? sc[s][2 * r] * c : -INFINITY;
-                    sc[s][2 * r + 1] = on ? sc[s][2 * r + 1] * c : -INFINITY;
                     x0 = fmaxf(x0, sc[s][2 * r]);
                     x1 = fmaxf(x1, sc[s][2 * r + 1]);
                 }
@@ -378,7 +468,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP>::BLOCKS)
                     l0 += sc[s][2 * r];
                     l1 += sc[s][2 * r + 1];
                 }
-            if (seen != (TT == 32 ? FULL : 0xffffu)) {  // 0 * (a stale infinity or NaN) must not reach the sums
+            if (WIDE && seen != ALL) {
 #pragma unroll
                 for (int s = 0; s < NS; s++)
 #pragma unroll
@@ -434,7 +524,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP>::BLOCKS)
                 if (WIDE) load_keys(i + 1, pages_next);
                 else load_values(i + 1, pages_next);
                 pages = pages_next;
-                pages_next = i + 2 < last ? pages_at(i + 2) : -1;
+                if (i + 2 < last) pages_next = pages_at(i + 2);
             }
         }
 #pragma unroll
@@ -497,37 +587,56 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP>::BLOCKS)
     }
 }
 
-// One block per (query head, sequence): the pieces of an item that was cut, in the order of the tokens, each scaled
-// to the largest maximum (the same sums in the same order on every run); rows that see nothing become 0.
+// One block per (query head, sequence): the pieces of an item that was cut, each scaled to the largest maximum, in an
+// order that only the lengths decide (the same sums on every run); rows that see nothing become 0. A warp takes 32
+// pieces at a time: their maxima and sums one per lane, then their outputs, several loads in flight.
 template <typename T, int TT>
-__global__ void __launch_bounds__(128) paged_join_kernel(PageView pv, int window, int sinks, T* __restrict__ out,
-                                                         float* __restrict__ lse, SplitWork wk) {
-    constexpr int WARPS = 4, PER = 8;  // d <= 256: at most 8 values per lane
+__global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(PageView pv, int window, int sinks, int workers,
+                                                                  T* __restrict__ out, float* __restrict__ lse,
+                                                                  SplitWork wk) {
+    constexpr int WARPS = JOIN_THREADS / 32, PER = 8;  // d <= 256: at most 8 values per lane
     const int lane = lane_id(), warp = threadIdx.x >> 5, hq = blockIdx.x, b = blockIdx.y;
     const int group = pv.hq / pv.hkv, gt = group_tiles(pv), qi = hq % group;
     const int tiles = Span(row_length(pv, b, nullptr), window, sinks, TT).tiles;
     const int64_t head = (int64_t)b * pv.hq + hq;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (tiles == 0) {
-        for (int x = threadIdx.x; x < pv.d; x += 128) out[head * pv.d + x] = narrow<T>(0.f);
+        for (int x = threadIdx.x; x < pv.d; x += JOIN_THREADS) out[head * pv.d + x] = narrow<T>(0.f);
         if (lse && threadIdx.x == 0) lse[head] = -INFINITY;
         return;
     }
-    const int64_t per = *wk.per, at = wk.base[b] + (int64_t)(hq / group * gt + qi / QT) * tiles;
-    const int64_t w0 = at / per, w1 = (at + tiles - 1) / per;
+    const Cut cut(*wk.total, workers);
+    const int64_t at = wk.base[b] + (int64_t)(hq / group * gt + qi / QT) * tiles;
+    const int64_t w0 = cut.worker_of(at), w1 = cut.worker_of(at + tiles - 1);
     if (w0 == w1) return;
+    const int64_t pieces = w1 - w0 + 1;
+    // the first piece is the last of its worker, the others the first of theirs
+    auto slot = [&](int64_t k) { return (2 * (w0 + k) + (k == 0)) * wk.rows + qi % QT; };
     float m = -INFINITY, l = 0.f, acc[PER];
 #pragma unroll
     for (int i = 0; i < PER; i++) acc[i] = 0.f;
-    for (int64_t w = w0 + warp; w <= w1; w += WARPS) {
-        const int64_t r = (2 * w + (w == w0)) * wk.rows + qi % QT;
-        const float pm = wk.m[r], pl = wk.l[r];
-        const float mn = fmaxf(m, pm), base = mn == -INFINITY ? 0.f : mn;
+    const int64_t each = (pieces + WARPS - 1) / WARPS;  // consecutive pieces per warp
+    const int64_t end = min(pieces, (warp + 1) * each);
+    for (int64_t k0 = warp * each; k0 < end; k0 += 32) {
+        const int count = (int)min((int64_t)32, end - k0);
+        float pm = -INFINITY, pl = 0.f;
+        if (lane < count) {
+            pm = wk.m[slot(k0 + lane)];
+            pl = wk.l[slot(k0 + lane)];
+        }
+        const float mn = fmaxf(m, warp_max(pm)), base = mn == -INFINITY ? 0.f : mn;
         const float a = ex2(m - base), e = ex2(pm - base);
-        l = l * a + pl * e;
+        l = l * a + warp_sum(pl * e);
 #pragma unroll
-        for (int i = 0; i < PER; i++)
-            if (lane + 32 * i < pv.d) acc[i] = acc[i] * a + wk.o[r * wk.dp + lane + 32 * i] * e;
+        for (int i = 0; i < PER; i++) acc[i] *= a;
+#pragma unroll 4
+        for (int k = 0; k < count; k++) {
+            const float f = __shfl_sync(FULL, e, k);
+            const float* src = wk.o + slot(k0 + k) * wk.dp + lane;
+#pragma unroll
+            for (int i = 0; i < PER; i++)
+                if (32 * i < wk.dp) acc[i] += f * src[32 * i];  // columns past d are not used
+        }
         m = mn;
     }
     __shared__ float sm[WARPS], sl[WARPS], so[WARPS][256];
@@ -543,7 +652,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(PageView pv, int window
     const float base = mx == -INFINITY ? 0.f : mx;
     for (int w = 0; w < WARPS; w++) sum += sl[w] * ex2(sm[w] - base);
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    for (int x = threadIdx.x; x < pv.d; x += 128) {
+    for (int x = threadIdx.x; x < pv.d; x += JOIN_THREADS) {
         float v = 0.f;
         for (int w = 0; w < WARPS; w++) v += so[w][x] * ex2(sm[w] - base);
         out[head * pv.d + x] = narrow<T>(v * inv);
@@ -620,9 +729,11 @@ static int fill_view(PageView& pv, const char* what, const void* k, const void* 
                    "%s: %lld pages, %lld table columns (stride %lld)", what, (long long)n_pages,
                    (long long)max_blocks, (long long)table_stride);
     const int es = element_bytes(dtype);
-    for (int i = 0; i < 6; i++)
+    for (int i = 0; i < 6; i++) {
         SMLM_CHECK_ARG(strides[i] >= 0 && strides[i] * es % 16 == 0,
                        "%s: page, head and token strides are multiples of 16 bytes", what);
+        SMLM_CHECK_ARG(i % 3 == 1 || strides[i] <= UINT32_MAX / es, "%s: page and token strides below 4 GiB", what);
+    }
     SMLM_CHECK_ARG(((uintptr_t)k | (uintptr_t)v) % 16 == 0, "%s: the pages are not 16-byte aligned", what);
     pv = PageView{k, v, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], table, lengths,
                   table_stride, (int)batch, (int)hq, (int)hkv, (int)d, (int)n_pages, 0, (int)max_blocks};
@@ -648,7 +759,7 @@ static void split_work(W& ws, SplitWork& wk, int64_t batch, int64_t hq, int64_t 
     wk.dp = (int)dp;
     if constexpr (std::is_same_v<W, Workspace>) {
         wk.base = ws.template take<int64_t>(batch);
-        wk.per = ws.template take<int64_t>(1);
+        wk.total = ws.template take<int64_t>(1);
         wk.m = ws.template take<float>(slots * wk.rows);
         wk.l = ws.template take<float>(slots * wk.rows);
         wk.o = ws.template take<float>(slots * wk.rows * dp);
@@ -661,25 +772,27 @@ static void split_work(W& ws, SplitWork& wk, int64_t batch, int64_t hq, int64_t 
     }
 }
 
-template <typename T, int DP, bool PART>
+template <typename T, int DP, bool PART, bool SMALL>
 static int launch_split(const PageView& pv, const void* q, float scale, int window, int sinks, void* out, float* lse,
                         const SplitWork& wk, int* status, cudaStream_t st) {
     using S = SplitShape<T, DP>;
-    paged_split_kernel<T, DP, PART><<<sm_count() * S::BLOCKS, SPLIT_THREADS, 0, st>>>(
+    const int blocks = sm_count() * S::BLOCKS;
+    paged_split_kernel<T, DP, PART, SMALL><<<blocks, SPLIT_THREADS, 0, st>>>(
         pv, static_cast<const T*>(q), scale * 1.4426950408889634074f, window, sinks, static_cast<T*>(out), lse, wk,
         status);
     SMLM_LAUNCHED("paged_attention");
     // launched while the first kernel still runs; it waits for that kernel's end itself
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(pv.hq, pv.batch);
-    cfg.blockDim = dim3(128);
+    cfg.blockDim = dim3(JOIN_THREADS);
     cfg.stream = st;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    SMLM_CUDA(cudaLaunchKernelEx(&cfg, paged_join_kernel<T, S::TT>, pv, window, sinks, static_cast<T*>(out), lse, wk));
+    SMLM_CUDA(cudaLaunchKernelEx(&cfg, paged_join_kernel<T, S::TT>, pv, window, sinks, blocks * SPLIT_WARPS,
+                                 static_cast<T*>(out), lse, wk));
     return SMLM_OK;
 }
 
@@ -688,8 +801,9 @@ static int launch_attention(const PageView& pv, const void* q, float scale, int 
                             float* lse, const SplitWork& wk, int* status, cudaStream_t st) {
     const auto go = [&](auto dp) {
         constexpr int DP = decltype(dp)::value;
-        return pv.d == DP ? launch_split<T, DP, false>(pv, q, scale, window, sinks, out, lse, wk, status, st)
-                          : launch_split<T, DP, true>(pv, q, scale, window, sinks, out, lse, wk, status, st);
+        if (pv.page_shift < 4) return launch_split<T, DP, true, true>(pv, q, scale, window, sinks, out, lse, wk, status, st);
+        return pv.d == DP ? launch_split<T, DP, false, false>(pv, q, scale, window, sinks, out, lse, wk, status, st)
+                          : launch_split<T, DP, true, false>(pv, q, scale, window, sinks, out, lse, wk, status, st);
     };
     if (pv.d <= 32) return go(std::integral_constant<int, 32>());
     if (pv.d <= 64) return go(std::integral_constant<int, 64>());
