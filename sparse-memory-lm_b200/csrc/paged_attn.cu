@@ -24,6 +24,7 @@ namespace smlm {
 
 constexpr int SPLIT_WARPS = 4, SPLIT_THREADS = SPLIT_WARPS * 32;
 constexpr int JOIN_THREADS = 256;
+constexpr int HEAD = 2;  // what beginning an item costs, in tiles (two dependent loads and the output), in the cut
 constexpr int QT = 8;  // query heads per item
 
 __device__ __forceinline__ float ex2(float x) {
@@ -129,19 +130,15 @@ struct Cut {
         }
     }
     __device__ __forceinline__ int64_t start(int64_t w) const { return w * per + min(w, extra); }
-    __device__ __forceinline__ int64_t worker_of(int64_t tile) const {
-        const int64_t wide = extra * (per + 1);
-        return tile < wide ? tile / (per + 1) : extra + (tile - wide) / per;
-    }
 };
 
+// Where the pieces of items that were cut lie. A worker has at most two: the one it began inside an item (slot 2 w)
+// and the one that holds an item's first tile but not its last (slot 2 w + 1).
 struct SplitWork {
-    int64_t* base;   // (batch): first tile of each sequence in the list
-    int64_t* total;  // tiles of all
-    float* m;        // (2 workers, rows): a worker's first and last piece
-    float* l;
-    float* o;        // (2 workers, rows, dp)
-    int rows, dp;    // rows = min(group, QT)
+    int2* cut;  // (batch, items): the workers of the item's first and last tile; x = -1: not cut
+    float* ml;  // (slots, rows, 2): running maximum and sum
+    float* o;   // (slots, rows, dp)
+    int rows, dp;  // rows = min(group, QT)
 };
 
 __device__ __forceinline__ int group_tiles(const PageView& pv) { return (pv.hq / pv.hkv + QT - 1) / QT; }
@@ -177,12 +174,16 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP>::BLOCKS)
     const int lane = lane_id(), warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
     const int group = pv.hq / pv.hkv, gt = group_tiles(pv), items = pv.hkv * gt;
 
+    // what the items of row r take in the list
+    auto cost = [&](int r, int* st) {
+        const int tiles = Span(row_length(pv, r, st), window, sinks, TT).tiles;
+        return tiles ? (int64_t)items * (tiles + HEAD) : 0;
+    };
     // the list's length and this thread's sequences' place in it
     const int chunk = (pv.batch + SPLIT_THREADS - 1) / SPLIT_THREADS;
     const int r0 = min(pv.batch, (int)threadIdx.x * chunk), r1 = min(pv.batch, r0 + chunk);
     int64_t mine = 0;
-    for (int r = r0; r < r1; r++) mine += Span(row_length(pv, r, status), window, sinks, TT).tiles;
-    mine *= items;
+    for (int r = r0; r < r1; r++) mine += cost(r, status);
     {
         int64_t x = mine;
 #pragma unroll
@@ -199,20 +200,12 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP>::BLOCKS)
     }
     const int64_t total = pre[SPLIT_THREADS];
     const Cut cut(total, gridDim.x * SPLIT_WARPS);
-    if (blockIdx.x == 0) {
-        if (threadIdx.x == 0) *wk.total = total;
-        int64_t x = pre[threadIdx.x];
-        for (int r = r0; r < r1; r++) {
-            wk.base[r] = x;
-            x += (int64_t)items * Span(row_length(pv, r, nullptr), window, sinks, TT).tiles;
-        }
-    }
     const int worker = warp * gridDim.x + blockIdx.x;  // few tiles: one warp per SM first
     int64_t left = cut.per + (worker < cut.extra);
     if (left <= 0) return;
 
-    // the sequence, item and tile where this worker starts
-    int b, item, tile;
+    // the sequence, the item and the place in it where this worker starts
+    int b, item, place;
     {
         const int64_t start = cut.start(worker);
         int a = 0, e = SPLIT_THREADS;  // pre[a] <= start < pre[e]
@@ -226,8 +219,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP>::BLOCKS)
         if (chunk > 1) {
             while (true) {
                 const int r = b + lane;
-                const int64_t w =
-                    r < pv.batch ? (int64_t)items * Span(row_length(pv, r, nullptr), window, sinks, TT).tiles : 0;
+                const int64_t w = r < pv.batch ? cost(r, nullptr) : 0;
                 int64_t x = w;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -245,13 +237,13 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP>::BLOCKS)
                 b += 32;
             }
         }
-        const int tiles = Span(row_length(pv, b, nullptr), window, sinks, TT).tiles;
+        const int each = Span(row_length(pv, b, nullptr), window, sinks, TT).tiles + HEAD;
         if (off >> 31) {
-            item = (int)(off / tiles);
-            tile = (int)(off % tiles);
+            item = (int)(off / each);
+            place = (int)(off % each);
         } else {
-            item = (uint32_t)off / (uint32_t)tiles;
-            tile = (uint32_t)off % (uint32_t)tiles;
+            item = (uint32_t)off / (uint32_t)each;
+            place = (uint32_t)off % (uint32_t)each;
         }
     }
 
@@ -263,9 +255,20 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP>::BLOCKS)
             b++;
             continue;
         }
-        const int first = tile, last = (int)min((int64_t)span.tiles, tile + left);
-        const int h = item / gt, q0 = item % gt * QT;
-        const int32_t* row = pv.table + b * pv.table_stride;
+        const int stop = (int)min((int64_t)span.tiles + HEAD, place + left);
+        const int first = max(place - HEAD, 0), last = max(stop - HEAD, 0);
+        left -= stop - place;
+        place = 0;
+        const int at = item;
+        if (++item == items) item = 0;
+        const int bb = b;
+        if (item == 0) b++;
+        if (first == last) {
+            if (left == 0) return;
+            continue;
+        }
+        const int h = at / gt, q0 = at % gt * QT;
+        const int32_t* row = pv.table + bb * pv.table_stride;
         auto entry = [&](int t) {  // the page of token t, or -1 past the end, in a hole or outside the pool
             int p = -1;
             if (t < span.n) {
@@ -308,7 +311,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP>::BLOCKS)
         };
         PagesOf pages = pages_at(first), pages_next;
         const int qrow = q0 + g;  // this lane's column of the first product
-        const T* qp = q + ((int64_t)b * pv.hq + h * group) * pv.d;
+        const T* qp = q + ((int64_t)bb * pv.hq + h * group) * pv.d;
         uint4 qf[WIDE ? 1 : KJ];
 #pragma unroll
         for (int j = 0; j < KJ; j++) {
@@ -540,14 +543,13 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP>::BLOCKS)
             const int col = 2 * t4 + x;
             if (q0 + col >= group) continue;
             const float l = x ? l1 : l0, m = x ? m1 : m0;
-            const int64_t head = (int64_t)b * pv.hq + h * group + q0 + col;
+            const int64_t head = (int64_t)bb * pv.hq + h * group + q0 + col;
             const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
             if (g == 0) {
                 if (whole) {
                     if (lse) lse[head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
                 } else {
-                    wk.m[slot * wk.rows + col] = m;
-                    wk.l[slot * wk.rows + col] = l;
+                    *reinterpret_cast<float2*>(wk.ml + 2 * (slot * wk.rows + col)) = make_float2(m, l);
                 }
             }
 #pragma unroll
@@ -577,26 +579,25 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP>::BLOCKS)
                 }
             }
         }
-        left -= last - first;
-        if (left == 0) return;
-        tile = 0;
-        if (++item == items) {
-            item = 0;
-            b++;
+        if (lane == 0) {
+            int2* cut_at = wk.cut + (int64_t)bb * items + at;
+            if (first == 0) cut_at->x = whole ? -1 : worker;
+            if (last == span.tiles) cut_at->y = worker;
         }
+        if (left == 0) return;
     }
 }
 
 // One block per (query head, sequence): the pieces of an item that was cut, each scaled to the largest maximum, in an
-// order that only the lengths decide (the same sums on every run); rows that see nothing become 0. A warp takes 32
-// pieces at a time: their maxima and sums one per lane, then their outputs, several loads in flight.
-template <typename T, int TT>
-__global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(PageView pv, int window, int sinks, int workers,
+// order that only the lengths decide (the same sums on every run); rows that see nothing become 0. DP / 4 lanes take
+// a piece, JOIN_THREADS / (DP / 4) pieces go at a time, and every lane has four of them in flight: what this kernel
+// costs is a chain of dependent loads (where the pieces are; the pieces), not their bytes.
+template <typename T, int DP, int TT>
+__global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(PageView pv, int window, int sinks,
                                                                   T* __restrict__ out, float* __restrict__ lse,
                                                                   SplitWork wk) {
-    constexpr int WARPS = JOIN_THREADS / 32, PER = 8;  // d <= 256: at most 8 values per lane
-    const int lane = lane_id(), warp = threadIdx.x >> 5, hq = blockIdx.x, b = blockIdx.y;
-    const int group = pv.hq / pv.hkv, gt = group_tiles(pv), qi = hq % group;
+    constexpr int LANES = DP / 4, SETS = JOIN_THREADS / LANES, U = 4;
+    const int hq = blockIdx.x, b = blockIdx.y, group = pv.hq / pv.hkv, gt = group_tiles(pv), qi = hq % group;
     const int tiles = Span(row_length(pv, b, nullptr), window, sinks, TT).tiles;
     const int64_t head = (int64_t)b * pv.hq + hq;
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -605,59 +606,79 @@ __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(PageView pv, i
         if (lse && threadIdx.x == 0) lse[head] = -INFINITY;
         return;
     }
-    const Cut cut(*wk.total, workers);
-    const int64_t at = wk.base[b] + (int64_t)(hq / group * gt + qi / QT) * tiles;
-    const int64_t w0 = cut.worker_of(at), w1 = cut.worker_of(at + tiles - 1);
-    if (w0 == w1) return;
-    const int64_t pieces = w1 - w0 + 1;
-    // the first piece is the last of its worker, the others the first of theirs
-    auto slot = [&](int64_t k) { return (2 * (w0 + k) + (k == 0)) * wk.rows + qi % QT; };
-    float m = -INFINITY, l = 0.f, acc[PER];
+    const int2 cut = wk.cut[((int64_t)b * pv.hkv + hq / group) * gt + qi / QT];
+    if (cut.x < 0) return;
+    const int pieces = cut.y - cut.x + 1, set = threadIdx.x / LANES, x = threadIdx.x % LANES * 4;
+    float m = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k0 = set; k0 < pieces; k0 += SETS * U) {
+        float2 ml[U];
+        float4 o[U];
 #pragma unroll
-    for (int i = 0; i < PER; i++) acc[i] = 0.f;
-    const int64_t each = (pieces + WARPS - 1) / WARPS;  // consecutive pieces per warp
-    const int64_t end = min(pieces, (warp + 1) * each);
-    for (int64_t k0 = warp * each; k0 < end; k0 += 32) {
-        const int count = (int)min((int64_t)32, end - k0);
-        float pm = -INFINITY, pl = 0.f;
-        if (lane < count) {
-            pm = wk.m[slot(k0 + lane)];
-            pl = wk.l[slot(k0 + lane)];
+        for (int u = 0; u < U; u++) {
+            const int k = k0 + u * SETS;
+            // the first piece is the last of its worker, the others the first of theirs
+            const int64_t r = (2 * ((int64_t)cut.x + k) + (k == 0)) * wk.rows + qi % QT;
+            ml[u] = make_float2(-INFINITY, 0.f);
+            o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (k < pieces) {
+                ml[u] = *reinterpret_cast<const float2*>(wk.ml + 2 * r);
+                o[u] = *reinterpret_cast<const float4*>(wk.o + r * DP + x);  // columns past d are not stored
+            }
         }
-        const float mn = fmaxf(m, warp_max(pm)), base = mn == -INFINITY ? 0.f : mn;
-        const float a = ex2(m - base), e = ex2(pm - base);
-        l = l * a + warp_sum(pl * e);
+        float mn = m;
 #pragma unroll
-        for (int i = 0; i < PER; i++) acc[i] *= a;
-#pragma unroll 4
-        for (int k = 0; k < count; k++) {
-            const float f = __shfl_sync(FULL, e, k);
-            const float* src = wk.o + slot(k0 + k) * wk.dp + lane;
+        for (int u = 0; u < U; u++) mn = fmaxf(mn, ml[u].x);
+        const float base = mn == -INFINITY ? 0.f : mn, a = ex2(m - base);
+        l *= a;
+        acc.x *= a;
+        acc.y *= a;
+        acc.z *= a;
+        acc.w *= a;
 #pragma unroll
-            for (int i = 0; i < PER; i++)
-                if (32 * i < wk.dp) acc[i] += f * src[32 * i];  // columns past d are not used
+        for (int u = 0; u < U; u++) {
+            if (k0 + u * SETS >= pieces) break;
+            const float e = ex2(ml[u].x - base);
+            l += ml[u].y * e;
+            acc.x += o[u].x * e;
+            acc.y += o[u].y * e;
+            acc.z += o[u].z * e;
+            acc.w += o[u].w * e;
         }
         m = mn;
     }
-    __shared__ float sm[WARPS], sl[WARPS], so[WARPS][256];
-    if (lane == 0) {
-        sm[warp] = m;
-        sl[warp] = l;
+    __shared__ float sm[SETS], sl[SETS];
+    __shared__ float4 so[SETS][LANES];
+    if (x == 0) {
+        sm[set] = m;
+        sl[set] = l;
     }
-#pragma unroll
-    for (int i = 0; i < PER; i++) so[warp][lane + 32 * i] = acc[i];
+    so[set][x / 4] = acc;
     __syncthreads();
+    if (set) return;
+    const int sets = min(pieces, SETS);
     float mx = -INFINITY, sum = 0.f;
-    for (int w = 0; w < WARPS; w++) mx = fmaxf(mx, sm[w]);
+    for (int w = 0; w < sets; w++) mx = fmaxf(mx, sm[w]);
     const float base = mx == -INFINITY ? 0.f : mx;
-    for (int w = 0; w < WARPS; w++) sum += sl[w] * ex2(sm[w] - base);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    for (int x = threadIdx.x; x < pv.d; x += JOIN_THREADS) {
-        float v = 0.f;
-        for (int w = 0; w < WARPS; w++) v += so[w][x] * ex2(sm[w] - base);
-        out[head * pv.d + x] = narrow<T>(v * inv);
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int w = 0; w < sets; w++) {
+        const float e = ex2(sm[w] - base);
+        const float4 o = so[w][x / 4];
+        sum += sl[w] * e;
+        acc.x += o.x * e;
+        acc.y += o.y * e;
+        acc.z += o.z * e;
+        acc.w += o.w * e;
     }
-    if (lse && threadIdx.x == 0) lse[head] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * 0.69314718055994530942f;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (x < pv.d) {
+        T* dst = out + head * pv.d + x;
+        dst[0] = narrow<T>(acc.x * inv);
+        dst[1] = narrow<T>(acc.y * inv);
+        dst[2] = narrow<T>(acc.z * inv);
+        dst[3] = narrow<T>(acc.w * inv);
+    }
+    if (lse && x == 0) lse[head] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * 0.69314718055994530942f;
 }
 
 // Rotary positions on the queries and keys of a fused projection, keys and values into their pages. One thread per
@@ -757,17 +778,14 @@ static void split_work(W& ws, SplitWork& wk, int64_t batch, int64_t hq, int64_t 
     const int64_t dp = padded_d(d), slots = 2 * (int64_t)sm_count() * split_blocks(es, dp) * SPLIT_WARPS;
     wk.rows = (int)std::min<int64_t>(hq / std::max<int64_t>(hkv, 1), QT);
     wk.dp = (int)dp;
+    const int64_t items = batch * hkv * ((hq / std::max<int64_t>(hkv, 1) + QT - 1) / QT);
     if constexpr (std::is_same_v<W, Workspace>) {
-        wk.base = ws.template take<int64_t>(batch);
-        wk.total = ws.template take<int64_t>(1);
-        wk.m = ws.template take<float>(slots * wk.rows);
-        wk.l = ws.template take<float>(slots * wk.rows);
+        wk.cut = ws.template take<int2>(items);
+        wk.ml = ws.template take<float>(2 * slots * wk.rows);
         wk.o = ws.template take<float>(slots * wk.rows * dp);
     } else {
-        ws.template take<int64_t>(batch);
-        ws.template take<int64_t>(1);
-        ws.template take<float>(slots * wk.rows);
-        ws.template take<float>(slots * wk.rows);
+        ws.template take<int2>(items);
+        ws.template take<float>(2 * slots * wk.rows);
         ws.template take<float>(slots * wk.rows * dp);
     }
 }
@@ -791,8 +809,7 @@ static int launch_split(const PageView& pv, const void* q, float scale, int wind
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    SMLM_CUDA(cudaLaunchKernelEx(&cfg, paged_join_kernel<T, S::TT>, pv, window, sinks, blocks * SPLIT_WARPS,
-                                 static_cast<T*>(out), lse, wk));
+    SMLM_CUDA(cudaLaunchKernelEx(&cfg, paged_join_kernel<T, DP, S::TT>, pv, window, sinks, static_cast<T*>(out), lse, wk));
     return SMLM_OK;
 }
 

@@ -221,7 +221,7 @@ class timed:
 
 
 def checked():
-    return os.environ.get("SMLM_B200_CHECK", "0") == "1"
+    return os.environb.get(b"SMLM_B200_CHECK") == b"1"
 
 
 def status_ptr(device):
@@ -245,6 +245,30 @@ def read_status(device, reset=True):
     if reset:
         st.zero_()
     return v
+
+
+# The same for calls that are worth a few microseconds in all (one decoding step makes two per layer): addresses as
+# plain integers, no wrapper objects.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def stream_int(device):
+    if _raw_stream is None or device.index is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    return _raw_stream(device.index)
+
+
+def status_int(device):
+    st = _STATUS.get(device.index)
+    if st is None:
+        p = status_ptr(device)
+        return p.value if p is not None else None
+    return st.data_ptr()
+
+
+def instrumented():
+    """Whether calls are timed, ranged or checked (timed / after do something)."""
+    return PROFILE is not None or NVTX or checked()
 
 
 def after(device, what):

@@ -26,26 +26,64 @@ import torch
 from . import _lib as L
 
 
+_I32 = torch.int32
+_CODES = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
+_Strides = ctypes.c_int64 * 6
+
+
 def _int32(what, t, dim):
-    if t.dtype != torch.int32 or t.dim() != dim or (t.numel() and t.stride(-1) != 1):
+    if t.dtype != _I32 or t.dim() != dim or (t.numel() and t.stride(-1) != 1):
         raise ValueError(f"{what} has to be an int32 tensor of {dim} dimension(s) with contiguous rows")
 
 
+def _call(name, launches, device, fn, *args):
+    """fn(*args, status, stream) on the current stream."""
+    if not L.instrumented():
+        rc = fn(*args, L.status_int(device), L.stream_int(device))
+        if rc:
+            L.check(rc, name)
+        return
+    with L.timed(name, launches):
+        rc = fn(*args, L.status_int(device), L.stream_int(device))
+    L.check(rc, name)
+    L.after(device, name)
+
+
 def _cache(what, x, k_pages, v_pages, table, lengths, batch):
-    """Checks a layer's pages against the activations x; returns the cache's common arguments."""
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+    """Checks a layer's pages against the activations x; returns the pages' shape, both strides and the dtype code."""
+    shape, dtype = k_pages.shape, x.dtype
+    if len(shape) != 4 or shape != v_pages.shape:
         raise ValueError(f"{what}: k_pages and v_pages have to be (pages, key heads, page_size, head dimension)")
-    if x.dtype != k_pages.dtype or x.dtype != v_pages.dtype:
+    if dtype != k_pages.dtype or dtype != v_pages.dtype:
         raise ValueError(f"{what}: activations and pages have to be of one type, got {x.dtype}, {k_pages.dtype}, "
                          f"{v_pages.dtype}")
-    if k_pages.stride(3) != 1 or v_pages.stride(3) != 1:
+    code = _CODES.get(dtype)
+    if code is None:
+        raise ValueError(f"{what}: unsupported type {dtype} (fp32, bf16 or fp16)")
+    ks, vs = k_pages.stride(), v_pages.stride()
+    if ks[3] != 1 or vs[3] != 1:
         raise ValueError(f"{what}: the pages' head dimension has to be contiguous")
-    _int32(f"{what}: table", table, 2)
-    _int32(f"{what}: lengths", lengths, 1)
-    if table.shape[0] != batch or lengths.shape[0] != batch:
-        raise ValueError(f"{what}: {batch} sequences, but a table of {table.shape[0]} rows and {lengths.shape[0]} lengths")
-    strides = (ctypes.c_int64 * 6)(*k_pages.stride()[:3], *v_pages.stride()[:3])
-    return strides
+    if table.dtype != _I32 or table.dim() != 2 or table.shape[0] != batch or (batch and table.stride(1) != 1):
+        raise ValueError(f"{what}: the table has to be int32, ({batch} sequences, blocks) with contiguous rows; got "
+                         f"{table.dtype} {tuple(table.shape)}")
+    if lengths.dtype != _I32 or lengths.shape != (batch,) or not lengths.is_contiguous():
+        raise ValueError(f"{what}: lengths has to be a contiguous int32 tensor of {batch} lengths; got "
+                         f"{lengths.dtype} {tuple(lengths.shape)}")
+    if not (x.is_cuda and x.device == k_pages.device == v_pages.device == table.device == lengths.device):
+        L.require_cuda(x, k_pages, v_pages, table, lengths)
+    return shape, _Strides(ks[0], ks[1], ks[2], vs[0], vs[1], vs[2]), code
+
+
+_WORKSPACE = {}
+
+
+def _attention_workspace(*sizes):
+    """smlm_paged_attention_workspace, asked once per sizes and device."""
+    key = (torch.cuda.current_device(), *sizes)
+    n = _WORKSPACE.get(key)
+    if n is None:
+        n = _WORKSPACE[key] = L.lib().smlm_paged_attention_workspace(*sizes)
+    return n
 
 
 def paged_attention(q, k_pages, v_pages, table, lengths, *, scale=None, window=0, sinks=0, return_lse=False):
@@ -60,25 +98,22 @@ def paged_attention(q, k_pages, v_pages, table, lengths, *, scale=None, window=0
     if q.dim() != 3:
         raise ValueError(f"paged_attention: q has to be (sequences, heads, head dimension), got {tuple(q.shape)}")
     B, HQ, D = q.shape
-    strides = _cache("paged_attention", q, k_pages, v_pages, table, lengths, B)
-    P, HKV, page, Dk = k_pages.shape
+    (P, HKV, page, Dk), strides, code = _cache("paged_attention", q, k_pages, v_pages, table, lengths, B)
     if D != Dk or HQ % HKV:
         raise ValueError(f"paged_attention: {HQ} query heads of {D} over {HKV} key heads of {Dk}")
     if window < 0 or sinks < 0:
         raise ValueError(f"paged_attention: window {window}, sinks {sinks}")
-    dev = L.require_cuda(q, k_pages, v_pages, table, lengths)
-    q = q if q.is_contiguous() else q.contiguous()
+    if not q.is_contiguous():
+        q = q.contiguous()
+    dev = q.device
     out = torch.empty_like(q)
     lse = torch.empty(B, HQ, dtype=torch.float32, device=dev) if return_lse else None
-    lib = L.lib()
-    ws = L.workspace(lib.smlm_paged_attention_workspace(B, HQ, HKV, D, L.dtype_code(q.dtype)), dev)
-    with L.timed("paged_attention", 2):
-        rc = lib.smlm_paged_attention(L.ptr(q), L.ptr(k_pages), L.ptr(v_pages), L.dtype_code(q.dtype), strides,
-                                      L.ptr(table), table.stride(0), L.ptr(lengths), B, HQ, HKV, D, P, page,
-                                      table.shape[1], D ** -0.5 if scale is None else scale, window, sinks,
-                                      L.ptr(out), L.ptr(lse), L.ptr(ws), ws.numel(), L.status_ptr(dev), L.stream(dev))
-    L.check(rc, "paged_attention")
-    L.after(dev, "paged_attention")
+    nbytes = _attention_workspace(B, HQ, HKV, D, code)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _call("paged_attention", 2, dev, L.lib().smlm_paged_attention, q.data_ptr(), k_pages.data_ptr(),
+          v_pages.data_ptr(), code, strides, table.data_ptr(), table.stride(0), lengths.data_ptr(), B, HQ, HKV, D, P,
+          page, table.shape[1], D ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(),
+          lse.data_ptr() if return_lse else None, ws.data_ptr(), nbytes)
     return (out, lse) if return_lse else out
 
 
@@ -91,30 +126,27 @@ def paged_append(qkv, k_pages, v_pages, table, lengths, cos=None, sin=None):
     if qkv.dim() != 3:
         raise ValueError(f"paged_append: qkv has to be (sequences, tokens, width), got {tuple(qkv.shape)}")
     B, T, W = qkv.shape
-    strides = _cache("paged_append", qkv, k_pages, v_pages, table, lengths, B)
-    P, HKV, page, D = k_pages.shape
+    (P, HKV, page, D), strides, code = _cache("paged_append", qkv, k_pages, v_pages, table, lengths, B)
     HQ = W // D - 2 * HKV
     if W % D or HQ < 1 or HQ % HKV:
         raise ValueError(f"paged_append: a projection of {W} values with {HKV} key heads of {D}")
-    max_pos = 0
-    if (cos is None) != (sin is None):
-        raise ValueError("paged_append: cos and sin come together")
-    if cos is not None:
-        for t in (cos, sin):
-            if t.dtype != torch.float32 or t.dim() != 2 or t.shape != cos.shape or 2 * t.shape[1] != D or \
-                    not t.is_contiguous():
-                raise ValueError(f"paged_append: cos and sin have to be contiguous fp32 (positions, {D // 2})")
-        max_pos = cos.shape[0]
-    dev = L.require_cuda(qkv, k_pages, v_pages, table, lengths, cos, sin)
-    qkv = qkv if qkv.is_contiguous() else qkv.contiguous()
-    q = torch.empty(B, T, HQ, D, dtype=qkv.dtype, device=dev)
-    with L.timed("paged_append", 1):
-        rc = L.lib().smlm_paged_append(L.ptr(qkv), L.ptr(k_pages), L.ptr(v_pages), L.dtype_code(qkv.dtype), strides,
-                                       L.ptr(table), table.stride(0), L.ptr(lengths), B, T, HQ, HKV, D, P, page,
-                                       table.shape[1], L.ptr(cos), L.ptr(sin), max_pos, L.ptr(q), L.status_ptr(dev),
-                                       L.stream(dev))
-    L.check(rc, "paged_append")
-    L.after(dev, "paged_append")
+    dev = qkv.device
+    positions, pcos, psin = 0, None, None
+    if cos is not None or sin is not None:
+        if cos is None or sin is None:
+            raise ValueError("paged_append: cos and sin come together")
+        if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.shape != sin.shape or cos.dim() != 2 or \
+                2 * cos.shape[1] != D or not (cos.is_contiguous() and sin.is_contiguous()):
+            raise ValueError(f"paged_append: cos and sin have to be contiguous fp32 (positions, {D // 2})")
+        if cos.device != dev or sin.device != dev:
+            L.require_cuda(qkv, cos, sin)
+        positions, pcos, psin = cos.shape[0], cos.data_ptr(), sin.data_ptr()
+    if not qkv.is_contiguous():
+        qkv = qkv.contiguous()
+    q = torch.empty((B, T, HQ, D), dtype=qkv.dtype, device=dev)
+    _call("paged_append", 1, dev, L.lib().smlm_paged_append, qkv.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+          code, strides, table.data_ptr(), table.stride(0), lengths.data_ptr(), B, T, HQ, HKV, D, P, page,
+          table.shape[1], pcos, psin, positions, q.data_ptr())
     return q
 
 
@@ -122,13 +154,19 @@ def paged_append(qkv, k_pages, v_pages, table, lengths, cos=None, sin=None):
 def _tables(what, table, lengths, refcount, *rows):
     _int32(f"{what}: table", table, 2)
     _int32(f"{what}: reference counts", refcount, 1)
+    dev = table.device
+    same = table.is_cuda and refcount.device == dev
     for r in rows:
         _int32(f"{what}: row numbers", r, 1)
+        same = same and r.device == dev
     if lengths is not None:
         _int32(f"{what}: lengths", lengths, 1)
         if lengths.shape[0] != table.shape[0]:
             raise ValueError(f"{what}: {table.shape[0]} table rows, {lengths.shape[0]} lengths")
-    return L.require_cuda(table, lengths, refcount, *rows)
+        same = same and lengths.device == dev
+    if not same:
+        L.require_cuda(table, lengths, refcount, *rows)
+    return dev
 
 
 def _pool(what, pool, refcount):
@@ -138,45 +176,36 @@ def _pool(what, pool, refcount):
                          f"dimension) tensor, got {tuple(pool.shape)}")
     if pool.shape[2] != refcount.shape[0]:
         raise ValueError(f"{what}: {pool.shape[2]} pages, {refcount.shape[0]} reference counts")
-    L.require_cuda(pool, refcount)
+    if pool.device != refcount.device:
+        L.require_cuda(pool, refcount)
     return 2 * pool.shape[0], pool.shape[3], pool.shape[5] * pool.element_size(), pool.shape[4]
 
 
 def pages_free(table, lengths, refcount, rows):
     """The sequences `rows` (int32) end: their pages are released, their table entries become -1, their lengths 0."""
     dev = _tables("pages_free", table, lengths, refcount, rows)
-    with L.timed("pages_free", 1):
-        rc = L.lib().smlm_pages_free(L.ptr(table), table.stride(0), table.shape[0], table.shape[1], L.ptr(lengths),
-                                     L.ptr(refcount), refcount.shape[0], L.ptr(rows), rows.shape[0],
-                                     L.status_ptr(dev), L.stream(dev))
-    L.check(rc, "pages_free")
-    L.after(dev, "pages_free")
+    _call("pages_free", 1, dev, L.lib().smlm_pages_free, table.data_ptr(), table.stride(0), *table.shape,
+          lengths.data_ptr(), refcount.data_ptr(), refcount.shape[0], rows.data_ptr(), rows.shape[0])
 
 
 def pages_trim(table, lengths, refcount, rows, page_size, window, sinks=0):
     """Releases the pages of the sequences `rows` that paged_attention with this window and these sinks no longer reads:
     those that hold only tokens in [sinks, length - window)."""
     dev = _tables("pages_trim", table, lengths, refcount, rows)
-    with L.timed("pages_trim", 1):
-        rc = L.lib().smlm_pages_trim(L.ptr(table), table.stride(0), table.shape[0], table.shape[1], L.ptr(lengths),
-                                     L.ptr(refcount), refcount.shape[0], page_size, L.ptr(rows), rows.shape[0], window,
-                                     sinks, L.status_ptr(dev), L.stream(dev))
-    L.check(rc, "pages_trim")
-    L.after(dev, "pages_trim")
+    _call("pages_trim", 1, dev, L.lib().smlm_pages_trim, table.data_ptr(), table.stride(0), *table.shape,
+          lengths.data_ptr(), refcount.data_ptr(), refcount.shape[0], page_size, rows.data_ptr(), rows.shape[0],
+          window, sinks)
 
 
 def pages_extend(table, lengths, refcount, rows, n_new, page_size):
     """Every sequence in `rows` grows by n_new tokens: lengths[r] += n_new, with the lowest free pages (row by row) where
     its last page is full. A sequence that finds too few keeps its length."""
     dev = _tables("pages_extend", table, lengths, refcount, rows)
-    lib = L.lib()
-    ws = L.workspace(lib.smlm_pages_extend_workspace(rows.shape[0], refcount.shape[0]), dev)
-    with L.timed("pages_extend", 1):
-        rc = lib.smlm_pages_extend(L.ptr(table), table.stride(0), table.shape[0], table.shape[1], L.ptr(lengths),
-                                   L.ptr(refcount), refcount.shape[0], page_size, L.ptr(rows), rows.shape[0], n_new,
-                                   L.ptr(ws), ws.numel(), L.status_ptr(dev), L.stream(dev))
-    L.check(rc, "pages_extend")
-    L.after(dev, "pages_extend")
+    lib, n, pages = L.lib(), rows.shape[0], refcount.shape[0]
+    nbytes = lib.smlm_pages_extend_workspace(n, pages)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _call("pages_extend", 1, dev, lib.smlm_pages_extend, table.data_ptr(), table.stride(0), *table.shape,
+          lengths.data_ptr(), refcount.data_ptr(), pages, page_size, rows.data_ptr(), n, n_new, ws.data_ptr(), nbytes)
 
 
 def pages_fork(pool, table, lengths, refcount, parents, children):
@@ -188,14 +217,11 @@ def pages_fork(pool, table, lengths, refcount, parents, children):
     if parents.shape != children.shape:
         raise ValueError(f"pages_fork: {parents.shape[0]} parents, {children.shape[0]} children")
     lib, n = L.lib(), parents.shape[0]
-    ws = L.workspace(lib.smlm_pages_fork_workspace(n, table.shape[0], table.shape[1], refcount.shape[0]), dev)
-    with L.timed("pages_fork", 2):
-        rc = lib.smlm_pages_fork(L.ptr(pool), planes, heads, token, L.ptr(table), table.stride(0), table.shape[0],
-                                 table.shape[1], L.ptr(lengths), L.ptr(refcount), refcount.shape[0], page,
-                                 L.ptr(parents), L.ptr(children), n, L.ptr(ws), ws.numel(), L.status_ptr(dev),
-                                 L.stream(dev))
-    L.check(rc, "pages_fork")
-    L.after(dev, "pages_fork")
+    nbytes = lib.smlm_pages_fork_workspace(n, *table.shape, refcount.shape[0])
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _call("pages_fork", 2, dev, lib.smlm_pages_fork, pool.data_ptr(), planes, heads, token, table.data_ptr(),
+          table.stride(0), *table.shape, lengths.data_ptr(), refcount.data_ptr(), refcount.shape[0], page,
+          parents.data_ptr(), children.data_ptr(), n, ws.data_ptr(), nbytes)
 
 
 def pages_compact(pool, table, refcount):
@@ -204,10 +230,7 @@ def pages_compact(pool, table, refcount):
     dev = _tables("pages_compact", table, None, refcount)
     planes, heads, token, page = _pool("pages_compact", pool, refcount)
     lib = L.lib()
-    ws = L.workspace(lib.smlm_pages_compact_workspace(refcount.shape[0]), dev)
-    with L.timed("pages_compact", 2):
-        rc = lib.smlm_pages_compact(L.ptr(pool), planes, heads, token, L.ptr(table), table.stride(0), table.shape[0],
-                                    table.shape[1], L.ptr(refcount), refcount.shape[0], page, L.ptr(ws), ws.numel(),
-                                    L.status_ptr(dev), L.stream(dev))
-    L.check(rc, "pages_compact")
-    L.after(dev, "pages_compact")
+    nbytes = lib.smlm_pages_compact_workspace(refcount.shape[0])
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _call("pages_compact", 2, dev, lib.smlm_pages_compact, pool.data_ptr(), planes, heads, token, table.data_ptr(),
+          table.stride(0), *table.shape, refcount.data_ptr(), refcount.shape[0], page, ws.data_ptr(), nbytes)
