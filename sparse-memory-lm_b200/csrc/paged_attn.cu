@@ -681,51 +681,143 @@ __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(PageView pv, i
     if (lse && x == 0) lse[head] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * 0.69314718055994530942f;
 }
 
-// Rotary positions on the queries and keys of a fused projection, keys and values into their pages. One thread per
-// pair (i, i + d / 2) of one head of one token; token t of row b is at position lengths[b] - T + t (negative: the
-// padding before a shorter chunk, whose queries become 0).
+// ---------------------------------------------------------------------------------------------------- append
+// Rotary positions on the queries and keys of a fused projection, keys and values into their pages: every byte is read
+// once and written once. A block takes `per_block` tokens: their positions and pages are looked up once into shared
+// memory, then a thread handles 16 bytes of a head's first half and the 16 bytes they are paired with in its second
+// half (value i with i + d / 2), four such pairs in flight; cos and sin come from L1 after a token's first head.
+// Token t of row b is at position lengths[b] - T + t; a negative one is the padding before a shorter chunk.
+constexpr int APPEND_THREADS = 256, APPEND_TOKENS = 32, APPEND_UNROLL = 4;
+
 template <typename T>
-__global__ void __launch_bounds__(256) paged_append_kernel(PageView pv, const T* qkv, int tokens, const float* cosb,
-                                                           const float* sinb, int max_pos, T* q_out, int* status) {
-    const int heads = pv.hq + 2 * pv.hkv, half = pv.d / 2;
-    const int64_t all = (int64_t)pv.batch * tokens * heads * half;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (int64_t)gridDim.x * blockDim.x) {
-        const int c = i % half, hd = (i / half) % heads;
-        const int64_t tok = i / ((int64_t)half * heads);
-        const int b = tok / tokens, t = tok % tokens;
-        const int pos = row_length(pv, b, status) - tokens + t;
-        const T* src = qkv + (tok * heads + hd) * pv.d;
-        float x = widen(src[c]), y = widen(src[c + half]);
-        if (hd < pv.hq + pv.hkv && cosb && pos >= 0) {
-            if (pos >= max_pos) {
-                flag(status, SMLM_FLAG_INDEX_RANGE);
-                continue;
-            }
-            const float co = cosb[(int64_t)pos * half + c], si = sinb[(int64_t)pos * half + c];
-            const float a = x;
-            x = a * co - y * si;
-            y = y * co + a * si;
-        }
-        T* dst;
-        if (hd < pv.hq) {
-            dst = q_out + (tok * pv.hq + hd) * pv.d;
-            if (pos < 0) x = y = 0.f;
+__device__ __forceinline__ void widen16(const uint4& v, float (&f)[16 / sizeof(T)]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4) {
+            f[i] = __uint_as_float(w[i]);
         } else {
-            if (pos < 0) continue;
-            const int p = page_of(pv, b, pos, status);
-            if (p < 0) {
-                flag(status, SMLM_FLAG_NO_PAGES);
-                continue;
-            }
-            const int slot = pos & ((1 << pv.page_shift) - 1);
-            if (hd < pv.hq + pv.hkv)
-                dst = static_cast<T*>(const_cast<void*>(pv.k)) + p * pv.kp + (hd - pv.hq) * pv.kh + slot * pv.kt;
-            else
-                dst = static_cast<T*>(const_cast<void*>(pv.v)) + p * pv.vp + (hd - pv.hq - pv.hkv) * pv.vh +
-                      slot * pv.vt;
+            const float2 p = unpack16<T>(w[i]);
+            f[2 * i] = p.x;
+            f[2 * i + 1] = p.y;
         }
-        dst[c] = narrow<T>(x);
-        dst[c + half] = narrow<T>(y);
+    }
+}
+template <typename T>
+__device__ __forceinline__ uint4 narrow16(const float (&f)[16 / sizeof(T)]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(f[i]);
+        else w[i] = pack16<T>(f[2 * i], f[2 * i + 1]);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(APPEND_THREADS)
+    paged_append_kernel(PageView pv, const T* __restrict__ qkv, int tokens, const float* __restrict__ cosb,
+                        const float* __restrict__ sinb, int max_pos, T* __restrict__ q_out, int per_block,
+                        uint32_t by_token, uint32_t by_head, int* status) {
+    constexpr int CH = 16 / sizeof(T), U = APPEND_UNROLL;
+    __shared__ int pos_of[APPEND_TOKENS];
+    __shared__ int state_of[APPEND_TOKENS];  // 1: stored, 0: only its queries, -1: skipped
+    __shared__ int64_t k_of[APPEND_TOKENS], v_of[APPEND_TOKENS];
+    const int64_t first = (int64_t)blockIdx.x * per_block;
+    const int count = (int)min((int64_t)per_block, (int64_t)pv.batch * tokens - first);
+    const int half = pv.d / 2, lanes = half / CH, heads = pv.hq + 2 * pv.hkv, rot = pv.hq + pv.hkv;
+    const uint32_t per_token = heads * lanes, all = count * per_token;
+    // pair i of the block: token i / per_token, head and 16 bytes from the rest; by_token and by_head are the
+    // divisors' reciprocals (exact here: dividend x divisor < 2^32)
+    auto place = [&](uint32_t i, uint32_t& tk, uint32_t& hd, uint32_t& c) {
+        tk = per_token == 1 ? i : __umulhi(i, by_token);
+        const uint32_t r = i - tk * per_token;
+        hd = lanes == 1 ? r : __umulhi(r, by_head);
+        c = (r - hd * lanes) * CH;
+    };
+    const T* block_in = qkv + first * heads * pv.d;
+    uint4 xa[U], ya[U];
+    auto load = [&](uint32_t i0) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const uint32_t i = i0 + u * APPEND_THREADS;
+            if (i >= all) break;
+            uint32_t tk, hd, c;
+            place(i, tk, hd, c);
+            const T* src = block_in + (tk * heads + hd) * pv.d + c;
+            xa[u] = load16(src);
+            ya[u] = load16(src + half);
+        }
+    };
+    load(threadIdx.x);  // in flight during the look-ups
+    for (int i = threadIdx.x; i < count; i += APPEND_THREADS) {
+        const int b = (int)((first + i) / tokens), t = (int)((first + i) % tokens);
+        const int pos = row_length(pv, b, status) - tokens + t;
+        int state = 0;
+        if (pos >= 0) {
+            const int page = page_of(pv, b, pos, status);
+            const int64_t slot = pos & ((1 << pv.page_shift) - 1);
+            if (page >= 0) {
+                state = 1;
+                k_of[i] = page * pv.kp + slot * pv.kt;
+                v_of[i] = page * pv.vp + slot * pv.vt;
+            } else {
+                flag(status, SMLM_FLAG_NO_PAGES);
+            }
+            if (cosb && pos >= max_pos) {
+                flag(status, SMLM_FLAG_INDEX_RANGE);
+                state = -1;
+            }
+        }
+        pos_of[i] = pos;
+        state_of[i] = state;
+    }
+    __syncthreads();
+    for (uint32_t i0 = threadIdx.x; i0 < all; i0 += APPEND_THREADS * U) {
+        if (i0 != threadIdx.x) load(i0);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const uint32_t i = i0 + u * APPEND_THREADS;
+            if (i >= all) break;
+            uint32_t tk, hd, c;
+            place(i, tk, hd, c);
+            const int pos = pos_of[tk], state = state_of[tk];
+            if (state < 0) continue;
+            uint4 xo = xa[u], yo = ya[u];
+            T* dst;
+            if (hd < (uint32_t)pv.hq) {
+                dst = q_out + ((first + tk) * pv.hq + hd) * pv.d + c;
+                if (pos < 0) xo = yo = make_uint4(0, 0, 0, 0);
+            } else {
+                if (state == 0) continue;
+                if (hd < (uint32_t)rot)
+                    dst = static_cast<T*>(const_cast<void*>(pv.k)) + k_of[tk] + (hd - pv.hq) * pv.kh + c;
+                else
+                    dst = static_cast<T*>(const_cast<void*>(pv.v)) + v_of[tk] + (hd - rot) * pv.vh + c;
+            }
+            if (cosb && hd < (uint32_t)rot && pos >= 0) {
+                float x[CH], y[CH];
+                widen16<T>(xo, x);
+                widen16<T>(yo, y);
+                const float4* cp = reinterpret_cast<const float4*>(cosb + (int64_t)pos * half + c);
+                const float4* sp = reinterpret_cast<const float4*>(sinb + (int64_t)pos * half + c);
+#pragma unroll
+                for (int k = 0; k < CH; k += 4) {
+                    const float4 co = __ldg(cp + k / 4), si = __ldg(sp + k / 4);
+                    const float cs[4] = {co.x, co.y, co.z, co.w}, sn[4] = {si.x, si.y, si.z, si.w};
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float a = x[k + e], d = y[k + e];
+                        x[k + e] = a * cs[e] - d * sn[e];
+                        y[k + e] = d * cs[e] + a * sn[e];
+                    }
+                }
+                xo = narrow16<T>(x);
+                yo = narrow16<T>(y);
+            }
+            *reinterpret_cast<uint4*>(dst) = xo;
+            *reinterpret_cast<uint4*>(dst + half) = yo;
+        }
     }
 }
 
@@ -882,13 +974,21 @@ extern "C" int smlm_paged_append(const void* qkv, void* k_pages, void* v_pages, 
                    "paged_append: qkv and the query output have to be 16-byte aligned");
     SMLM_CHECK_ARG((cos == nullptr) == (sin == nullptr) && (!cos || max_pos > 0),
                    "paged_append: cos and sin come together");
-    const int64_t all = batch * tokens * (hq + 2 * hkv) * (d / 2);
-    const int grid = (int)std::min<int64_t>((all + 255) / 256, (int64_t)sm_count() * 32);
+    SMLM_CHECK_ARG(!cos || ((uintptr_t)cos | (uintptr_t)sin) % 16 == 0, "paged_append: cos and sin have to be 16-byte "
+                   "aligned");
+    // few tokens: one a block (a decoding step's latency is one token's); many: enough for four pairs a thread
+    const int64_t all = batch * tokens, pairs = (hq + 2 * hkv) * (d / 2) * element_bytes(dtype) / 16;
+    const int64_t fill = std::max<int64_t>(1, APPEND_THREADS * APPEND_UNROLL / pairs);
+    const int per_block = (int)std::min<int64_t>({fill, APPEND_TOKENS, std::max<int64_t>(1, all / (sm_count() * 4))});
+    const int64_t grid = (all + per_block - 1) / per_block;
+    SMLM_CHECK_ARG(grid <= INT32_MAX && pairs <= 32768, "paged_append: %lld tokens of %lld bytes (at most 1 MiB each)",
+                   (long long)all, (long long)(pairs * 32));
+    const auto reciprocal = [](int64_t n) { return (uint32_t)(((int64_t(1) << 32) + n - 1) / n); };  // unused for 1
     return by_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        paged_append_kernel<T><<<grid, 256, 0, as_stream(stream)>>>(
+        paged_append_kernel<T><<<(unsigned)grid, APPEND_THREADS, 0, as_stream(stream)>>>(
             pv, static_cast<const T*>(qkv), (int)tokens, cos, sin, (int)std::min<int64_t>(max_pos, INT32_MAX),
-            static_cast<T*>(q_out), status);
+            static_cast<T*>(q_out), per_block, reciprocal(pairs), reciprocal(pairs / (hq + 2 * hkv)), status);
         SMLM_LAUNCHED("paged_append");
         return SMLM_OK;
     });

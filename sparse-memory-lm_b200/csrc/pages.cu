@@ -9,6 +9,7 @@
 namespace smlm {
 
 constexpr int PLAN_THREADS = 1024;
+constexpr int COPY_UNROLL = 4;
 
 struct Pages {
     int32_t* table;
@@ -85,21 +86,67 @@ __device__ __forceinline__ int block_scan(int v, int* total) {
     return x - v + (warp ? part[warp - 1] : 0);
 }
 
+// The blocks of one cluster that plan together (one to eight): phases that read what others wrote are separated by the
+// cluster's barrier, which costs a fraction of a kernel launch. What crosses blocks is read past L1 (__ldcg).
+struct Team {
+    int rank, size;
+    __device__ __forceinline__ Team() {
+        asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+        asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
+    }
+    __device__ __forceinline__ void sync() const {
+        if (size > 1)
+            asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        else
+            __syncthreads();
+    }
+    __device__ __forceinline__ int thread() const { return rank * PLAN_THREADS + threadIdx.x; }
+    __device__ __forceinline__ int threads() const { return size * PLAN_THREADS; }
+};
+constexpr int MAX_TEAM = 8;
+
+// Exclusive sum over the team's threads in order, of one value each; totals: MAX_TEAM ints in global memory. Every
+// thread of the team calls it; it passes one barrier.
+__device__ __forceinline__ int team_scan(const Team& team, int v, int32_t* totals, int* total) {
+    int mine;
+    const int x = block_scan(v, &mine);
+    if (team.size == 1) {
+        *total = mine;
+        return x;
+    }
+    if (threadIdx.x == 0) totals[team.rank] = mine;
+    team.sync();
+    int before = 0, all = 0;
+    for (int r = 0; r < team.size; r++) {
+        const int c = __ldcg(totals + r);
+        before += r < team.rank ? c : 0;
+        all += c;
+    }
+    *total = all;
+    return before + x;
+}
+
 // The free pages in increasing order: list[k] = the k-th free page, for k < most. Returns how many there are. Each
-// thread counts a contiguous piece, one scan gives its first rank.
-__device__ int list_free(const Pages& pg, int32_t* list, int most) {
-    const int per = (pg.n_pages + PLAN_THREADS - 1) / PLAN_THREADS;
-    const int a = min(pg.n_pages, (int)threadIdx.x * per), e = min(pg.n_pages, a + per);
+// thread counts a contiguous piece, one scan gives its first rank. Ends with a barrier.
+__device__ int list_free(const Team& team, const Pages& pg, int32_t* list, int most, int32_t* totals) {
+    const int per = (pg.n_pages + team.threads() - 1) / team.threads();
+    const int a = min(pg.n_pages, team.thread() * per), e = min(pg.n_pages, a + per);
+    uint32_t bits = 0;  // the first 32 of the piece, not to read them twice
     int count = 0, total;
-    for (int p = a; p < e; p++) count += __ldcg(pg.refcount + p) == 0;
-    int k = block_scan(count, &total);
-    for (int p = a; p < e && k < most; p++)
+    for (int p = a; p < e; p++)
+        if (__ldcg(pg.refcount + p) == 0) {
+            count++;
+            if (p - a < 32) bits |= 1u << (p - a);
+        }
+    int k = team_scan(team, count, totals, &total);
+    for (; bits && k < most; bits &= bits - 1) list[k++] = a + __ffs(bits) - 1;
+    for (int p = a + 32; p < e && k < most; p++)
         if (__ldcg(pg.refcount + p) == 0) list[k++] = p;
-    __syncthreads();
+    team.sync();
     return total;
 }
 
-// offset[i] = sum of need(0 .. i-1); returns the sum of all. need(i) is called once for each i < n.
+// offset[i] = sum of need(0 .. i-1); returns the sum of all. need(i) is called once for each i < n. One block.
 template <typename F>
 __device__ int scan_needs(int n, int32_t* offset, F need) {
     int sum = 0;
@@ -116,34 +163,41 @@ __device__ int scan_needs(int n, int32_t* offset, F need) {
 
 // lengths[r] += n_new for every listed row, with the pages that takes: rows in order, lowest free pages first. A row
 // whose pages are not there, or whose table is too narrow, stays as it is and raises a flag. The lengths are taken by
-// an exchange and put back at the end, which finds rows listed twice (the second does nothing).
+// an exchange and put back at the end, which finds rows listed twice (the second does nothing). Without a page to
+// hand out (most decoding steps) the counts are not read.
 __global__ void __launch_bounds__(PLAN_THREADS) pages_extend_kernel(Pages pg, const int32_t* rows, int n, int n_new,
                                                                     int shift, int32_t* offset, int32_t* len_of,
-                                                                    int32_t* list) {
+                                                                    int32_t* list, int32_t* totals) {
     constexpr int TAKEN = INT32_MIN;
+    const Team team;
     const int64_t cap = (int64_t)pg.max_blocks << shift;
     auto blocks = [&](int64_t len) { return (int)((len + (1 << shift) - 1) >> shift); };
     auto fits = [&](int len) { return len >= 0 && (int64_t)len + n_new <= cap; };
-    const int wanted = scan_needs(n, offset, [&](int i) {
-        const int r = rows[i];
-        const int len = r >= 0 && r < pg.table_rows ? atomicExch(pg.lengths + r, TAKEN) : TAKEN;
-        len_of[i] = len;
-        if (len == TAKEN || !fits(len)) flag(pg.status, SMLM_FLAG_INDEX_RANGE);
-        return len != TAKEN && fits(len) ? blocks((int64_t)len + n_new) - blocks(len) : 0;
-    });
-    const int have = wanted ? list_free(pg, list, wanted) : 0;
-    for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
-        const int len = len_of[i];
+    if (team.rank == 0) {
+        const int wanted = scan_needs(n, offset, [&](int i) {
+            const int r = rows[i];
+            const int len = r >= 0 && r < pg.table_rows ? atomicExch(pg.lengths + r, TAKEN) : TAKEN;
+            len_of[i] = len;
+            if (len == TAKEN || !fits(len)) flag(pg.status, SMLM_FLAG_INDEX_RANGE);
+            return len != TAKEN && fits(len) ? blocks((int64_t)len + n_new) - blocks(len) : 0;
+        });
+        if (threadIdx.x == 0) totals[MAX_TEAM] = wanted;
+    }
+    team.sync();
+    const int wanted = __ldcg(totals + MAX_TEAM);
+    const int have = wanted ? list_free(team, pg, list, wanted, totals) : 0;
+    for (int i = team.thread(); i < n; i += team.threads()) {
+        const int len = __ldcg(len_of + i);
         if (len == TAKEN) continue;
         bool grow = fits(len);
-        const int b0 = blocks(len), need = grow ? blocks((int64_t)len + n_new) - b0 : 0;
-        if (need && offset[i] + need > have) {
+        const int b0 = blocks(len), need = grow ? blocks((int64_t)len + n_new) - b0 : 0, off = __ldcg(offset + i);
+        if (need && off + need > have) {
             flag(pg.status, SMLM_FLAG_NO_PAGES);
             grow = false;
         }
         if (grow)
             for (int m = 0; m < need; m++) {
-                const int page = list[offset[i] + m];
+                const int page = __ldcg(list + off + m);
                 pg.table[rows[i] * pg.table_stride + b0 + m] = page;
                 pg.refcount[page] = 1;
             }
@@ -157,101 +211,117 @@ struct CopyList {
     int n;
 };
 
-// Row children[i] becomes a copy of row parents[i] as it was before the call, for all i at once.
+// Row children[i] becomes a copy of row parents[i] as it was before the call, for all i at once: the parents' entries
+// are read (with a reference more for each whole page, and one that holds the partly filled pages meanwhile) before
+// the children's are released, and pages are handed out after that. One warp per pair, lanes over its entries. The
+// time is the phases' chains of dependent loads, so each phase leaves what the next ones need side by side
+// (snap_len, cl.tokens, cl.src: -1 / 0 where nothing is to be done).
 __global__ void __launch_bounds__(PLAN_THREADS)
     pages_fork_kernel(Pages pg, const int32_t* parents, const int32_t* children, int n, int shift, int32_t* claim,
-                      int32_t* snap, int32_t* snap_len, int32_t* offset, int32_t* list, CopyList cl) {
-    const int mb = pg.max_blocks;
-    // a child listed twice takes its first parent; out-of-range rows are left out
-    for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
-        const int c = children[i];
-        if (c >= 0 && c < pg.table_rows) claim[c] = INT32_MAX;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += PLAN_THREADS)
-        if (row_ok(pg, children[i]) && row_ok(pg, parents[i])) atomicMin(claim + children[i], i);
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
+                      int32_t* snap, int32_t* snap_len, int32_t* offset, int32_t* list, int32_t* totals, CopyList cl) {
+    const Team team;
+    const int mb = pg.max_blocks, lane = lane_id();
+    const int warp0 = team.thread() >> 5, warps = team.threads() >> 5;
+    auto inside = [&](int r) { return r >= 0 && r < pg.table_rows; };
+    // of the pairs that list the same child one remains: the one whose number stays here
+    for (int i = team.thread(); i < n; i += team.threads()) {
         const int c = children[i], p = parents[i];
-        const bool in = c >= 0 && c < pg.table_rows && p >= 0 && p < pg.table_rows;
-        const bool mine = in && claim[c] == i;
-        if (in && !mine) flag(pg.status, SMLM_FLAG_INDEX_RANGE);
-        snap_len[i] = mine && c != p ? min(max(pg.lengths[p], 0), mb << shift) : -1;
+        if (inside(c) && inside(p)) claim[c] = i;
+        else flag(pg.status, SMLM_FLAG_INDEX_RANGE);
     }
-    __syncthreads();
-    // the parents' entries, one more reference for each whole page; the partly filled ones are held meanwhile
-    for (int64_t x = threadIdx.x; x < (int64_t)n * mb; x += PLAN_THREADS) {
-        const int i = x / mb, j = x % mb;
-        if (snap_len[i] < 0 || ((int64_t)j << shift) >= snap_len[i]) continue;
-        int e = pg.table[parents[i] * pg.table_stride + j];
-        if (e >= pg.n_pages) {
-            flag(pg.status, SMLM_FLAG_INDEX_RANGE);
-            e = -1;
-        }
-        snap[x] = e;
-        if (e >= 0) atomicAdd(pg.refcount + e, 1);
-    }
-    __syncthreads();
-    for (int64_t x = threadIdx.x; x < (int64_t)n * mb; x += PLAN_THREADS)
-        if (snap_len[x / mb] >= 0) drop_entry(pg, pg.table + children[x / mb] * pg.table_stride + x % mb);
-    __syncthreads();
-    auto part = [&](int i) {  // tokens in the partly filled last page
-        const int len = snap_len[i];
-        if (len < 0) return 0;
-        const int t = len & ((1 << shift) - 1);
-        return t && snap[(int64_t)i * mb + (len >> shift)] >= 0 ? t : 0;
-    };
-    const int wanted = scan_needs(n, offset, [&](int i) { return part(i) ? 1 : 0; });
-    const int have = wanted ? list_free(pg, list, wanted) : 0;
-    for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
-        int tokens = part(i);
-        if (tokens) {
-            const int64_t at = (int64_t)i * mb + (snap_len[i] >> shift);
-            const int src = snap[at];
-            atomicSub(pg.refcount + src, 1);
-            cl.src[i] = src;
-            if (offset[i] < have) {
-                const int dst = list[offset[i]];
-                cl.dst[i] = snap[at] = dst;
-                pg.refcount[dst] = 1;
-            } else {
-                flag(pg.status, SMLM_FLAG_NO_PAGES);
-                snap[at] = -1;
-                tokens = 0;
+    team.sync();
+    for (int i = warp0; i < n; i += warps) {
+        const int c = children[i], p = parents[i];
+        int len = -1, tokens = 0;
+        if (inside(c) && inside(p)) {
+            const int owner = __ldcg(claim + c), held = __ldcg(pg.lengths + p);
+            const int32_t* row = pg.table + p * pg.table_stride;
+            const int head = lane < mb ? row[lane] : -1;  // not waiting for the length
+            if (owner != i) {
+                if (lane == 0) flag(pg.status, SMLM_FLAG_INDEX_RANGE);
+            } else if (c != p) {
+                len = min(max(held, 0), mb << shift);
+                const int used = (len + (1 << shift) - 1) >> shift, rest = len & ((1 << shift) - 1);
+                for (int j = lane; j < used; j += 32) {
+                    int e = j < 32 ? head : row[j];
+                    if (e >= pg.n_pages) {
+                        flag(pg.status, SMLM_FLAG_INDEX_RANGE);
+                        e = -1;
+                    }
+                    snap[(int64_t)i * mb + j] = e;
+                    if (e >= 0) atomicAdd(pg.refcount + e, 1);
+                    if (rest && j == used - 1) {
+                        cl.src[i] = e;
+                        tokens = e >= 0 ? rest : 0;
+                    }
+                }
+                tokens = __reduce_add_sync(FULL, tokens);
             }
         }
-        cl.tokens[i] = tokens;
-        if (snap_len[i] >= 0) pg.lengths[children[i]] = snap_len[i];
+        if (lane == 0) {
+            snap_len[i] = len;
+            cl.tokens[i] = tokens;
+        }
     }
-    __syncthreads();
-    for (int64_t x = threadIdx.x; x < (int64_t)n * mb; x += PLAN_THREADS) {
-        const int i = x / mb, j = x % mb;
-        if (snap_len[i] >= 0 && ((int64_t)j << shift) < snap_len[i])
-            pg.table[children[i] * pg.table_stride + j] = snap[x];
+    team.sync();
+    if (team.rank == 0) {
+        const int wanted = scan_needs(n, offset, [&](int i) { return __ldcg(cl.tokens + i) ? 1 : 0; });
+        if (threadIdx.x == 0) totals[MAX_TEAM] = wanted;
+    }
+    for (int i = warp0; i < n; i += warps) {
+        const int len = __ldcg(snap_len + i), c = children[i];
+        if (!inside(c)) continue;
+        for (int j = lane; j < mb; j += 32) {
+            int32_t* entry = pg.table + c * pg.table_stride + j;
+            const int e = __ldcg(entry);
+            if (len < 0 || e < 0) continue;
+            *entry = -1;
+            if (e < pg.n_pages) atomicSub(pg.refcount + e, 1);
+            else flag(pg.status, SMLM_FLAG_INDEX_RANGE);
+        }
+    }
+    team.sync();
+    const int wanted = __ldcg(totals + MAX_TEAM);
+    const int have = wanted ? list_free(team, pg, list, wanted, totals) : 0;
+    for (int i = warp0; i < n; i += warps) {
+        const int len = __ldcg(snap_len + i), tokens = __ldcg(cl.tokens + i), src = __ldcg(cl.src + i);
+        const int off = __ldcg(offset + i), c = children[i];
+        if (len < 0) continue;
+        const int page = tokens && off < have ? __ldcg(list + off) : -1;
+        for (int j = lane; j << shift < len; j += 32)
+            pg.table[c * pg.table_stride + j] =
+                tokens && j == len >> shift ? page : __ldcg(snap + (int64_t)i * mb + j);
+        if (lane) continue;
+        pg.lengths[c] = len;
+        if (!tokens) continue;
+        atomicSub(pg.refcount + src, 1);
+        cl.dst[i] = page;
+        if (page >= 0) {
+            pg.refcount[page] = 1;
+        } else {
+            cl.tokens[i] = 0;
+            flag(pg.status, SMLM_FLAG_NO_PAGES);
+        }
     }
 }
 
 // With L pages in use: the k-th used page numbered L or above moves to the k-th free page below L. to[p] (p >= L) is
-// where page p went.
+// where page p went. Each thread has a contiguous piece of the pages; two scans give L and the ranks.
 __global__ void __launch_bounds__(PLAN_THREADS) pages_compact_kernel(Pages pg, int32_t* to, int32_t* live_out,
-                                                                     CopyList cl) {
-    const int per = (pg.n_pages + PLAN_THREADS - 1) / PLAN_THREADS;
-    const int a = min(pg.n_pages, (int)threadIdx.x * per), e = min(pg.n_pages, a + per);
-    int count = 0, live;
-    for (int p = a; p < e; p++) count += pg.refcount[p] > 0;
-    const int before = block_scan(count, &live);
-    __shared__ int used_below;  // used pages below L
-    if (a <= live && live < e) {
-        int k = before;
-        for (int p = a; p < live; p++) k += pg.refcount[p] > 0;
-        used_below = k;
-    }
-    if (threadIdx.x == 0 && live == pg.n_pages) used_below = live;
-    __syncthreads();
-    const int below = used_below, moves = live - below;
+                                                                     int32_t* totals, CopyList cl) {
+    const Team team;
+    const int per = (pg.n_pages + team.threads() - 1) / team.threads();
+    const int a = min(pg.n_pages, team.thread() * per), e = min(pg.n_pages, a + per);
+    int count = 0, live, below;
+    for (int p = a; p < e; p++) count += __ldcg(pg.refcount + p) > 0;
+    const int before = team_scan(team, count, totals, &live);
+    count = 0;  // of them below L
+    for (int p = a; p < min(e, live); p++) count += __ldcg(pg.refcount + p) > 0;
+    team_scan(team, count, totals + MAX_TEAM, &below);
+    const int moves = live - below;
     int used = before;
     for (int p = a; p < e; p++) {
-        const bool u = pg.refcount[p] > 0;
+        const bool u = __ldcg(pg.refcount + p) > 0;
         if (p < live) {
             if (!u) cl.dst[p - used] = p;
         } else {
@@ -260,14 +330,14 @@ __global__ void __launch_bounds__(PLAN_THREADS) pages_compact_kernel(Pages pg, i
         }
         used += u;
     }
-    if (threadIdx.x == 0) {
+    if (team.thread() == 0) {
         *cl.count = moves;
         *live_out = live;
     }
-    __syncthreads();
-    for (int k = threadIdx.x; k < moves; k += PLAN_THREADS) {
-        const int s = cl.src[k], d = cl.dst[k];
-        pg.refcount[d] = pg.refcount[s];
+    team.sync();
+    for (int k = team.thread(); k < moves; k += team.threads()) {
+        const int s = __ldcg(cl.src + k), d = __ldcg(cl.dst + k);
+        pg.refcount[d] = __ldcg(pg.refcount + s);
         pg.refcount[s] = 0;
         to[s] = d;
     }
@@ -301,8 +371,15 @@ __global__ void __launch_bounds__(256) pages_copy_kernel(char* pool, CopyList cl
         const char* s = pool + ((plane * n_pages + cl.src[i]) * heads + h) * page_bytes;
         char* d = pool + ((plane * n_pages + cl.dst[i]) * heads + h) * page_bytes;
         const int bytes = tokens * token_bytes;
-        for (int x = lane * 16; x < bytes; x += 512)
-            *reinterpret_cast<int4*>(d + x) = *reinterpret_cast<const int4*>(s + x);
+        for (int x0 = lane * 16; x0 < bytes; x0 += 512 * COPY_UNROLL) {
+            int4 v[COPY_UNROLL];
+#pragma unroll
+            for (int k = 0; k < COPY_UNROLL; k++)
+                if (x0 + 512 * k < bytes) v[k] = __ldcs(reinterpret_cast<const int4*>(s + x0 + 512 * k));
+#pragma unroll
+            for (int k = 0; k < COPY_UNROLL; k++)
+                if (x0 + 512 * k < bytes) __stcs(reinterpret_cast<int4*>(d + x0 + 512 * k), v[k]);
+        }
     }
 }
 
@@ -335,6 +412,25 @@ static int check_pool(const char* what, const void* pool, int64_t planes, int64_
                    "%s: %lld planes, %lld heads, %lld bytes per token and head (a multiple of 16 up to 4096)", what,
                    (long long)planes, (long long)heads, (long long)token_bytes);
     return SMLM_OK;
+}
+
+// Plans with one block for small caches, up to eight for large ones (`entries`: about how many threads it wants).
+template <typename... P, typename... A>
+static int launch_plan(void (*kernel)(P...), const char* what, int64_t entries, cudaStream_t st, A... args) {
+    int size = 1;
+    while (size < MAX_TEAM && (int64_t)size * PLAN_THREADS < entries) size *= 2;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(size);
+    cfg.blockDim = dim3(PLAN_THREADS);
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = size;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+    return e == cudaSuccess ? SMLM_OK : cuda_status(e, what);
 }
 
 static int copy_grid(int64_t most_units) {
@@ -383,6 +479,7 @@ extern "C" size_t smlm_pages_extend_workspace(int64_t n, int64_t n_pages) {
     ws.take<int32_t>(n);
     ws.take<int32_t>(n);
     ws.take<int32_t>(n_pages);
+    ws.take<int32_t>(2 * MAX_TEAM);
     return ws.used;
 }
 
@@ -401,14 +498,13 @@ extern "C" int smlm_pages_extend(int32_t* table, int64_t table_stride, int64_t t
     int32_t* offset = ws.take<int32_t>(n);
     int32_t* len_of = ws.take<int32_t>(n);
     int32_t* list = ws.take<int32_t>(n_pages);
+    int32_t* totals = ws.take<int32_t>(2 * MAX_TEAM);
     if (!workspace || !ws.ok()) {
         set_error("pages_extend: workspace of %zu bytes, %zu needed", workspace_bytes, ws.used);
         return SMLM_ERR_WORKSPACE;
     }
-    pages_extend_kernel<<<1, PLAN_THREADS, 0, as_stream(stream)>>>(pg, rows, (int)n, (int)n_new, log2_of(page_size),
-                                                                   offset, len_of, list);
-    SMLM_LAUNCHED("pages_extend");
-    return SMLM_OK;
+    return launch_plan(pages_extend_kernel, "pages_extend", std::max(n, n_pages / 4), as_stream(stream), pg, rows, (int)n,
+                       (int)n_new, log2_of(page_size), offset, len_of, list, totals);
 }
 
 extern "C" size_t smlm_pages_fork_workspace(int64_t n, int64_t table_rows, int64_t max_blocks, int64_t n_pages) {
@@ -417,6 +513,7 @@ extern "C" size_t smlm_pages_fork_workspace(int64_t n, int64_t table_rows, int64
     ws.take<int32_t>(n * max_blocks);
     for (int i = 0; i < 5; i++) ws.take<int32_t>(n);
     ws.take<int32_t>(n_pages);
+    ws.take<int32_t>(2 * MAX_TEAM);
     return ws.used;
 }
 
@@ -444,13 +541,14 @@ extern "C" int smlm_pages_fork(void* pool, int64_t planes, int64_t heads, int64_
     cl.tokens = ws.take<int32_t>(n);
     cl.n = (int)n;
     int32_t* list = ws.take<int32_t>(n_pages);
+    int32_t* totals = ws.take<int32_t>(2 * MAX_TEAM);
     if (!workspace || !ws.ok()) {
         set_error("pages_fork: workspace of %zu bytes, %zu needed", workspace_bytes, ws.used);
         return SMLM_ERR_WORKSPACE;
     }
-    pages_fork_kernel<<<1, PLAN_THREADS, 0, as_stream(stream)>>>(pg, parents, children, (int)n, log2_of(page_size),
-                                                                 claim, snap, snap_len, offset, list, cl);
-    SMLM_LAUNCHED("pages_fork: plan");
+    rc = launch_plan(pages_fork_kernel, "pages_fork: plan", std::max(32 * n, n_pages / 4), as_stream(stream), pg,
+                     parents, children, (int)n, log2_of(page_size), claim, snap, snap_len, offset, list, totals, cl);
+    if (rc != SMLM_OK) return rc;
     pages_copy_kernel<<<copy_grid(n * planes * heads), 256, 0, as_stream(stream)>>>(
         static_cast<char*>(pool), cl, (int)planes, (int)heads, (int)n_pages, (int)page_size, (int)token_bytes, pg,
         nullptr, nullptr);
@@ -462,6 +560,7 @@ extern "C" size_t smlm_pages_compact_workspace(int64_t n_pages) {
     WorkspaceSize ws;
     for (int i = 0; i < 3; i++) ws.take<int32_t>(n_pages);
     ws.take<int32_t>(2);
+    ws.take<int32_t>(2 * MAX_TEAM);
     return ws.used;
 }
 
@@ -480,12 +579,14 @@ extern "C" int smlm_pages_compact(void* pool, int64_t planes, int64_t heads, int
     cl.src = ws.take<int32_t>(n_pages);
     cl.dst = ws.take<int32_t>(n_pages);
     cl.count = ws.take<int32_t>(2);
+    int32_t* totals = ws.take<int32_t>(2 * MAX_TEAM);
     if (!workspace || !ws.ok()) {
         set_error("pages_compact: workspace of %zu bytes, %zu needed", workspace_bytes, ws.used);
         return SMLM_ERR_WORKSPACE;
     }
-    pages_compact_kernel<<<1, PLAN_THREADS, 0, as_stream(stream)>>>(pg, to, cl.count + 1, cl);
-    SMLM_LAUNCHED("pages_compact: plan");
+    rc = launch_plan(pages_compact_kernel, "pages_compact: plan", n_pages / 4, as_stream(stream), pg, to, cl.count + 1,
+                     totals, cl);
+    if (rc != SMLM_OK) return rc;
     pages_copy_kernel<<<copy_grid(n_pages / 2 * planes * heads), 256, 0, as_stream(stream)>>>(
         static_cast<char*>(pool), cl, (int)planes, (int)heads, (int)n_pages, (int)page_size, (int)token_bytes, pg, to,
         cl.count + 1);
