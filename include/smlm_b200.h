@@ -515,7 +515,8 @@ SMLM_API int smlm_paged_append(const void *qkv, void *k_pages, void *v_pages, in
 /* ------------------------------------------------------------------------------- pages of a paged cache
  * No counterpart in the reference. refcount (int32, n_pages): how many table entries hold each page, 0 = free; this
  * is the whole state of the allocator, and the lowest free page is always taken first. rows, parents, children:
- * device int32 row numbers; rows listed twice and rows outside the table set SMLM_FLAG_INDEX_RANGE. A sequence of n
+ * device int32 row numbers; negative ones are left out (so that lists can have a fixed length), rows listed twice and
+ * rows past the table set SMLM_FLAG_INDEX_RANGE. A sequence of n
  * tokens has ceil(n / page_size) entries, the later ones of its row being -1 (entries that smlm_pages_trim dropped
  * are -1 too). */
 

@@ -27,9 +27,10 @@ __device__ __forceinline__ void release(const Pages& pg, int page) {
     }
 }
 
+// Whether r is a row; negative numbers pad lists of a fixed length, larger ones are flagged.
 __device__ __forceinline__ bool row_ok(const Pages& pg, int r) {
     if (r >= 0 && r < pg.table_rows) return true;
-    flag(pg.status, SMLM_FLAG_INDEX_RANGE);
+    if (r >= 0) flag(pg.status, SMLM_FLAG_INDEX_RANGE);
     return false;
 }
 
@@ -176,9 +177,10 @@ __global__ void __launch_bounds__(PLAN_THREADS) pages_extend_kernel(Pages pg, co
     if (team.rank == 0) {
         const int wanted = scan_needs(n, offset, [&](int i) {
             const int r = rows[i];
-            const int len = r >= 0 && r < pg.table_rows ? atomicExch(pg.lengths + r, TAKEN) : TAKEN;
+            const bool ok = row_ok(pg, r);
+            const int len = ok ? atomicExch(pg.lengths + r, TAKEN) : TAKEN;
             len_of[i] = len;
-            if (len == TAKEN || !fits(len)) flag(pg.status, SMLM_FLAG_INDEX_RANGE);
+            if (ok && (len == TAKEN || !fits(len))) flag(pg.status, SMLM_FLAG_INDEX_RANGE);
             return len != TAKEN && fits(len) ? blocks((int64_t)len + n_new) - blocks(len) : 0;
         });
         if (threadIdx.x == 0) totals[MAX_TEAM] = wanted;
@@ -226,8 +228,7 @@ __global__ void __launch_bounds__(PLAN_THREADS)
     // of the pairs that list the same child one remains: the one whose number stays here
     for (int i = team.thread(); i < n; i += team.threads()) {
         const int c = children[i], p = parents[i];
-        if (inside(c) && inside(p)) claim[c] = i;
-        else flag(pg.status, SMLM_FLAG_INDEX_RANGE);
+        if (row_ok(pg, c) && row_ok(pg, p)) claim[c] = i;
     }
     team.sync();
     for (int i = warp0; i < n; i += warps) {

@@ -10,9 +10,10 @@ first add an Engram n-gram memory (smlm_b200.engram).
 
 Design of this module: the rotary tables are built once per model and sliced once per forward call for every
 layer (a _Positions object carries the call's cos / sin, cast once per dtype, and the static cache's visibility
-mask); attention has three cache modes, chosen by the cache the caller passes: none (training, prefill without a
-cache), a growing cache (the reference's decoding loop: {"k", "v"} concatenated per step) and a static cache
-(smlm_b200.decode.GraphDecoder: preallocated {"kbuf", "vbuf"}, positions on the device, fixed shapes).
+mask); attention has four cache modes, chosen by the cache the caller passes: none (training, prefill without a
+cache), a growing cache (the reference's decoding loop: {"k", "v"} concatenated per step), a static cache
+(smlm_b200.decode.GraphDecoder: preallocated {"kbuf", "vbuf"}, positions on the device, fixed shapes) and a paged
+cache (smlm_b200.decode.PagedDecoder: {"paged", "layer"}, a view of a smlm_b200.paged.PagedKVCache).
 """
 import math
 from dataclasses import asdict, dataclass, field
@@ -112,6 +113,10 @@ def _is_static(cache):
     return cache is not None and "kbuf" in cache
 
 
+def _is_paged(cache):
+    return cache is not None and "paged" in cache
+
+
 # ------------------------------------------------------------------------------------------- attention
 # backends that need no per-shape plan, for the growing cache (a new length every step)
 _GROWING_BACKENDS = [SDPBackend.FLASH_ATTENTION, SDPBackend.EFFICIENT_ATTENTION, SDPBackend.MATH]
@@ -130,6 +135,8 @@ class Attention(nn.Module):
     def forward(self, x, pos, cache=None):
         """x (B, T, d) -> (B, T, d). pos: the call's _Positions; cache: None, a growing or a static cache."""
         B, T, d = x.shape
+        if _is_paged(cache):
+            return self.wo(self._paged_cache(self.wqkv(x), cache, pos).reshape(B, T, d))
         # (B, T, 3 d) -> q, k, v each (B, heads, T, head_dim)
         q, k, v = self.wqkv(x).unflatten(-1, (3, self.n_heads, self.head_dim)).movedim(1, -2).unbind(1)
         cos, sin = pos.rope(q.dtype)
@@ -141,6 +148,21 @@ class Attention(nn.Module):
         else:
             y = self._growing_cache(q, k, v, cache)
         return self.wo(y.transpose(1, 2).reshape(B, T, d))
+
+    @staticmethod
+    def _paged_cache(qkv, cache, pos):
+        """Rotated keys and values into their pages; one token per sequence attends over the pages in place, several
+        (a prompt, or a chunk after cached tokens) over the gathered sequence."""
+        view, layer = cache["paged"], cache["layer"]
+        q = view.append(layer, qkv, pos.cos, pos.sin)
+        T = q.shape[1]
+        if T == 1:
+            return view.attend(layer, q[:, 0])
+        k, v = view.gather(layer)
+        seen = view.visible(T)
+        with sdpa_kernel(_GROWING_BACKENDS):
+            y = F.scaled_dot_product_attention(q.transpose(1, 2), k, v, attn_mask=seen, is_causal=seen is None)
+        return y.transpose(1, 2)
 
     @staticmethod
     def _growing_cache(q, k, v, cache):
@@ -333,6 +355,8 @@ class Transformer(nn.Module):
     # ----------------------------------------------------------------------------------------- forward
     def _positions(self, T, pos0, caches):
         first = caches[0] if caches else None
+        if _is_paged(first):              # positions follow from the cache's lengths, on the device
+            return _Positions(self.rope_cos, self.rope_sin)
         if _is_static(first):
             index = first["pos"]
             visible = first["arange"].view(1, -1) <= index.view(-1, 1)

@@ -234,3 +234,187 @@ def pages_compact(pool, table, refcount):
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _call("pages_compact", 2, dev, lib.smlm_pages_compact, pool.data_ptr(), planes, heads, token, table.data_ptr(),
           table.stride(0), *table.shape, refcount.data_ptr(), refcount.shape[0], page, ws.data_ptr(), nbytes)
+
+
+# ----------------------------------------------------------------------------------------------- the cache
+class PagedKVCache:
+    """Keys and values of up to max_seqs sequences for all layers of a model, in n_pages pages of page_size tokens.
+
+    A page number means the same page in every layer, so one table serves them all: pool (layers, 2, pages, key heads,
+    page_size, d), table (max_seqs, blocks), lengths, refcount as the functions above take them. The lengths and the
+    number of free pages are also known on the host (from the calls made here), so a call that would run out of pages
+    raises before anything is launched, without a synchronisation in steps that only grow sequences."""
+
+    def __init__(self, n_layers, n_pages, page_size, n_kv_heads, head_dim, max_seqs, max_len, dtype=torch.bfloat16,
+                 device="cuda"):
+        if page_size < 1 or page_size > 4096 or page_size & (page_size - 1):
+            raise ValueError(f"page_size {page_size} (a power of two up to 4096)")
+        if dtype not in _CODES:
+            raise ValueError(f"unsupported type {dtype} (fp32, bf16 or fp16)")
+        if head_dim % 16 or not 16 <= head_dim <= 256:
+            raise ValueError(f"head dimension {head_dim} (a multiple of 16 up to 256)")
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError("PagedKVCache runs on CUDA (there is no CPU path)")
+        self.page_size, self.max_seqs, self.max_len = page_size, max_seqs, max_len
+        blocks = -(-max_len // page_size)
+        self.pool = torch.zeros(n_layers, 2, n_pages, n_kv_heads, page_size, head_dim, dtype=dtype, device=device)
+        self.table = torch.full((max_seqs, blocks), -1, dtype=torch.int32, device=device)
+        self.lengths = torch.zeros(max_seqs, dtype=torch.int32, device=device)
+        self.refcount = torch.zeros(n_pages, dtype=torch.int32, device=device)
+        self.version = 0                  # counts the pools (resize makes a new one; a captured graph reads the old)
+        self._len = [0] * max_seqs
+        self._free = n_pages              # free pages, None: to be counted again
+
+    @classmethod
+    def for_model(cls, model, max_seqs, max_len=None, page_size=16, n_pages=None, dtype=torch.bfloat16):
+        """A cache of the model's shape; n_pages defaults to what max_seqs sequences of max_len tokens need."""
+        cfg = model.cfg
+        max_len = max_len or cfg.max_seq_len
+        if n_pages is None:
+            n_pages = max_seqs * -(-max_len // page_size)
+        return cls(cfg.n_layers, n_pages, page_size, cfg.n_heads, cfg.head_dim, max_seqs, max_len, dtype,
+                   model.tok_emb.weight.device)
+
+    def _rows(self, rows):
+        rows = list(rows)
+        for r in rows:
+            if not 0 <= r < self.max_seqs:
+                raise ValueError(f"sequence {r} of {self.max_seqs}")
+        if len(set(rows)) < len(rows):
+            raise ValueError(f"sequences listed twice: {rows}")
+        return rows
+
+    def _device(self, rows):
+        return torch.tensor(rows, dtype=torch.int32, device=self.table.device)
+
+    def length(self, row):
+        return self._len[row]
+
+    def free_pages(self):
+        """Pages no sequence holds (reads them from the device if a call since has released some)."""
+        if self._free is None:
+            self._free = int((self.refcount == 0).sum())
+        return self._free
+
+    def _take(self, need, what):
+        # the count known is exact, so a shortage is one; shared pages make releases unpredictable, hence None above
+        if need > self.free_pages():
+            raise RuntimeError(f"{what}: {need} pages needed, {self._free} of {self.refcount.shape[0]} free")
+        self._free -= need
+
+    def reserve(self, rows, n):
+        """Host side of extend: checks and counts n more tokens for each of `rows`."""
+        p = self.page_size
+        for r in rows:
+            if self._len[r] + n > self.max_len:
+                raise ValueError(f"sequence {r}: {self._len[r]} + {n} tokens, max_len {self.max_len}")
+        self._take(sum(-(-(self._len[r] + n) // p) - -(-self._len[r] // p) for r in rows), "PagedKVCache.extend")
+        for r in rows:
+            self._len[r] += n
+
+    def extend(self, rows, n):
+        """Room for n more tokens of each of the sequences `rows` (their lengths grow by n; paged_append fills it)."""
+        rows = self._rows(rows)
+        self.reserve(rows, n)
+        pages_extend(self.table, self.lengths, self.refcount, self._device(rows), n, self.page_size)
+
+    def fork(self, parents, children):
+        """children[i] becomes a copy of parents[i] (as both were before the call). Needs a free page for every child
+        whose parent's last page is partly filled."""
+        children, parents = self._rows(children), list(parents)
+        for r in parents:
+            self._rows([r])
+        if len(parents) != len(children):
+            raise ValueError(f"{len(parents)} parents, {len(children)} children")
+        need = sum(self._len[p] % self.page_size > 0 for p, c in zip(parents, children) if p != c)
+        if need > self.free_pages():
+            raise RuntimeError(f"PagedKVCache.fork: {need} pages needed, {self._free} of {self.refcount.shape[0]} free")
+        pages_fork(self.pool, self.table, self.lengths, self.refcount, self._device(parents), self._device(children))
+        self._free = None
+        for c, n in zip(children, [self._len[p] for p in parents]):
+            self._len[c] = n
+
+    def free(self, rows):
+        """The sequences end; pages that no other sequence shares become free."""
+        rows = self._rows(rows)
+        pages_free(self.table, self.lengths, self.refcount, self._device(rows))
+        self._free = None
+        for r in rows:
+            self._len[r] = 0
+
+    def trim(self, rows, window, sinks=0):
+        """Releases the pages that attention with this window and these sinks no longer reads. (A trimmed sequence can
+        only be attended with a window and sinks no larger than these.)"""
+        rows = self._rows(rows)
+        pages_trim(self.table, self.lengths, self.refcount, self._device(rows), self.page_size, window, sinks)
+        self._free = None
+
+    def compact(self):
+        """Moves the pages in use to the lowest numbers; returns how many there are (synchronises)."""
+        pages_compact(self.pool, self.table, self.refcount)
+        self._free = None
+        return self.refcount.shape[0] - self.free_pages()
+
+    def resize(self, n_pages):
+        """A pool of n_pages pages (at least those in use) in place of this one: compacts, then copies the pages in
+        use. Graphs captured over the old pool do not follow (version changes)."""
+        used = self.compact()
+        if n_pages < used:
+            raise ValueError(f"{used} pages are in use, {n_pages} wanted")
+        L_, two, _, h, p, d = self.pool.shape
+        pool = torch.zeros(L_, two, n_pages, h, p, d, dtype=self.pool.dtype, device=self.pool.device)
+        pool[:, :, :used] = self.pool[:, :, :used]
+        count = torch.zeros(n_pages, dtype=torch.int32, device=self.pool.device)
+        count[:used] = self.refcount[:used]
+        self.pool, self.refcount, self._free = pool, count, n_pages - used
+        self.version += 1
+
+    def view(self, rows=None, window=0, sinks=0):
+        """What a forward pass over these sequences (all of them by default) passes to the model."""
+        if rows is None:
+            return PagedView(self, self.table, self.lengths, None, window, sinks)
+        rows = self._rows(rows)
+        held = {self._len[r] for r in rows}
+        if len(held) > 1:
+            raise ValueError(f"sequences of one length, got {sorted(held)}")
+        at = torch.tensor(rows, device=self.table.device)
+        return PagedView(self, self.table[at], self.lengths[at], held.pop(), window, sinks)
+
+
+class PagedView:
+    """Some sequences of a PagedKVCache for one forward pass: their table rows and lengths, the length they all have (for
+    passes of several tokens; None: any), and the window and sinks of the attention."""
+
+    def __init__(self, cache, table, lengths, held, window, sinks):
+        self.cache, self.table, self.lengths, self.held = cache, table, lengths, held
+        self.window, self.sinks = window, sinks
+
+    def caches(self):
+        """The kv_caches argument of Transformer.forward."""
+        return [{"paged": self, "layer": i} for i in range(self.cache.pool.shape[0])]
+
+    def append(self, layer, qkv, cos, sin):
+        k, v = self.cache.pool[layer]
+        return paged_append(qkv, k, v, self.table, self.lengths, cos, sin)
+
+    def attend(self, layer, q):
+        k, v = self.cache.pool[layer]
+        return paged_attention(q, k, v, self.table, self.lengths, window=self.window, sinks=self.sinks)
+
+    def gather(self, layer):
+        """keys and values of the sequences, (B, heads, held, d) each (trimmed pages as page 0: masked by the window)."""
+        out = self.cache.pool[layer][:, self.table.clamp(min=0).long()].transpose(2, 3).flatten(3, 4)
+        return out[0, :, :, :self.held], out[1, :, :, :self.held]
+
+    def visible(self, tokens):
+        """(tokens, held) bool: what each of the last `tokens` positions sees; None: all before it (plain causal)."""
+        n = self.held
+        if n == tokens and (not self.window or self.window >= n):
+            return None
+        dev = self.table.device
+        j, t = torch.arange(n, device=dev)[None], torch.arange(n - tokens, n, device=dev)[:, None]
+        seen = j <= t
+        if self.window:
+            seen &= (j > t - self.window) | (j < self.sinks)
+        return seen
