@@ -25,7 +25,6 @@ namespace smlm {
 constexpr int SPLIT_WARPS = 4, SPLIT_THREADS = SPLIT_WARPS * 32;
 constexpr int JOIN_THREADS = 256;
 constexpr int HEAD = 2;  // what beginning an item costs, in tiles (two dependent loads and the output), in the cut
-constexpr int QT = 8;  // query heads per item
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -60,15 +59,14 @@ __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, u
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// fp32 operands as tf32 hi + lo: x = hi + lo up to 2^-22 of x. fin is hi without infinities and NaN, for the products
-// with a lo, whose sign and zeros would turn an infinite product into a NaN.
+// fp32 operands as tf32 hi + lo: x = hi + lo up to 2^-22 of x (KEEP: not to be computed once and held in registers)
+template <bool KEEP = false>
 struct Split32 {
-    uint32_t hi, lo, fin;
+    uint32_t hi, lo;
     __device__ __forceinline__ explicit Split32(uint32_t bits) {
-        asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(__uint_as_float(bits)));
-        const bool finite = (hi & 0x7f800000u) != 0x7f800000u;
-        lo = finite ? __float_as_uint(__uint_as_float(bits) - __uint_as_float(hi)) : 0;
-        fin = finite ? hi : 0;
+        if constexpr (KEEP) asm volatile("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(__uint_as_float(bits)));
+        else asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(__uint_as_float(bits)));
+        lo = __float_as_uint(__uint_as_float(bits) - __uint_as_float(hi));
     }
 };
 __device__ __forceinline__ void mma8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -79,11 +77,12 @@ __device__ __forceinline__ void mma8(float (&c)[4], uint32_t a0, uint32_t a1, ui
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+template <bool KEEP>
 __device__ __forceinline__ void mma_split32(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                            const Split32& b0, const Split32& b1) {
-    const Split32 x0(a0), x1(a1), x2(a2), x3(a3);
-    mma8(c, x0.lo, x1.lo, x2.lo, x3.lo, b0.fin, b1.fin);
-    mma8(c, x0.fin, x1.fin, x2.fin, x3.fin, b0.lo, b1.lo);
+                                            const Split32<KEEP>& b0, const Split32<KEEP>& b1) {
+    const Split32<> x0(a0), x1(a1), x2(a2), x3(a3);
+    mma8(c, x0.lo, x1.lo, x2.lo, x3.lo, b0.hi, b1.hi);
+    mma8(c, x0.hi, x1.hi, x2.hi, x3.hi, b0.lo, b1.lo);
     mma8(c, x0.hi, x1.hi, x2.hi, x3.hi, b0.hi, b1.hi);
 }
 
@@ -101,6 +100,31 @@ template <typename T>
 __device__ __forceinline__ float2 unpack16(uint32_t p) {
     if constexpr (std::is_same_v<T, __half>) return __half22float2(*reinterpret_cast<const __half2*>(&p));
     else return make_float2(bf16_bits_to_f32(p & 0xffffu), __uint_as_float(p & 0xffff0000u));
+}
+
+template <typename T>
+__device__ __forceinline__ void widen16(const uint4& v, float (&f)[16 / sizeof(T)]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4) {
+            f[i] = __uint_as_float(w[i]);
+        } else {
+            const float2 p = unpack16<T>(w[i]);
+            f[2 * i] = p.x;
+            f[2 * i + 1] = p.y;
+        }
+    }
+}
+template <typename T>
+__device__ __forceinline__ uint4 narrow16(const float (&f)[16 / sizeof(T)]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(f[i]);
+        else w[i] = pack16<T>(f[2 * i], f[2 * i + 1]);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // The tiles of one sequence: all of [0, n), or with a window those of the first tokens and of [lo, n).
@@ -138,41 +162,391 @@ struct SplitWork {
     int2* cut;  // (batch, items): the workers of the item's first and last tile; x = -1: not cut
     float* ml;  // (slots, rows, 2): running maximum and sum
     float* o;   // (slots, rows, dp)
-    int rows, dp;  // rows = min(group, QT)
+    int rows, dp;  // rows = min(group, query heads of an item)
 };
 
-__device__ __forceinline__ int group_tiles(const PageView& pv) { return (pv.hq / pv.hkv + QT - 1) / QT; }
-
-template <typename T, int DP>
+// NT: eights of query heads an item has (two where a group has more than eight and the registers allow it).
+template <typename T, int DP, int NT>
 struct SplitShape {
     static constexpr int ES = sizeof(T);
     static constexpr int CH = 16 / ES;                   // elements of a 16-byte load
-    static constexpr int TT = ES == 2 && DP <= 64 ? 32 : 16;  // tokens per tile: 64 registers of keys and values
+    static constexpr int TT = ES == 2 && DP <= 64 && NT == 1 ? 32 : 16;  // tokens per tile: 64 registers
     static constexpr int NS = TT / 16;
     static constexpr int KJ = DP / (4 * CH);             // loads per key row and lane
     static constexpr int VB = DP >= 8 * CH ? DP / (8 * CH) : 1;  // loads per value row and lane
     static constexpr int MT = ES == 2 ? 4 : 2;           // 16-row tiles of O^T per value load
-    static constexpr bool WIDE = DP * ES > 256;          // queries from shared memory, values loaded after the scores
-    static constexpr int BLOCKS = DP * ES <= 128 ? 4 : DP * ES <= 256 ? 3 : 2;  // resident per SM (registers)
+    static constexpr int QT = 8 * NT;
+    // rows of more than 256 bytes: queries from shared memory, values loaded after the scores; of 1 KB: keys and
+    // values in two halves
+    static constexpr bool WIDE = DP * ES > 256, HALVES = DP * ES > 512;
+    static constexpr int KK = HALVES ? KJ / 2 : KJ, VR = HALVES ? 2 : 4;
+    static constexpr int BLOCKS = DP * ES * NT <= 128 ? 4 : DP * ES * NT <= 256 ? 3 : 2;  // per SM (registers)
 };
 
-// SMALL: pages of fewer than 16 tokens, whose tokens are looked up one by one (PART: d < DP).
-template <typename T, int DP, bool PART, bool SMALL>
-__global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP>::BLOCKS)
+// Tiles first .. last - 1 of one item by one warp: the sums of its columns. PART: d < DP; SMALL: pages of fewer than
+// 16 tokens, whose tokens are looked up one by one.
+template <typename T, int DP, int NT, bool PART, bool SMALL>
+struct Stream {
+    using S = SplitShape<T, DP, NT>;
+    static constexpr int CH = S::CH, TT = S::TT, NS = S::NS, KJ = S::KJ, KK = S::KK, VB = S::VB, VR = S::VR, MT = S::MT;
+    static constexpr bool WIDE = S::WIDE, HALVES = S::HALVES, F = S::ES == 4;
+    static constexpr unsigned ALL = TT == 32 ? FULL : 0xffffu;
+    struct PagesOf {  // the pages of a tile: SMALL: of token `lane`; else of each 16 tokens (the same in all lanes)
+        int p[SMALL ? 1 : NS];
+    };
+
+    float o[NT][VB * MT][4];
+    float m[NT][2], l[NT][2];  // columns 2 t4 and 2 t4 + 1 of each eight
+
+    // Lane's share of the loads: keys of tokens g, g + 8 of 16; values as value_token says; see the head of this part.
+    static __device__ __forceinline__ int value_token(int s, int r) {
+        const int t4 = lane_id() & 3;
+        return 16 * s + (F ? t4 + 4 * r : 2 * t4 + (r & 1) + 8 * (r >> 1));
+    }
+
+    __device__ __forceinline__ void scores(float (&sc)[NT][NS][4], const uint4 (&kr)[NS][2][KK],
+                                           const uint4 (&qf)[NT][WIDE ? 1 : KJ], const uint4* qs, int j0) {
+#pragma unroll
+        for (int s = 0; s < NS; s++)
+#pragma unroll
+            for (int jj = 0; jj < KK; jj++) {
+                const uint4 a = kr[s][0][jj], e = kr[s][1][jj];
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    uint4 w;
+                    if constexpr (WIDE) w = qs[(n * KJ + j0 + jj) * 32 + lane_id()];
+                    else w = qf[n][jj];
+                    if constexpr (F) {
+                        constexpr bool KEEP = DP > 64;  // the split queries have no registers there
+                        mma_split32(sc[n][s], a.x, e.x, a.y, e.y, Split32<KEEP>(w.x), Split32<KEEP>(w.y));
+                        mma_split32(sc[n][s], a.z, e.z, a.w, e.w, Split32<KEEP>(w.z), Split32<KEEP>(w.w));
+                    } else {
+                        mma16<T>(sc[n][s], a.x, e.x, a.y, e.y, w.x, w.y);
+                        mma16<T>(sc[n][s], a.z, e.z, a.w, e.w, w.z, w.w);
+                    }
+                }
+            }
+    }
+
+    // qs: this warp's shared memory, NT KJ 32 vectors (WIDE)
+    __device__ __forceinline__ void run(const PageView& pv, const T* q, float c, const Span& span, int b, int h, int q0,
+                                        int first, int last, uint4* qs, int* status) {
+        const int lane = lane_id(), g = lane >> 2, t4 = lane & 3, group = pv.hq / pv.hkv;
+        const int shift = pv.page_shift, slots = (1 << shift) - 1;
+        const uint32_t kpb = pv.kp * S::ES, ktb = pv.kt * S::ES, vpb = pv.vp * S::ES, vtb = pv.vt * S::ES;  // bytes
+        const int32_t* row = pv.table + b * pv.table_stride;
+        auto entry = [&](int t) {  // the page of token t, or -1 past the end, in a hole or outside the pool
+            int p = -1;
+            if (t < span.n) {
+                p = __ldg(row + (t >> shift));
+                if (p >= pv.n_pages) {
+                    flag(status, SMLM_FLAG_INDEX_RANGE);
+                    p = -1;
+                }
+            }
+            return p;
+        };
+        auto pages_at = [&](int i) {
+            const int t0 = span.token(i, TT);
+            PagesOf x;
+            if constexpr (SMALL) {
+                x.p[0] = lane < TT ? entry(t0 + lane) : -1;
+            } else {
+#pragma unroll
+                for (int s = 0; s < NS; s++) x.p[s] = entry(t0 + 16 * s);
+            }
+            return x;
+        };
+        auto seen_of = [&](int i, const PagesOf& x) {  // which of the tile's tokens are seen
+            const int t0 = span.token(i, TT);
+            bool whole = t0 + TT <= span.n && (t0 >= span.lo || t0 + TT <= span.sinks);
+            if constexpr (!SMALL) {
+#pragma unroll
+                for (int s = 0; s < NS; s++) whole = whole && x.p[s] >= 0;
+                if (whole) return ALL;
+                const int p = lane < 16 ? x.p[0] : x.p[NS - 1];
+                return __ballot_sync(FULL, lane < TT && p >= 0 && span.sees(t0 + lane));
+            } else {
+                return __ballot_sync(FULL, x.p[0] >= 0 && span.sees(t0 + lane));
+            }
+        };
+        PagesOf pages = pages_at(first), pages_next;
+        const T* qp = q + ((int64_t)b * pv.hq + h * group) * pv.d;
+        uint4 qf[NT][WIDE ? 1 : KJ];
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int j = 0; j < KJ; j++) {
+                const int d0 = (t4 + 4 * j) * CH, qrow = q0 + 8 * n + g;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (qrow < group && (!PART || d0 < pv.d)) v = load16(qp + (int64_t)qrow * pv.d + d0);
+                if constexpr (WIDE) qs[(n * KJ + j) * 32 + lane] = v;  // read back by the same lane only
+                else qf[n][j] = v;
+            }
+        const char* kp = reinterpret_cast<const char*>(static_cast<const T*>(pv.k) + h * pv.kh + t4 * CH);
+        const char* vp = reinterpret_cast<const char*>(static_cast<const T*>(pv.v) + h * pv.vh);
+        uint4 kr[NS][2][KK], vr[NS][VR][VB];
+        // Tokens that are not seen are loaded all the same, from their own page or page 0 (mapped memory), and masked.
+        auto load_keys = [&](int i, const PagesOf& x, int j0) {
+            const int t0 = span.token(i, TT);
+#pragma unroll
+            for (int s = 0; s < NS; s++) {
+                const char* base = kp;
+                if constexpr (!SMALL)
+                    base += (uint64_t)(uint32_t)max(x.p[s], 0) * kpb + (uint64_t)(uint32_t)((t0 + 16 * s) & slots) * ktb +
+                            (uint64_t)(uint32_t)g * ktb;
+#pragma unroll
+                for (int r = 0; r < 2; r++) {
+                    const char* src;
+                    if constexpr (SMALL) {
+                        const int y = 16 * s + 8 * r + g;
+                        const int p = max(__shfl_sync(FULL, x.p[0], y), 0);
+                        src = kp + (uint64_t)(uint32_t)p * kpb + (uint64_t)(uint32_t)((t0 + y) & slots) * ktb;
+                    } else {
+                        src = base + (uint64_t)(8 * r) * ktb;
+                    }
+#pragma unroll
+                    for (int j = 0; j < KK; j++) {
+                        if (!PART || (t4 + 4 * (j0 + j)) * CH < pv.d) kr[s][r][j] = load16(src + 64 * (j0 + j));
+                        else kr[s][r][j] = make_uint4(0, 0, 0, 0);
+                    }
+                }
+            }
+        };
+        auto load_values = [&](int i, const PagesOf& x, int first_row) {
+            const int t0 = span.token(i, TT);
+#pragma unroll
+            for (int s = 0; s < NS; s++) {
+                const char* base = vp;
+                if constexpr (!SMALL)
+                    base += (uint64_t)(uint32_t)max(x.p[s], 0) * vpb + (uint64_t)(uint32_t)((t0 + 16 * s) & slots) * vtb +
+                            (uint64_t)(uint32_t)(F ? t4 : 2 * t4) * vtb;
+#pragma unroll
+                for (int rr = 0; rr < VR; rr++) {
+                    const int r = first_row + rr;
+                    const char* src;
+                    if constexpr (SMALL) {
+                        const int y = value_token(s, r);
+                        const int p = max(__shfl_sync(FULL, x.p[0], y), 0);
+                        src = vp + (uint64_t)(uint32_t)p * vpb + (uint64_t)(uint32_t)((t0 + y) & slots) * vtb;
+                    } else {
+                        src = base + (uint64_t)(F ? 4 * r : (r & 1) + 8 * (r >> 1)) * vtb;
+                    }
+#pragma unroll
+                    for (int vb = 0; vb < VB; vb++) {
+                        const int d0 = (g + 8 * vb) * CH;  // columns past d are not stored
+                        const bool in = (!PART && DP >= 8 * CH) || d0 < pv.d;
+                        vr[s][rr][vb] = load16(src + (in ? 16 * g + 128 * vb : 0));
+                    }
+                }
+            }
+        };
+        auto clear_unseen = [&](unsigned seen, int first_row) {  // 0 * (a stale infinity or NaN) is not 0
+#pragma unroll
+            for (int s = 0; s < NS; s++)
+#pragma unroll
+                for (int r = 0; r < VR; r++)
+                    if (!(seen >> value_token(s, first_row + r) & 1)) {
+#pragma unroll
+                        for (int vb = 0; vb < VB; vb++) vr[s][r][vb] = make_uint4(0, 0, 0, 0);
+                    }
+        };
+
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            m[n][0] = m[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+            for (int i = 0; i < VB * MT; i++) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+        }
+        load_keys(first, pages, 0);
+        if (!WIDE) load_values(first, pages, 0);
+        if (first + 1 < last) pages_next = pages_at(first + 1);
+        for (int i = first; i < last; i++) {
+            float sc[NT][NS][4];
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int s = 0; s < NS; s++) sc[n][s][0] = sc[n][s][1] = sc[n][s][2] = sc[n][s][3] = 0.f;
+            scores(sc, kr, qf, qs, 0);
+            if constexpr (HALVES) {
+                load_keys(i, pages, KK);
+                scores(sc, kr, qf, qs, KK);
+            }
+            if constexpr (F) {  // inf - inf in a split operand? Then once more, product by product
+                const bool odd = !(sc[0][0][0] == sc[0][0][0] && sc[0][0][1] == sc[0][0][1] &&
+                                   sc[0][0][2] == sc[0][0][2] && sc[0][0][3] == sc[0][0][3]);
+                if (__any_sync(FULL, odd)) {
+                    const int t0 = span.token(i, TT);
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        const int y = g + 8 * (x >> 1), col = q0 + 2 * t4 + (x & 1);
+                        int p = pages.p[0];
+                        if constexpr (SMALL) p = __shfl_sync(FULL, p, y);
+                        const T* src = static_cast<const T*>(pv.k) + h * pv.kh + max(p, 0) * pv.kp +
+                                       ((t0 + y) & slots) * pv.kt;
+                        float sum = 0.f;
+                        if (col < group) {
+#pragma unroll 1
+                            for (int d = 0; d < pv.d; d++) sum = fmaf(src[d], qp[(int64_t)col * pv.d + d], sum);
+                        }
+                        sc[0][0][x] = sum;
+                    }
+                }
+            }
+            if (WIDE) load_values(i, pages, 0);
+            const unsigned seen = seen_of(i, pages);
+            if (!WIDE && i + 1 < last) load_keys(i + 1, pages_next, 0);
+            if (seen != ALL && !WIDE) clear_unseen(seen, 0);
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+#pragma unroll
+                for (int s = 0; s < NS; s++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++) sc[n][s][x] *= c;
+                if (seen != ALL) {
+#pragma unroll
+                    for (int s = 0; s < NS; s++)
+#pragma unroll
+                        for (int r = 0; r < 2; r++)
+                            if (!(seen >> (16 * s + 8 * r + g) & 1)) sc[n][s][2 * r] = sc[n][s][2 * r + 1] = -INFINITY;
+                }
+                float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+                for (int s = 0; s < NS; s++)
+#pragma unroll
+                    for (int r = 0; r < 2; r++) {
+                        x0 = fmaxf(x0, sc[n][s][2 * r]);
+                        x1 = fmaxf(x1, sc[n][s][2 * r + 1]);
+                    }
+#pragma unroll
+                for (int w = 4; w < 32; w <<= 1) {
+                    x0 = fmaxf(x0, __shfl_xor_sync(FULL, x0, w));
+                    x1 = fmaxf(x1, __shfl_xor_sync(FULL, x1, w));
+                }
+                if (__any_sync(FULL, x0 > m[n][0] || x1 > m[n][1])) {
+                    const float n0 = fmaxf(m[n][0], x0), n1 = fmaxf(m[n][1], x1);
+                    const float f0 = m[n][0] == n0 ? 1.f : ex2(m[n][0] - n0), f1 = m[n][1] == n1 ? 1.f : ex2(m[n][1] - n1);
+                    m[n][0] = n0;
+                    m[n][1] = n1;
+                    l[n][0] *= f0;
+                    l[n][1] *= f1;
+#pragma unroll
+                    for (int x = 0; x < VB * MT; x++) {
+                        o[n][x][0] *= f0;
+                        o[n][x][1] *= f1;
+                        o[n][x][2] *= f0;
+                        o[n][x][3] *= f1;
+                    }
+                }
+                const float z0 = m[n][0] == -INFINITY ? 0.f : m[n][0], z1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
+#pragma unroll
+                for (int s = 0; s < NS; s++)
+#pragma unroll
+                    for (int r = 0; r < 2; r++) {
+                        sc[n][s][2 * r] = ex2(sc[n][s][2 * r] - z0);
+                        sc[n][s][2 * r + 1] = ex2(sc[n][s][2 * r + 1] - z1);
+                        l[n][0] += sc[n][s][2 * r];
+                        l[n][1] += sc[n][s][2 * r + 1];
+                    }
+            }
+            if (WIDE && seen != ALL) clear_unseen(seen, 0);
+            if constexpr (F) {
+#pragma unroll
+                for (int s = 0; s < NS; s++)
+#pragma unroll
+                    for (int r = 0; r < 2; r++) {  // tokens 8 r .. 8 r + 7 of the 16
+                        if (HALVES && r) {
+                            load_values(i, pages, 2);
+                            if (seen != ALL) clear_unseen(seen, 2);
+                        }
+                        // P^T: weight of token t4 (+ 4) for query g, from lane (token, query / 2)
+                        const int from = 4 * t4 + (g >> 1);
+                        const float a = __shfl_sync(FULL, sc[0][s][2 * r], from);
+                        const float b1 = __shfl_sync(FULL, sc[0][s][2 * r + 1], from);
+                        const float a4 = __shfl_sync(FULL, sc[0][s][2 * r], from + 16);
+                        const float b4 = __shfl_sync(FULL, sc[0][s][2 * r + 1], from + 16);
+                        const Split32<> p0(__float_as_uint(g & 1 ? b1 : a)), p1(__float_as_uint(g & 1 ? b4 : a4));
+#pragma unroll
+                        for (int vb = 0; vb < VB; vb++) {
+                            const uint4 x = vr[s][HALVES ? 0 : 2 * r][vb], y = vr[s][HALVES ? 1 : 2 * r + 1][vb];
+                            mma_split32(o[0][vb * MT], x.x, x.y, y.x, y.y, p0, p1);
+                            mma_split32(o[0][vb * MT + 1], x.z, x.w, y.z, y.w, p0, p1);
+                        }
+                    }
+            } else {
+#pragma unroll
+                for (int s = 0; s < NS; s++) {
+                    uint32_t hi[NT][2], lo[NT][2];  // P^T: tokens 0 .. 7 and 8 .. 15 of the 16
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int r = 0; r < 2; r++) {
+                            const float x = sc[n][s][2 * r], y = sc[n][s][2 * r + 1];
+                            const uint32_t w = pack16<T>(x, y);
+                            const float2 u = unpack16<T>(w);
+                            hi[n][r] = transpose8x8(w);
+                            lo[n][r] = transpose8x8(pack16<T>(x - u.x, y - u.y));
+                        }
+#pragma unroll
+                    for (int vb = 0; vb < VB; vb++) {
+                        const uint4 x = vr[s][0][vb], y = vr[s][1][vb], z = vr[s][2 % VR][vb], w = vr[s][3 % VR][vb];
+                        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+                        const uint32_t zs[4] = {z.x, z.y, z.z, z.w}, ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const uint32_t a0 = __byte_perm(xs[k], ys[k], 0x5410);
+                            const uint32_t a1 = __byte_perm(xs[k], ys[k], 0x7632);
+                            const uint32_t a2 = __byte_perm(zs[k], ws[k], 0x5410);
+                            const uint32_t a3 = __byte_perm(zs[k], ws[k], 0x7632);
+#pragma unroll
+                            for (int n = 0; n < NT; n++) {
+                                mma16<T>(o[n][vb * MT + k], a0, a1, a2, a3, lo[n][0], lo[n][1]);
+                                mma16<T>(o[n][vb * MT + k], a0, a1, a2, a3, hi[n][0], hi[n][1]);
+                            }
+                        }
+                    }
+                }
+            }
+            if (i + 1 < last) {
+                if (WIDE) load_keys(i + 1, pages_next, 0);
+                else load_values(i + 1, pages_next, 0);
+                pages = pages_next;
+                if (i + 2 < last) pages_next = pages_at(i + 2);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) {
+                l[n][0] += __shfl_xor_sync(FULL, l[n][0], w);
+                l[n][1] += __shfl_xor_sync(FULL, l[n][1], w);
+            }
+    }
+
+    // CH consecutive values, (g + 8 vb) CH and on, of column 2 t4 + x of eight n
+    __device__ __forceinline__ void values(int n, int x, int vb, float scale, float (&v)[CH]) const {
+#pragma unroll
+        for (int k = 0; k < MT; k++) {
+            v[2 * k] = o[n][vb * MT + k][x] * scale;
+            v[2 * k + 1] = o[n][vb * MT + k][2 + x] * scale;
+        }
+    }
+};
+
+template <typename T, int DP, int NT, bool PART, bool SMALL>
+__global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP, NT>::BLOCKS)
     paged_split_kernel(PageView pv, const T* __restrict__ q, float c, int window, int sinks, T* __restrict__ out,
                        float* __restrict__ lse, SplitWork wk, int* status) {
-    using S = SplitShape<T, DP>;
-    constexpr int CH = S::CH, TT = S::TT, NS = S::NS, KJ = S::KJ, VB = S::VB, MT = S::MT;
-    constexpr bool WIDE = S::WIDE;
-    constexpr bool F = S::ES == 4;
-    constexpr unsigned ALL = TT == 32 ? FULL : 0xffffu;
+    using S = SplitShape<T, DP, NT>;
+    constexpr int CH = S::CH, TT = S::TT, VB = S::VB, QT = S::QT;
     __shared__ int64_t pre[SPLIT_THREADS + 1];
     __shared__ int64_t part[SPLIT_WARPS];
-    __shared__ uint4 qs[WIDE ? SPLIT_WARPS : 1][WIDE ? KJ : 1][WIDE ? 32 : 1];
+    __shared__ uint4 qs[S::WIDE ? SPLIT_WARPS * NT * S::KJ * 32 : 1];
     asm volatile("griddepcontrol.launch_dependents;");
 
     const int lane = lane_id(), warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
-    const int group = pv.hq / pv.hkv, gt = group_tiles(pv), items = pv.hkv * gt;
+    const int group = pv.hq / pv.hkv, gt = (group + QT - 1) / QT, items = pv.hkv * gt;
 
     // what the items of row r take in the list
     auto cost = [&](int r, int* st) {
@@ -247,8 +621,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP>::BLOCKS)
         }
     }
 
-    const int shift = pv.page_shift, slots = (1 << shift) - 1;
-    const uint32_t kpb = pv.kp * S::ES, ktb = pv.kt * S::ES, vpb = pv.vp * S::ES, vtb = pv.vt * S::ES;  // bytes
+    Stream<T, DP, NT, PART, SMALL> st;
     while (true) {
         const Span span(row_length(pv, b, nullptr), window, sinks, TT);
         if (span.tiles == 0) {  // an empty sequence (paged_join_kernel writes its output)
@@ -257,332 +630,54 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP>::BLOCKS)
         }
         const int stop = (int)min((int64_t)span.tiles + HEAD, place + left);
         const int first = max(place - HEAD, 0), last = max(stop - HEAD, 0);
+        const int bb = b, at = item;
         left -= stop - place;
         place = 0;
-        const int at = item;
-        if (++item == items) item = 0;
-        const int bb = b;
-        if (item == 0) b++;
-        if (first == last) {
-            if (left == 0) return;
-            continue;
+        if (++item == items) {
+            item = 0;
+            b++;
         }
-        const int h = at / gt, q0 = at % gt * QT;
-        const int32_t* row = pv.table + bb * pv.table_stride;
-        auto entry = [&](int t) {  // the page of token t, or -1 past the end, in a hole or outside the pool
-            int p = -1;
-            if (t < span.n) {
-                p = __ldg(row + (t >> shift));
-                if (p >= pv.n_pages) {
-                    flag(status, SMLM_FLAG_INDEX_RANGE);
-                    p = -1;
-                }
-            }
-            return p;
-        };
-        // the pages of a tile: SMALL: of token `lane`; else of each 16 tokens (the same in all lanes)
-        struct PagesOf {
-            int p[SMALL ? 1 : NS];
-        };
-        auto pages_at = [&](int i) {
-            const int t0 = span.token(i, TT);
-            PagesOf x;
-            if constexpr (SMALL) {
-                x.p[0] = lane < TT ? entry(t0 + lane) : -1;
-            } else {
+        if (first < last) {
+            const int h = at / gt, q0 = at % gt * QT;
+            st.run(pv, q, c, span, bb, h, q0, first, last, qs + (S::WIDE ? warp * NT * S::KJ * 32 : 0), status);
+            const bool whole = first == 0 && last == span.tiles;
+            const int64_t slot = 2 * (int64_t)worker + (first == 0);
 #pragma unroll
-                for (int s = 0; s < NS; s++) x.p[s] = entry(t0 + 16 * s);
-            }
-            return x;
-        };
-        // which of the tile's tokens are seen
-        auto seen_of = [&](int i, const PagesOf& x) {
-            const int t0 = span.token(i, TT);
-            bool whole = t0 + TT <= span.n && (t0 >= span.lo || t0 + TT <= span.sinks);
-            if constexpr (!SMALL) {
+            for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int s = 0; s < NS; s++) whole = whole && x.p[s] >= 0;
-                if (whole) return ALL;
-                const int p = lane < 16 ? x.p[0] : x.p[NS - 1];
-                return __ballot_sync(FULL, lane < TT && p >= 0 && span.sees(t0 + lane));
-            } else {
-                return __ballot_sync(FULL, x.p[0] >= 0 && span.sees(t0 + lane));
-            }
-        };
-        PagesOf pages = pages_at(first), pages_next;
-        const int qrow = q0 + g;  // this lane's column of the first product
-        const T* qp = q + ((int64_t)bb * pv.hq + h * group) * pv.d;
-        uint4 qf[WIDE ? 1 : KJ];
-#pragma unroll
-        for (int j = 0; j < KJ; j++) {
-            const int d0 = (t4 + 4 * j) * CH;
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (qrow < group && (!PART || d0 < pv.d)) v = load16(qp + (int64_t)qrow * pv.d + d0);
-            if constexpr (WIDE) qs[warp][j][lane] = v;
-            else qf[j] = v;
-        }
-        const char* kp = reinterpret_cast<const char*>(static_cast<const T*>(pv.k) + h * pv.kh + t4 * CH);
-        const char* vp = reinterpret_cast<const char*>(static_cast<const T*>(pv.v) + h * pv.vh);
-        uint4 kr[NS][2][KJ], vr[NS][4][VB];
-        // Tokens that are not seen are loaded all the same, from their own page or page 0 (mapped memory), and masked.
-        auto load_keys = [&](int i, const PagesOf& x) {
-            const int t0 = span.token(i, TT);
-#pragma unroll
-            for (int s = 0; s < NS; s++) {
-                const char* base = kp;
-                if constexpr (!SMALL)
-                    base += (uint64_t)(uint32_t)max(x.p[s], 0) * kpb + (uint64_t)(uint32_t)((t0 + 16 * s) & slots) * ktb +
-                            (uint64_t)(uint32_t)g * ktb;
-#pragma unroll
-                for (int r = 0; r < 2; r++) {
-                    const char* src;
-                    if constexpr (SMALL) {
-                        const int y = 16 * s + 8 * r + g;
-                        const int p = max(__shfl_sync(FULL, x.p[0], y), 0);
-                        src = kp + (uint64_t)(uint32_t)p * kpb + (uint64_t)(uint32_t)((t0 + y) & slots) * ktb;
-                    } else {
-                        src = base + (uint64_t)(8 * r) * ktb;
-                    }
-#pragma unroll
-                    for (int j = 0; j < KJ; j++) {
-                        if (!PART || (t4 + 4 * j) * CH < pv.d) kr[s][r][j] = load16(src + 64 * j);
-                        else kr[s][r][j] = make_uint4(0, 0, 0, 0);
-                    }
-                }
-            }
-        };
-        auto value_token = [&](int s, int r) {  // token of value row r in tile order
-            return 16 * s + (F ? t4 + 4 * r : 2 * t4 + (r & 1) + 8 * (r >> 1));
-        };
-        auto load_values = [&](int i, const PagesOf& x) {
-            const int t0 = span.token(i, TT);
-#pragma unroll
-            for (int s = 0; s < NS; s++) {
-                const char* base = vp;
-                if constexpr (!SMALL)
-                    base += (uint64_t)(uint32_t)max(x.p[s], 0) * vpb + (uint64_t)(uint32_t)((t0 + 16 * s) & slots) * vtb +
-                            (uint64_t)(uint32_t)(F ? t4 : 2 * t4) * vtb;
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const char* src;
-                    if constexpr (SMALL) {
-                        const int y = value_token(s, r);
-                        const int p = max(__shfl_sync(FULL, x.p[0], y), 0);
-                        src = vp + (uint64_t)(uint32_t)p * vpb + (uint64_t)(uint32_t)((t0 + y) & slots) * vtb;
-                    } else {
-                        src = base + (uint64_t)(F ? 4 * r : (r & 1) + 8 * (r >> 1)) * vtb;
+                for (int x = 0; x < 2; x++) {
+                    const int col = 8 * n + 2 * t4 + x;
+                    if (q0 + col >= group) continue;
+                    const float l = st.l[n][x], m = st.m[n][x];
+                    const int64_t head = (int64_t)bb * pv.hq + h * group + q0 + col;
+                    const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+                    if (g == 0) {
+                        if (!whole)
+                            *reinterpret_cast<float2*>(wk.ml + 2 * (slot * wk.rows + col)) = make_float2(m, l);
+                        else if (lse)
+                            lse[head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
                     }
 #pragma unroll
                     for (int vb = 0; vb < VB; vb++) {
-                        const int d0 = (g + 8 * vb) * CH;  // columns past d are not stored
-                        const bool in = (!PART && DP >= 8 * CH) || d0 < pv.d;
-                        vr[s][r][vb] = load16(src + (in ? 16 * g + 128 * vb : 0));
-                    }
-                }
-            }
-        };
-
-        float o[VB * MT][4];
+                        const int d0 = (g + 8 * vb) * CH;
+                        if (d0 >= pv.d) continue;
+                        float v[CH];
+                        st.values(n, x, vb, inv, v);
+                        if (whole) {
+                            *reinterpret_cast<uint4*>(out + head * pv.d + d0) = narrow16<T>(v);
+                        } else {
+                            float* dst = wk.o + (slot * wk.rows + col) * wk.dp + d0;
 #pragma unroll
-        for (int i = 0; i < VB * MT; i++)
-#pragma unroll
-            for (int x = 0; x < 4; x++) o[i][x] = 0.f;
-        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;  // columns 2 t4, 2 t4 + 1
-
-        load_keys(first, pages);
-        if (!WIDE) load_values(first, pages);
-        if (first + 1 < last) pages_next = pages_at(first + 1);
-        for (int i = first; i < last; i++) {
-            float sc[NS][4];
-#pragma unroll
-            for (int s = 0; s < NS; s++) {
-                sc[s][0] = sc[s][1] = sc[s][2] = sc[s][3] = 0.f;
-#pragma unroll
-                for (int j = 0; j < KJ; j++) {
-                    const uint4 a = kr[s][0][j], e = kr[s][1][j];
-                    uint4 w;
-                    if constexpr (WIDE) w = qs[warp][j][lane];
-                    else w = qf[j];
-                    if constexpr (F) {
-                        mma_split32(sc[s], a.x, e.x, a.y, e.y, Split32(w.x), Split32(w.y));
-                        mma_split32(sc[s], a.z, e.z, a.w, e.w, Split32(w.z), Split32(w.w));
-                    } else {
-                        mma16<T>(sc[s], a.x, e.x, a.y, e.y, w.x, w.y);
-                        mma16<T>(sc[s], a.z, e.z, a.w, e.w, w.z, w.w);
-                    }
-                }
-            }
-            if (WIDE) load_values(i, pages);
-            const unsigned seen = seen_of(i, pages);
-            if (!WIDE && i + 1 < last) load_keys(i + 1, pages_next);
-#pragma unroll
-            for (int s = 0; s < NS; s++)
-#pragma unroll
-                for (int x = 0; x < 4; x++) sc[s][x] *= c;
-            if (seen != ALL) {  // 0 * (a stale infinity or NaN) must not reach the sums either
-#pragma unroll
-                for (int s = 0; s < NS; s++) {
-#pragma unroll
-                    for (int r = 0; r < 2; r++)
-                        if (!(seen >> (16 * s + 8 * r + g) & 1)) sc[s][2 * r] = sc[s][2 * r + 1] = -INFINITY;
-#pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        if (!WIDE && !(seen >> value_token(s, r) & 1)) {
-#pragma unroll
-                            for (int vb = 0; vb < VB; vb++) vr[s][r][vb] = make_uint4(0, 0, 0, 0);
-                        }
-                }
-            }
-            float x0 = -INFINITY, x1 = -INFINITY;
-#pragma unroll
-            for (int s = 0; s < NS; s++)
-#pragma unroll
-                for (int r = 0; r < 2; r++) {
-                    x0 = fmaxf(x0, sc[s][2 * r]);
-                    x1 = fmaxf(x1, sc[s][2 * r + 1]);
-                }
-#pragma unroll
-            for (int w = 4; w < 32; w <<= 1) {
-                x0 = fmaxf(x0, __shfl_xor_sync(FULL, x0, w));
-                x1 = fmaxf(x1, __shfl_xor_sync(FULL, x1, w));
-            }
-            if (__any_sync(FULL, x0 > m0 || x1 > m1)) {
-                const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
-                const float f0 = m0 == n0 ? 1.f : ex2(m0 - n0), f1 = m1 == n1 ? 1.f : ex2(m1 - n1);
-                m0 = n0;
-                m1 = n1;
-                l0 *= f0;
-                l1 *= f1;
-#pragma unroll
-                for (int x = 0; x < VB * MT; x++) {
-                    o[x][0] *= f0;
-                    o[x][1] *= f1;
-                    o[x][2] *= f0;
-                    o[x][3] *= f1;
-                }
-            }
-            const float z0 = m0 == -INFINITY ? 0.f : m0, z1 = m1 == -INFINITY ? 0.f : m1;
-#pragma unroll
-            for (int s = 0; s < NS; s++)
-#pragma unroll
-                for (int r = 0; r < 2; r++) {
-                    sc[s][2 * r] = ex2(sc[s][2 * r] - z0);
-                    sc[s][2 * r + 1] = ex2(sc[s][2 * r + 1] - z1);
-                    l0 += sc[s][2 * r];
-                    l1 += sc[s][2 * r + 1];
-                }
-            if (WIDE && seen != ALL) {
-#pragma unroll
-                for (int s = 0; s < NS; s++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        if (!(seen >> value_token(s, r) & 1)) {
-#pragma unroll
-                            for (int vb = 0; vb < VB; vb++) vr[s][r][vb] = make_uint4(0, 0, 0, 0);
-                        }
-            }
-#pragma unroll
-            for (int s = 0; s < NS; s++) {
-                if constexpr (F) {
-#pragma unroll
-                    for (int r = 0; r < 2; r++) {  // tokens 8 r .. 8 r + 7 of the 16
-                        // P^T: weight of token t4 (+ 4) for query g, from lane (token, query / 2)
-                        const int from = 4 * t4 + (g >> 1);
-                        const float a = __shfl_sync(FULL, sc[s][2 * r], from);
-                        const float b1 = __shfl_sync(FULL, sc[s][2 * r + 1], from);
-                        const float a4 = __shfl_sync(FULL, sc[s][2 * r], from + 16);
-                        const float b4 = __shfl_sync(FULL, sc[s][2 * r + 1], from + 16);
-                        const Split32 p0(__float_as_uint(g & 1 ? b1 : a)), p1(__float_as_uint(g & 1 ? b4 : a4));
-#pragma unroll
-                        for (int vb = 0; vb < VB; vb++) {
-                            const uint4 x = vr[s][2 * r][vb], y = vr[s][2 * r + 1][vb];
-                            mma_split32(o[vb * MT], x.x, x.y, y.x, y.y, p0, p1);
-                            mma_split32(o[vb * MT + 1], x.z, x.w, y.z, y.w, p0, p1);
-                        }
-                    }
-                } else {
-                    const uint32_t h0 = pack16<T>(sc[s][0], sc[s][1]), h1 = pack16<T>(sc[s][2], sc[s][3]);
-                    const float2 u0 = unpack16<T>(h0), u1 = unpack16<T>(h1);
-                    const uint32_t e0 = transpose8x8(pack16<T>(sc[s][0] - u0.x, sc[s][1] - u0.y));
-                    const uint32_t e1 = transpose8x8(pack16<T>(sc[s][2] - u1.x, sc[s][3] - u1.y));
-                    const uint32_t p0 = transpose8x8(h0), p1 = transpose8x8(h1);
-#pragma unroll
-                    for (int vb = 0; vb < VB; vb++) {
-                        const uint4 x = vr[s][0][vb], y = vr[s][1][vb], z = vr[s][2][vb], w = vr[s][3][vb];
-                        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-                        const uint32_t zs[4] = {z.x, z.y, z.z, z.w}, ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            const uint32_t a0 = __byte_perm(xs[k], ys[k], 0x5410);
-                            const uint32_t a1 = __byte_perm(xs[k], ys[k], 0x7632);
-                            const uint32_t a2 = __byte_perm(zs[k], ws[k], 0x5410);
-                            const uint32_t a3 = __byte_perm(zs[k], ws[k], 0x7632);
-                            mma16<T>(o[vb * MT + k], a0, a1, a2, a3, e0, e1);
-                            mma16<T>(o[vb * MT + k], a0, a1, a2, a3, p0, p1);
+                            for (int k = 0; k < CH; k += 4)
+                                *reinterpret_cast<float4*>(dst + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
                         }
                     }
                 }
+            if (lane == 0) {
+                int2* cut_at = wk.cut + (int64_t)bb * items + at;
+                if (first == 0) cut_at->x = whole ? -1 : worker;
+                if (last == span.tiles) cut_at->y = worker;
             }
-            if (i + 1 < last) {
-                if (WIDE) load_keys(i + 1, pages_next);
-                else load_values(i + 1, pages_next);
-                pages = pages_next;
-                if (i + 2 < last) pages_next = pages_at(i + 2);
-            }
-        }
-#pragma unroll
-        for (int w = 4; w < 32; w <<= 1) {
-            l0 += __shfl_xor_sync(FULL, l0, w);
-            l1 += __shfl_xor_sync(FULL, l1, w);
-        }
-        // columns 2 t4 (x = 0) and 2 t4 + 1: this lane has values CH (g + 8 vb) .. + CH - 1 of them
-        const bool whole = first == 0 && last == span.tiles;
-        const int64_t slot = 2 * (int64_t)worker + (first == 0);
-#pragma unroll
-        for (int x = 0; x < 2; x++) {
-            const int col = 2 * t4 + x;
-            if (q0 + col >= group) continue;
-            const float l = x ? l1 : l0, m = x ? m1 : m0;
-            const int64_t head = (int64_t)bb * pv.hq + h * group + q0 + col;
-            const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
-            if (g == 0) {
-                if (whole) {
-                    if (lse) lse[head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
-                } else {
-                    *reinterpret_cast<float2*>(wk.ml + 2 * (slot * wk.rows + col)) = make_float2(m, l);
-                }
-            }
-#pragma unroll
-            for (int vb = 0; vb < VB; vb++) {
-                const int d0 = (g + 8 * vb) * CH;
-                if (d0 >= pv.d) continue;
-                float v[CH];
-#pragma unroll
-                for (int k = 0; k < MT; k++) {
-                    v[2 * k] = o[vb * MT + k][x] * inv;
-                    v[2 * k + 1] = o[vb * MT + k][2 + x] * inv;
-                }
-                if (whole) {
-                    uint4 w;
-                    if constexpr (F)
-                        w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
-                                       __float_as_uint(v[3]));
-                    else
-                        w = make_uint4(pack16<T>(v[0], v[1]), pack16<T>(v[2], v[3]), pack16<T>(v[4], v[5]),
-                                       pack16<T>(v[6], v[7]));
-                    *reinterpret_cast<uint4*>(out + head * pv.d + d0) = w;
-                } else {
-                    float* dst = wk.o + (slot * wk.rows + col) * wk.dp + d0;
-#pragma unroll
-                    for (int k = 0; k < CH; k += 4)
-                        *reinterpret_cast<float4*>(dst + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
-                }
-            }
-        }
-        if (lane == 0) {
-            int2* cut_at = wk.cut + (int64_t)bb * items + at;
-            if (first == 0) cut_at->x = whole ? -1 : worker;
-            if (last == span.tiles) cut_at->y = worker;
         }
         if (left == 0) return;
     }
@@ -592,12 +687,12 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP>::BLOCKS)
 // order that only the lengths decide (the same sums on every run); rows that see nothing become 0. DP / 4 lanes take
 // a piece, JOIN_THREADS / (DP / 4) pieces go at a time, and every lane has four of them in flight: what this kernel
 // costs is a chain of dependent loads (where the pieces are; the pieces), not their bytes.
-template <typename T, int DP, int TT>
+template <typename T, int DP, int TT, int QT>
 __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(PageView pv, int window, int sinks,
                                                                   T* __restrict__ out, float* __restrict__ lse,
                                                                   SplitWork wk) {
     constexpr int LANES = DP / 4, SETS = JOIN_THREADS / LANES, U = 4;
-    const int hq = blockIdx.x, b = blockIdx.y, group = pv.hq / pv.hkv, gt = group_tiles(pv), qi = hq % group;
+    const int hq = blockIdx.x, b = blockIdx.y, group = pv.hq / pv.hkv, gt = (group + QT - 1) / QT, qi = hq % group;
     const int tiles = Span(row_length(pv, b, nullptr), window, sinks, TT).tiles;
     const int64_t head = (int64_t)b * pv.hq + hq;
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -688,31 +783,6 @@ __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(PageView pv, i
 // half (value i with i + d / 2), four such pairs in flight; cos and sin come from L1 after a token's first head.
 // Token t of row b is at position lengths[b] - T + t; a negative one is the padding before a shorter chunk.
 constexpr int APPEND_THREADS = 256, APPEND_TOKENS = 32, APPEND_UNROLL = 4;
-
-template <typename T>
-__device__ __forceinline__ void widen16(const uint4& v, float (&f)[16 / sizeof(T)]) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        if constexpr (sizeof(T) == 4) {
-            f[i] = __uint_as_float(w[i]);
-        } else {
-            const float2 p = unpack16<T>(w[i]);
-            f[2 * i] = p.x;
-            f[2 * i + 1] = p.y;
-        }
-    }
-}
-template <typename T>
-__device__ __forceinline__ uint4 narrow16(const float (&f)[16 / sizeof(T)]) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(f[i]);
-        else w[i] = pack16<T>(f[2 * i], f[2 * i + 1]);
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
 
 template <typename T>
 __global__ void __launch_bounds__(APPEND_THREADS)
@@ -861,33 +931,37 @@ static int by_dtype(int dtype, F f) {
     return f(__nv_bfloat16());
 }
 
-static int split_blocks(int64_t es, int64_t dp) { return es * dp <= 128 ? 4 : es * dp <= 256 ? 3 : 2; }
 static int64_t padded_d(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+// Two eights of query heads where a group has more than eight: each key and value is then read half as often. Rows of
+// more than 256 bytes have no registers for it (and fp32 none from 64 on).
+static int eights(int64_t group, int64_t dp, int64_t es) { return group > 8 && es == 2 && dp <= 128 ? 2 : 1; }
+static int split_blocks(int64_t es, int64_t dp, int nt) { return es * dp * nt <= 128 ? 4 : es * dp * nt <= 256 ? 3 : 2; }
 
 // Carves the workspace (sizes only without one).
 template <typename W>
 static void split_work(W& ws, SplitWork& wk, int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t es) {
-    const int64_t dp = padded_d(d), slots = 2 * (int64_t)sm_count() * split_blocks(es, dp) * SPLIT_WARPS;
-    wk.rows = (int)std::min<int64_t>(hq / std::max<int64_t>(hkv, 1), QT);
+    const int64_t dp = padded_d(d), group = hq / std::max<int64_t>(hkv, 1);
+    const int nt = eights(group, dp, es);
+    const int64_t slots = 2 * (int64_t)sm_count() * split_blocks(es, dp, nt) * SPLIT_WARPS;
+    const int64_t items = batch * hkv * ((group + 8 * nt - 1) / (8 * nt));
+    wk.rows = (int)std::min<int64_t>(group, 8 * nt);
     wk.dp = (int)dp;
-    const int64_t items = batch * hkv * ((hq / std::max<int64_t>(hkv, 1) + QT - 1) / QT);
-    if constexpr (std::is_same_v<W, Workspace>) {
-        wk.cut = ws.template take<int2>(items);
-        wk.ml = ws.template take<float>(2 * slots * wk.rows);
-        wk.o = ws.template take<float>(slots * wk.rows * dp);
-    } else {
-        ws.template take<int2>(items);
-        ws.template take<float>(2 * slots * wk.rows);
-        ws.template take<float>(slots * wk.rows * dp);
-    }
+    const auto take = [&](auto*& p, int64_t n) {
+        using E = std::remove_reference_t<decltype(*p)>;
+        if constexpr (std::is_same_v<W, Workspace>) p = ws.template take<E>(n);
+        else ws.template take<E>(n);
+    };
+    take(wk.cut, items);
+    take(wk.ml, 2 * slots * wk.rows);
+    take(wk.o, slots * wk.rows * dp);
 }
 
-template <typename T, int DP, bool PART, bool SMALL>
+template <typename T, int DP, int NT, bool PART, bool SMALL>
 static int launch_split(const PageView& pv, const void* q, float scale, int window, int sinks, void* out, float* lse,
                         const SplitWork& wk, int* status, cudaStream_t st) {
-    using S = SplitShape<T, DP>;
+    using S = SplitShape<T, DP, NT>;
     const int blocks = sm_count() * S::BLOCKS;
-    paged_split_kernel<T, DP, PART, SMALL><<<blocks, SPLIT_THREADS, 0, st>>>(
+    paged_split_kernel<T, DP, NT, PART, SMALL><<<blocks, SPLIT_THREADS, 0, st>>>(
         pv, static_cast<const T*>(q), scale * 1.4426950408889634074f, window, sinks, static_cast<T*>(out), lse, wk,
         status);
     SMLM_LAUNCHED("paged_attention");
@@ -901,18 +975,26 @@ static int launch_split(const PageView& pv, const void* q, float scale, int wind
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    SMLM_CUDA(cudaLaunchKernelEx(&cfg, paged_join_kernel<T, DP, S::TT>, pv, window, sinks, static_cast<T*>(out), lse, wk));
+    SMLM_CUDA(cudaLaunchKernelEx(&cfg, paged_join_kernel<T, DP, S::TT, S::QT>, pv, window, sinks, static_cast<T*>(out), lse, wk));
     return SMLM_OK;
 }
 
 template <typename T>
 static int launch_attention(const PageView& pv, const void* q, float scale, int window, int sinks, void* out,
                             float* lse, const SplitWork& wk, int* status, cudaStream_t st) {
+    const auto of = [&](auto dp, auto nt) {
+        constexpr int DP = decltype(dp)::value, NT = decltype(nt)::value;
+        if (pv.page_shift < 4)
+            return launch_split<T, DP, NT, true, true>(pv, q, scale, window, sinks, out, lse, wk, status, st);
+        if (pv.d < DP)
+            return launch_split<T, DP, NT, true, false>(pv, q, scale, window, sinks, out, lse, wk, status, st);
+        return launch_split<T, DP, NT, false, false>(pv, q, scale, window, sinks, out, lse, wk, status, st);
+    };
     const auto go = [&](auto dp) {
-        constexpr int DP = decltype(dp)::value;
-        if (pv.page_shift < 4) return launch_split<T, DP, true, true>(pv, q, scale, window, sinks, out, lse, wk, status, st);
-        return pv.d == DP ? launch_split<T, DP, false, false>(pv, q, scale, window, sinks, out, lse, wk, status, st)
-                          : launch_split<T, DP, true, false>(pv, q, scale, window, sinks, out, lse, wk, status, st);
+        if constexpr (sizeof(T) == 2 && decltype(dp)::value <= 128)
+            if (eights(pv.hq / pv.hkv, decltype(dp)::value, sizeof(T)) == 2)
+                return of(dp, std::integral_constant<int, 2>());
+        return of(dp, std::integral_constant<int, 1>());
     };
     if (pv.d <= 32) return go(std::integral_constant<int, 32>());
     if (pv.d <= 64) return go(std::integral_constant<int, 64>());
