@@ -141,21 +141,6 @@ struct Span {
     __device__ __forceinline__ bool sees(int t) const { return t < n && (t >= lo || t < sinks); }
 };
 
-// The list of `total` tiles cut into `workers` pieces: the first `extra` of `per` + 1 tiles, the others of `per`.
-struct Cut {
-    int64_t per, extra;
-    __device__ __forceinline__ Cut(int64_t total, int workers) {
-        if (total >> 31) {
-            per = total / workers;
-            extra = total % workers;
-        } else {  // 32-bit division is several times shorter
-            per = (uint32_t)total / (uint32_t)workers;
-            extra = (uint32_t)total % (uint32_t)workers;
-        }
-    }
-    __device__ __forceinline__ int64_t start(int64_t w) const { return w * per + min(w, extra); }
-};
-
 // Where the pieces of items that were cut lie. A worker has at most two: the one it began inside an item (slot 2 w)
 // and the one that holds an item's first tile but not its last (slot 2 w + 1).
 struct SplitWork {
@@ -540,85 +525,80 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP, NT>::BLOCKS)
                        float* __restrict__ lse, SplitWork wk, int* status) {
     using S = SplitShape<T, DP, NT>;
     constexpr int CH = S::CH, TT = S::TT, VB = S::VB, QT = S::QT;
-    __shared__ int64_t pre[SPLIT_THREADS + 1];
-    __shared__ int64_t part[SPLIT_WARPS];
+    __shared__ int4 pre[SPLIT_THREADS / 4];
+    __shared__ int part[SPLIT_WARPS];
     __shared__ uint4 qs[S::WIDE ? SPLIT_WARPS * NT * S::KJ * 32 : 1];
     asm volatile("griddepcontrol.launch_dependents;");
 
     const int lane = lane_id(), warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
     const int group = pv.hq / pv.hkv, gt = (group + QT - 1) / QT, items = pv.hkv * gt;
 
-    // what the items of row r take in the list
+    // what the items of row r take in the list (its length fits 31 bits: the host checks)
     auto cost = [&](int r, int* st) {
         const int tiles = Span(row_length(pv, r, st), window, sinks, TT).tiles;
-        return tiles ? (int64_t)items * (tiles + HEAD) : 0;
+        return tiles ? items * (tiles + HEAD) : 0;
     };
-    // the list's length and this thread's sequences' place in it
-    const int chunk = (pv.batch + SPLIT_THREADS - 1) / SPLIT_THREADS;
-    const int r0 = min(pv.batch, (int)threadIdx.x * chunk), r1 = min(pv.batch, r0 + chunk);
-    int64_t mine = 0;
-    for (int r = r0; r < r1; r++) mine += cost(r, status);
-    {
-        int64_t x = mine;
+    auto inclusive = [&](int x) {
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int64_t y = __shfl_up_sync(FULL, x, o);
+            const int y = __shfl_up_sync(FULL, x, o);
             if (lane >= o) x += y;
         }
+        return x;
+    };
+    // The sequence, the item and the place in it where this worker starts, and how much it does. Up to 32 rows: each
+    // warp for itself, a lane a row; more: a thread has `chunk` rows, and the warp looks for its start in the block's
+    // sums and then among the rows.
+    const int workers = gridDim.x * SPLIT_WARPS, worker = warp * gridDim.x + blockIdx.x;  // one warp per SM first
+    int b = 0, off, left;
+    auto cut = [&](int total) {  // the first total % workers pieces are one tile longer
+        const int per = (uint32_t)total / (uint32_t)workers, extra = total - per * workers;
+        left = per + (worker < extra);
+        off = worker * per + min(worker, extra);
+    };
+    auto among = [&](int x, int w) {  // x: inclusive sums, w: what lane's row takes
+        const unsigned beyond = __ballot_sync(FULL, x > off);
+        const int at = beyond ? __ffs(beyond) - 1 : 31;
+        off -= __shfl_sync(FULL, beyond ? x - w : x, at);
+        b += beyond ? at : 32;
+        return beyond != 0;
+    };
+    if (pv.batch <= 32) {
+        const int w = lane < pv.batch ? cost(lane, status) : 0, x = inclusive(w);
+        cut(__shfl_sync(FULL, x, 31));
+        if (left <= 0) return;
+        among(x, w);
+    } else {
+        const int chunk = (pv.batch + SPLIT_THREADS - 1) / SPLIT_THREADS;
+        const int r0 = min(pv.batch, (int)threadIdx.x * chunk), r1 = min(pv.batch, r0 + chunk);
+        int x = 0;
+        for (int r = r0; r < r1; r++) x += cost(r, status);
+        x = inclusive(x);
         if (lane == 31) part[warp] = x;
         __syncthreads();
         for (int w = 0; w < warp; w++) x += part[w];
-        pre[threadIdx.x + 1] = x;
-        if (threadIdx.x == 0) pre[0] = 0;
+        reinterpret_cast<int*>(pre)[threadIdx.x] = x;
         __syncthreads();
-    }
-    const int64_t total = pre[SPLIT_THREADS];
-    const Cut cut(total, gridDim.x * SPLIT_WARPS);
-    const int worker = warp * gridDim.x + blockIdx.x;  // few tiles: one warp per SM first
-    int64_t left = cut.per + (worker < cut.extra);
-    if (left <= 0) return;
-
-    // the sequence, the item and the place in it where this worker starts
-    int b, item, place;
-    {
-        const int64_t start = cut.start(worker);
-        int a = 0, e = SPLIT_THREADS;  // pre[a] <= start < pre[e]
-        while (e - a > 1) {
-            const int mid = (a + e) >> 1;
-            if (pre[mid] <= start) a = mid;
-            else e = mid;
-        }
-        int64_t off = start - pre[a];
-        b = a * chunk;
+        const int4 sums = pre[lane];  // of threads 4 lane .. 4 lane + 3
+        cut(__shfl_sync(FULL, sums.w, 31));
+        if (left <= 0) return;
+        // threads whose sum does not pass the start lie before it
+        const int before = (sums.x <= off) + (sums.y <= off) + (sums.z <= off) + (sums.w <= off);
+        const int skip = __reduce_add_sync(FULL, before);
+        b = skip * chunk;
+        off -= skip ? reinterpret_cast<const int*>(pre)[skip - 1] : 0;
         if (chunk > 1) {
             while (true) {
-                const int r = b + lane;
-                const int64_t w = r < pv.batch ? cost(r, nullptr) : 0;
-                int64_t x = w;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int64_t y = __shfl_up_sync(FULL, x, o);
-                    if (lane >= o) x += y;
-                }
-                const unsigned beyond = __ballot_sync(FULL, x > off);
-                if (beyond) {
-                    const int at = __ffs(beyond) - 1;
-                    off -= __shfl_sync(FULL, x - w, at);
-                    b += at;
-                    break;
-                }
-                off -= __shfl_sync(FULL, x, 31);
-                b += 32;
+                const int w = b + lane < pv.batch ? cost(b + lane, nullptr) : 0;
+                if (among(inclusive(w), w)) break;
             }
         }
-        const int each = Span(row_length(pv, b, nullptr), window, sinks, TT).tiles + HEAD;
-        if (off >> 31) {
-            item = (int)(off / each);
-            place = (int)(off % each);
-        } else {
-            item = (uint32_t)off / (uint32_t)each;
-            place = (uint32_t)off % (uint32_t)each;
-        }
+    }
+    int item, place;
+    {
+        const uint32_t each = Span(row_length(pv, b, nullptr), window, sinks, TT).tiles + HEAD;
+        item = (uint32_t)off / each;
+        place = (uint32_t)off - item * each;
     }
 
     Stream<T, DP, NT, PART, SMALL> st;
@@ -628,7 +608,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP, NT>::BLOCKS)
             b++;
             continue;
         }
-        const int stop = (int)min((int64_t)span.tiles + HEAD, place + left);
+        const int stop = min(span.tiles + HEAD, place + left);
         const int first = max(place - HEAD, 0), last = max(stop - HEAD, 0);
         const int bb = b, at = item;
         left -= stop - place;
@@ -683,97 +663,117 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP, NT>::BLOCKS)
     }
 }
 
-// One block per (query head, sequence): the pieces of an item that was cut, each scaled to the largest maximum, in an
-// order that only the lengths decide (the same sums on every run); rows that see nothing become 0. DP / 4 lanes take
-// a piece, JOIN_THREADS / (DP / 4) pieces go at a time, and every lane has four of them in flight: what this kernel
-// costs is a chain of dependent loads (where the pieces are; the pieces), not their bytes.
-template <typename T, int DP, int TT, int QT>
-__global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(PageView pv, int window, int sinks,
+// For each 32 columns of each (sequence, query head): the pieces of an item that was cut, each scaled to the largest
+// maximum, in an order that only the lengths decide (the same sums on every run); rows that see nothing become 0.
+// Eight lanes take a piece's 128 bytes, four pieces a warp go at a time and every lane has eight of them in flight:
+// what this kernel costs is a chain of dependent loads (where the pieces are; the pieces), not their bytes. W warps
+// share a head: all eight of a block where there are few heads with many pieces each, one where there are many
+// (more blocks than fit at once would cost 1.5 us a wave: 37 us instead of 20 at 1024 heads).
+template <typename T, int TT, int QT, int W>
+__global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(PageView pv, int window, int sinks, int columns,
                                                                   T* __restrict__ out, float* __restrict__ lse,
                                                                   SplitWork wk) {
-    constexpr int LANES = DP / 4, SETS = JOIN_THREADS / LANES, U = 4;
-    const int hq = blockIdx.x, b = blockIdx.y, group = pv.hq / pv.hkv, gt = (group + QT - 1) / QT, qi = hq % group;
+    constexpr int SETS = 4 * W, U = 8, UNITS = JOIN_THREADS / 32 / W;
+    const int lane = lane_id(), warp = threadIdx.x / 32 % W;
+    const uint32_t unit = blockIdx.x * UNITS + threadIdx.x / (32 * W);  // (sequence, query head, 32 columns)
+    if (unit >= (uint32_t)pv.batch * pv.hq * columns) return;
+    const int col = unit % columns, hq = unit / columns % pv.hq, b = unit / columns / pv.hq;
+    const int group = pv.hq / pv.hkv, gt = (group + QT - 1) / QT, qi = hq % group;
     const int tiles = Span(row_length(pv, b, nullptr), window, sinks, TT).tiles;
     const int64_t head = (int64_t)b * pv.hq + hq;
+    const int set = 4 * warp + lane / 8, x = col * 32 + lane % 8 * 4;
+    T* dst = out + head * pv.d + x;
+    const bool mine = set == 0 && x < pv.d, logs = lse && set == 0 && lane == 0 && col == 0;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (tiles == 0) {
-        for (int x = threadIdx.x; x < pv.d; x += JOIN_THREADS) out[head * pv.d + x] = narrow<T>(0.f);
-        if (lse && threadIdx.x == 0) lse[head] = -INFINITY;
+        if (mine) dst[0] = dst[1] = dst[2] = dst[3] = narrow<T>(0.f);
+        if (logs) lse[head] = -INFINITY;
         return;
     }
     const int2 cut = wk.cut[((int64_t)b * pv.hkv + hq / group) * gt + qi / QT];
     if (cut.x < 0) return;
-    const int pieces = cut.y - cut.x + 1, set = threadIdx.x / LANES, x = threadIdx.x % LANES * 4;
+    const int pieces = cut.y - cut.x + 1;
     float m = -INFINITY, l = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float f, const float4& o) {
+        acc.x = fmaf(o.x, f, acc.x);
+        acc.y = fmaf(o.y, f, acc.y);
+        acc.z = fmaf(o.z, f, acc.z);
+        acc.w = fmaf(o.w, f, acc.w);
+    };
+    auto rescale = [&](float mn) {  // to the maximum mn; returns what is subtracted from exponents
+        const float base = mn == -INFINITY ? 0.f : mn, a = ex2(m - base);
+        l *= a;
+        acc = make_float4(acc.x * a, acc.y * a, acc.z * a, acc.w * a);
+        m = mn;
+        return base;
+    };
     for (int k0 = set; k0 < pieces; k0 += SETS * U) {
         float2 ml[U];
         float4 o[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int k = k0 + u * SETS;
-            // the first piece is the last of its worker, the others the first of theirs
-            const int64_t r = (2 * ((int64_t)cut.x + k) + (k == 0)) * wk.rows + qi % QT;
             ml[u] = make_float2(-INFINITY, 0.f);
             o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
             if (k < pieces) {
+                // the first piece is the last of its worker, the others the first of theirs
+                const int64_t r = (int64_t)(2 * (cut.x + k) + (k == 0)) * wk.rows + qi % QT;
                 ml[u] = *reinterpret_cast<const float2*>(wk.ml + 2 * r);
-                o[u] = *reinterpret_cast<const float4*>(wk.o + r * DP + x);  // columns past d are not stored
+                o[u] = *reinterpret_cast<const float4*>(wk.o + r * wk.dp + x);  // columns past d are not stored
             }
         }
         float mn = m;
 #pragma unroll
         for (int u = 0; u < U; u++) mn = fmaxf(mn, ml[u].x);
-        const float base = mn == -INFINITY ? 0.f : mn, a = ex2(m - base);
-        l *= a;
-        acc.x *= a;
-        acc.y *= a;
-        acc.z *= a;
-        acc.w *= a;
+        const float base = rescale(mn);
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            if (k0 + u * SETS >= pieces) break;
             const float e = ex2(ml[u].x - base);
-            l += ml[u].y * e;
-            acc.x += o[u].x * e;
-            acc.y += o[u].y * e;
-            acc.z += o[u].z * e;
-            acc.w += o[u].w * e;
+            l = fmaf(ml[u].y, e, l);
+            add(e, o[u]);
         }
-        m = mn;
     }
-    __shared__ float sm[SETS], sl[SETS];
-    __shared__ float4 so[SETS][LANES];
-    if (x == 0) {
-        sm[set] = m;
-        sl[set] = l;
+    // the four sets of a warp, then the warps
+    float mn = fmaxf(m, __shfl_xor_sync(FULL, m, 8));
+    mn = fmaxf(mn, __shfl_xor_sync(FULL, mn, 16));
+    rescale(mn);
+#pragma unroll
+    for (int w = 8; w < 32; w <<= 1) {
+        l += __shfl_xor_sync(FULL, l, w);
+        acc.x += __shfl_xor_sync(FULL, acc.x, w);
+        acc.y += __shfl_xor_sync(FULL, acc.y, w);
+        acc.z += __shfl_xor_sync(FULL, acc.z, w);
+        acc.w += __shfl_xor_sync(FULL, acc.w, w);
     }
-    so[set][x / 4] = acc;
-    __syncthreads();
-    if (set) return;
-    const int sets = min(pieces, SETS);
-    float mx = -INFINITY, sum = 0.f;
-    for (int w = 0; w < sets; w++) mx = fmaxf(mx, sm[w]);
-    const float base = mx == -INFINITY ? 0.f : mx;
-    acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int w = 0; w < sets; w++) {
-        const float e = ex2(sm[w] - base);
-        const float4 o = so[w][x / 4];
-        sum += sl[w] * e;
-        acc.x += o.x * e;
-        acc.y += o.y * e;
-        acc.z += o.z * e;
-        acc.w += o.w * e;
+    if constexpr (W > 1) {
+        __shared__ float2 sm[W];
+        __shared__ float4 so[W][8];
+        if (lane == 0) sm[warp] = make_float2(m, l);
+        if (lane < 8) so[warp][lane] = acc;
+        __syncthreads();
+        if (set) return;
+        mn = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < W; w++) mn = fmaxf(mn, sm[w].x);
+        const float base = mn == -INFINITY ? 0.f : mn;
+        l = 0.f;
+        acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+            const float e = ex2(sm[w].x - base);
+            l = fmaf(sm[w].y, e, l);
+            add(e, so[w][lane]);
+        }
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    if (x < pv.d) {
-        T* dst = out + head * pv.d + x;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (mine) {
         dst[0] = narrow<T>(acc.x * inv);
         dst[1] = narrow<T>(acc.y * inv);
         dst[2] = narrow<T>(acc.z * inv);
         dst[3] = narrow<T>(acc.w * inv);
     }
-    if (lse && x == 0) lse[head] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * 0.69314718055994530942f;
+    if (logs) lse[head] = l == 0.f ? -INFINITY : (mn + log2f(l)) * 0.69314718055994530942f;
 }
 
 // ---------------------------------------------------------------------------------------------------- append
@@ -966,8 +966,12 @@ static int launch_split(const PageView& pv, const void* q, float scale, int wind
         status);
     SMLM_LAUNCHED("paged_attention");
     // launched while the first kernel still runs; it waits for that kernel's end itself
+    const int columns = (pv.d + 31) / 32;
+    const int64_t units = (int64_t)pv.batch * pv.hq * columns;
+    const int64_t items = (int64_t)pv.batch * pv.hkv * ((pv.hq / pv.hkv + S::QT - 1) / S::QT);
+    const bool shared = (int64_t)blocks * SPLIT_WARPS > 32 * items;  // over 32 pieces an item: a block for each
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(pv.hq, pv.batch);
+    cfg.gridDim = dim3((unsigned)(shared ? units : (units + 7) / 8));
     cfg.blockDim = dim3(JOIN_THREADS);
     cfg.stream = st;
     cudaLaunchAttribute attr{};
@@ -975,7 +979,8 @@ static int launch_split(const PageView& pv, const void* q, float scale, int wind
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    SMLM_CUDA(cudaLaunchKernelEx(&cfg, paged_join_kernel<T, DP, S::TT, S::QT>, pv, window, sinks, static_cast<T*>(out), lse, wk));
+    SMLM_CUDA(cudaLaunchKernelEx(&cfg, shared ? paged_join_kernel<T, S::TT, S::QT, 8> : paged_join_kernel<T, S::TT, S::QT, 1>,
+                                 pv, window, sinks, columns, static_cast<T*>(out), lse, wk));
     return SMLM_OK;
 }
 
@@ -1028,6 +1033,10 @@ extern "C" int smlm_paged_attention(const void* q, const void* k_pages, const vo
                    "paged_attention: q and out have to be 16-byte aligned");
     SMLM_CHECK_ARG(window >= 0 && sinks >= 0, "paged_attention: window %lld, sinks %lld", (long long)window,
                    (long long)sinks);
+    // the list of tiles is counted in 31 bits
+    SMLM_CHECK_ARG((double)batch * hq * ((double)max_blocks * page_size / 16 + HEAD + 1) < 2147483648.0,
+                   "paged_attention: %lld sequences x %lld heads x up to %lld tokens: fewer rows a call",
+                   (long long)batch, (long long)hq, (long long)(max_blocks * page_size));
     const int win = (int)std::min<int64_t>(window, INT32_MAX), snk = (int)std::min<int64_t>(sinks, INT32_MAX / 2);
     Workspace ws(workspace, workspace_bytes);
     SplitWork wk;
