@@ -26,6 +26,11 @@ constexpr int SPLIT_WARPS = 4, SPLIT_THREADS = SPLIT_WARPS * 32;
 constexpr int JOIN_THREADS = 256;
 constexpr int HEAD = 2;  // what beginning an item costs, in tiles (two dependent loads and the output), in the cut
 
+// Programmatic dependent launch: a kernel that was launched while its predecessor runs waits for that one's end and
+// memory before it touches anything the predecessor wrote; grid_release lets the successor be launched.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;"); }
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -528,7 +533,8 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP, NT>::BLOCKS)
     __shared__ int4 pre[SPLIT_THREADS / 4];
     __shared__ int part[SPLIT_WARPS];
     __shared__ uint4 qs[S::WIDE ? SPLIT_WARPS * NT * S::KJ * 32 : 1];
-    asm volatile("griddepcontrol.launch_dependents;");
+    grid_wait();
+    grid_release();
 
     const int lane = lane_id(), warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
     const int group = pv.hq / pv.hkv, gt = (group + QT - 1) / QT, items = pv.hkv * gt;
@@ -546,8 +552,8 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP, NT>::BLOCKS)
         }
         return x;
     };
-    // The sequence, the item and the place in it where this worker starts, and how much it does. Up to 32 rows: each
-    // warp for itself, a lane a row; more: a thread has `chunk` rows, and the warp looks for its start in the block's
+    // The sequence, the item and the place in it where this worker starts, and how much it does. Up to 128 rows:
+    // each warp for itself, a lane up to four rows; more: a thread has `chunk` rows, and the warp looks for its start in the block's
     // sums and then among the rows.
     const int workers = gridDim.x * SPLIT_WARPS, worker = warp * gridDim.x + blockIdx.x;  // one warp per SM first
     int b = 0, off, left;
@@ -563,11 +569,28 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP, NT>::BLOCKS)
         b += beyond ? at : 32;
         return beyond != 0;
     };
-    if (pv.batch <= 32) {
-        const int w = lane < pv.batch ? cost(lane, status) : 0, x = inclusive(w);
+    if (pv.batch <= 128) {
+        const int each = (pv.batch + 31) / 32;
+        int w[4], sum = 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int r = lane * each + k;
+            w[k] = k < each && r < pv.batch ? cost(r, status) : 0;
+            sum += w[k];
+        }
+        const int x = inclusive(sum);
         cut(__shfl_sync(FULL, x, 31));
         if (left <= 0) return;
-        among(x, w);
+        const int at = __ffs(__ballot_sync(FULL, x > off)) - 1;
+        off -= __shfl_sync(FULL, x - sum, at);
+        b = at * each;
+#pragma unroll
+        for (int k = 0; k < 3; k++) {
+            const int wk = __shfl_sync(FULL, w[k], at);
+            if (off < wk) break;
+            off -= wk;
+            b++;
+        }
     } else {
         const int chunk = (pv.batch + SPLIT_THREADS - 1) / SPLIT_THREADS;
         const int r0 = min(pv.batch, (int)threadIdx.x * chunk), r1 = min(pv.batch, r0 + chunk);
@@ -674,6 +697,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(PageView pv, i
                                                                   T* __restrict__ out, float* __restrict__ lse,
                                                                   SplitWork wk) {
     constexpr int SETS = 4 * W, U = 8, UNITS = JOIN_THREADS / 32 / W;
+    grid_release();
     const int lane = lane_id(), warp = threadIdx.x / 32 % W;
     const uint32_t unit = blockIdx.x * UNITS + threadIdx.x / (32 * W);  // (sequence, query head, 32 columns)
     if (unit >= (uint32_t)pv.batch * pv.hq * columns) return;
@@ -684,7 +708,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(PageView pv, i
     const int set = 4 * warp + lane / 8, x = col * 32 + lane % 8 * 4;
     T* dst = out + head * pv.d + x;
     const bool mine = set == 0 && x < pv.d, logs = lse && set == 0 && lane == 0 && col == 0;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    grid_wait();
     if (tiles == 0) {
         if (mine) dst[0] = dst[1] = dst[2] = dst[3] = narrow<T>(0.f);
         if (logs) lse[head] = -INFINITY;
@@ -793,6 +817,8 @@ __global__ void __launch_bounds__(APPEND_THREADS)
     __shared__ int pos_of[APPEND_TOKENS];
     __shared__ int state_of[APPEND_TOKENS];  // 1: stored, 0: only its queries, -1: skipped
     __shared__ int64_t k_of[APPEND_TOKENS], v_of[APPEND_TOKENS];
+    grid_wait();
+    grid_release();
     const int64_t first = (int64_t)blockIdx.x * per_block;
     const int count = (int)min((int64_t)per_block, (int64_t)pv.batch * tokens - first);
     const int half = pv.d / 2, lanes = half / CH, heads = pv.hq + 2 * pv.hkv, rot = pv.hq + pv.hkv;
@@ -956,32 +982,39 @@ static void split_work(W& ws, SplitWork& wk, int64_t batch, int64_t hq, int64_t 
     take(wk.o, slots * wk.rows * dp);
 }
 
-template <typename T, int DP, int NT, bool PART, bool SMALL>
-static int launch_split(const PageView& pv, const void* q, float scale, int window, int sinks, void* out, float* lse,
-                        const SplitWork& wk, int* status, cudaStream_t st) {
-    using S = SplitShape<T, DP, NT>;
-    const int blocks = sm_count() * S::BLOCKS;
-    paged_split_kernel<T, DP, NT, PART, SMALL><<<blocks, SPLIT_THREADS, 0, st>>>(
-        pv, static_cast<const T*>(q), scale * 1.4426950408889634074f, window, sinks, static_cast<T*>(out), lse, wk,
-        status);
-    SMLM_LAUNCHED("paged_attention");
-    // launched while the first kernel still runs; it waits for that kernel's end itself
-    const int columns = (pv.d + 31) / 32;
-    const int64_t units = (int64_t)pv.batch * pv.hq * columns;
-    const int64_t items = (int64_t)pv.batch * pv.hkv * ((pv.hq / pv.hkv + S::QT - 1) / S::QT);
-    const bool shared = (int64_t)blocks * SPLIT_WARPS > 32 * items;  // over 32 pieces an item: a block for each
+// Launches while the stream's previous kernel may still run: the kernel calls grid_wait.
+template <typename... P, typename... A>
+static int launch_dependent(void (*kernel)(P...), const char* what, int64_t grid, int threads, cudaStream_t st,
+                            A... args) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(shared ? units : (units + 7) / 8));
-    cfg.blockDim = dim3(JOIN_THREADS);
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(threads);
     cfg.stream = st;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    SMLM_CUDA(cudaLaunchKernelEx(&cfg, shared ? paged_join_kernel<T, S::TT, S::QT, 8> : paged_join_kernel<T, S::TT, S::QT, 1>,
-                                 pv, window, sinks, columns, static_cast<T*>(out), lse, wk));
-    return SMLM_OK;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+    return e == cudaSuccess ? SMLM_OK : cuda_status(e, what);
+}
+
+template <typename T, int DP, int NT, bool PART, bool SMALL>
+static int launch_split(const PageView& pv, const void* q, float scale, int window, int sinks, void* out, float* lse,
+                        const SplitWork& wk, int* status, cudaStream_t st) {
+    using S = SplitShape<T, DP, NT>;
+    const int blocks = sm_count() * S::BLOCKS;
+    int rc = launch_dependent(paged_split_kernel<T, DP, NT, PART, SMALL>, "paged_attention", blocks, SPLIT_THREADS, st, pv,
+                              static_cast<const T*>(q), scale * 1.4426950408889634074f, window, sinks,
+                              static_cast<T*>(out), lse, wk, status);
+    if (rc != SMLM_OK) return rc;
+    const int columns = (pv.d + 31) / 32;
+    const int64_t units = (int64_t)pv.batch * pv.hq * columns;
+    const int64_t items = (int64_t)pv.batch * pv.hkv * ((pv.hq / pv.hkv + S::QT - 1) / S::QT);
+    const bool shared = (int64_t)blocks * SPLIT_WARPS > 32 * items;  // over 32 pieces an item: a block for each
+    return launch_dependent(shared ? paged_join_kernel<T, S::TT, S::QT, 8> : paged_join_kernel<T, S::TT, S::QT, 1>,
+                            "paged_attention: join", shared ? units : (units + 7) / 8, JOIN_THREADS, st, pv, window, sinks,
+                            columns, static_cast<T*>(out), lse, wk);
 }
 
 template <typename T>
@@ -1077,10 +1110,9 @@ extern "C" int smlm_paged_append(const void* qkv, void* k_pages, void* v_pages, 
     const auto reciprocal = [](int64_t n) { return (uint32_t)(((int64_t(1) << 32) + n - 1) / n); };  // unused for 1
     return by_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        paged_append_kernel<T><<<(unsigned)grid, APPEND_THREADS, 0, as_stream(stream)>>>(
-            pv, static_cast<const T*>(qkv), (int)tokens, cos, sin, (int)std::min<int64_t>(max_pos, INT32_MAX),
-            static_cast<T*>(q_out), per_block, reciprocal(pairs), reciprocal(pairs / (hq + 2 * hkv)), status);
-        SMLM_LAUNCHED("paged_append");
-        return SMLM_OK;
+        return launch_dependent(paged_append_kernel<T>, "paged_append", grid, APPEND_THREADS, as_stream(stream), pv,
+                                static_cast<const T*>(qkv), (int)tokens, cos, sin,
+                                (int)std::min<int64_t>(max_pos, INT32_MAX), static_cast<T*>(q_out), per_block,
+                                reciprocal(pairs), reciprocal(pairs / (hq + 2 * hkv)), status);
     });
 }
