@@ -24,7 +24,7 @@ namespace smlm {
 
 constexpr int SPLIT_WARPS = 4, SPLIT_THREADS = SPLIT_WARPS * 32;
 constexpr int JOIN_THREADS = 256;
-constexpr int HEAD = 2;  // what beginning an item costs, in tiles (two dependent loads and the output), in the cut
+constexpr int HEAD = 1;  // what beginning an item costs in the cut, in tiles (measured: 1 and 2 alike, 0 and 4 slower)
 
 // Programmatic dependent launch: a kernel that was launched while its predecessor runs waits for that one's end and
 // memory before it touches anything the predecessor wrote; grid_release lets the successor be launched.
@@ -82,12 +82,15 @@ __device__ __forceinline__ void mma8(float (&c)[4], uint32_t a0, uint32_t a1, ui
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// c += a b, the small products into `small` (the same array, or one of its own). The tensor cores cut the sum of each
+// step off instead of rounding it, so long sums stay out of their accumulators: the scores add up in three, the
+// outputs' parts of 16 tokens are added to the sums with rounding.
 template <bool KEEP>
-__device__ __forceinline__ void mma_split32(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                            const Split32<KEEP>& b0, const Split32<KEEP>& b1) {
+__device__ __forceinline__ void mma_split32(float (&c)[4], float (&small)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                            uint32_t a3, const Split32<KEEP>& b0, const Split32<KEEP>& b1) {
     const Split32<> x0(a0), x1(a1), x2(a2), x3(a3);
-    mma8(c, x0.lo, x1.lo, x2.lo, x3.lo, b0.hi, b1.hi);
-    mma8(c, x0.hi, x1.hi, x2.hi, x3.hi, b0.lo, b1.lo);
+    mma8(small, x0.lo, x1.lo, x2.lo, x3.lo, b0.hi, b1.hi);
+    mma8(small, x0.hi, x1.hi, x2.hi, x3.hi, b0.lo, b1.lo);
     mma8(c, x0.hi, x1.hi, x2.hi, x3.hi, b0.hi, b1.hi);
 }
 
@@ -180,6 +183,10 @@ struct Stream {
     using S = SplitShape<T, DP, NT>;
     static constexpr int CH = S::CH, TT = S::TT, NS = S::NS, KJ = S::KJ, KK = S::KK, VB = S::VB, VR = S::VR, MT = S::MT;
     static constexpr bool WIDE = S::WIDE, HALVES = S::HALVES, F = S::ES == 4;
+    // The tile after next goes to L2 where few bytes are in flight otherwise (two eights of queries: 8 warps an SM; d
+    // well below DP): 64 x 8192 tokens, 32 heads on one: 107 -> 96 us, d 80: 70 -> 66, fp32 d 128: 58 -> 56. Where the
+    // loads alone fill the memory's queues it costs: d 64 40.3 -> 41.9, one of 131071 tokens 86.8 -> 91.9.
+    static constexpr bool AHEAD = !SMALL && !HALVES && (NT == 2 || (PART && DP == 128) || (F && DP == 128));
     static constexpr unsigned ALL = TT == 32 ? FULL : 0xffffu;
     struct PagesOf {  // the pages of a tile: SMALL: of token `lane`; else of each 16 tokens (the same in all lanes)
         int p[SMALL ? 1 : NS];
@@ -196,6 +203,7 @@ struct Stream {
 
     __device__ __forceinline__ void scores(float (&sc)[NT][NS][4], const uint4 (&kr)[NS][2][KK],
                                            const uint4 (&qf)[NT][WIDE ? 1 : KJ], const uint4* qs, int j0) {
+        float odd[4] = {0.f, 0.f, 0.f, 0.f}, small[4] = {0.f, 0.f, 0.f, 0.f};  // F: second and third accumulator
 #pragma unroll
         for (int s = 0; s < NS; s++)
 #pragma unroll
@@ -208,14 +216,18 @@ struct Stream {
                     else w = qf[n][jj];
                     if constexpr (F) {
                         constexpr bool KEEP = DP > 64;  // the split queries have no registers there
-                        mma_split32(sc[n][s], a.x, e.x, a.y, e.y, Split32<KEEP>(w.x), Split32<KEEP>(w.y));
-                        mma_split32(sc[n][s], a.z, e.z, a.w, e.w, Split32<KEEP>(w.z), Split32<KEEP>(w.w));
+                        mma_split32(sc[n][s], small, a.x, e.x, a.y, e.y, Split32<KEEP>(w.x), Split32<KEEP>(w.y));
+                        mma_split32(odd, small, a.z, e.z, a.w, e.w, Split32<KEEP>(w.z), Split32<KEEP>(w.w));
                     } else {
                         mma16<T>(sc[n][s], a.x, e.x, a.y, e.y, w.x, w.y);
                         mma16<T>(sc[n][s], a.z, e.z, a.w, e.w, w.z, w.w);
                     }
                 }
             }
+        if constexpr (F) {
+#pragma unroll
+            for (int x = 0; x < 4; x++) sc[0][0][x] += odd[x] + small[x];
+        }
     }
 
     // qs: this warp's shared memory, NT KJ 32 vectors (WIDE)
@@ -349,9 +361,28 @@ struct Stream {
 #pragma unroll
             for (int i = 0; i < VB * MT; i++) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
         }
+        auto prefetch = [&](int i, const PagesOf& x) {
+            if constexpr (AHEAD) {
+                const int t0 = span.token(i, TT);
+                const bool is_k = lane < 16;
+                const char* base = reinterpret_cast<const char*>(is_k ? static_cast<const T*>(pv.k) + h * pv.kh
+                                                                      : static_cast<const T*>(pv.v) + h * pv.vh);
+                const uint32_t pb = is_k ? kpb : vpb, tb = is_k ? ktb : vtb;
+#pragma unroll
+                for (int s = 0; s < NS; s++) {
+                    const char* src = base + (uint64_t)(uint32_t)max(x.p[s], 0) * pb +
+                                      (uint64_t)(uint32_t)(((t0 + 16 * s) & slots) + (lane & 15)) * tb;
+#pragma unroll
+                    for (int k = 0; k < (DP * S::ES + 127) / 128; k++)
+                        if (!PART || 128 * k < pv.d * S::ES) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + 128 * k));
+                }
+            }
+        };
+        PagesOf pages_far;
         load_keys(first, pages, 0);
         if (!WIDE) load_values(first, pages, 0);
         if (first + 1 < last) pages_next = pages_at(first + 1);
+        if (AHEAD && first + 2 < last) pages_far = pages_at(first + 2);
         for (int i = first; i < last; i++) {
             float sc[NT][NS][4];
 #pragma unroll
@@ -442,28 +473,45 @@ struct Stream {
             }
             if (WIDE && seen != ALL) clear_unseen(seen, 0);
             if constexpr (F) {
+                // P^T: weight of token 8 r + t4 (+ 4) for query g, from lane (token, query / 2)
+                auto weight = [&](int r, int up) {
+                    const int from = 4 * t4 + (g >> 1) + up;
+                    const float a = __shfl_sync(FULL, sc[0][0][2 * r], from);
+                    const float e = __shfl_sync(FULL, sc[0][0][2 * r + 1], from);
+                    return Split32<>(__float_as_uint(g & 1 ? e : a));
+                };
+                const Split32<> p00 = weight(0, 0), p01 = weight(0, 16), p10 = weight(1, 0), p11 = weight(1, 16);
+                auto add = [&](float (&to)[4], const float (&x)[4]) {
 #pragma unroll
-                for (int s = 0; s < NS; s++)
+                    for (int k = 0; k < 4; k++) to[k] += x[k];
+                };
 #pragma unroll
-                    for (int r = 0; r < 2; r++) {  // tokens 8 r .. 8 r + 7 of the 16
-                        if (HALVES && r) {
-                            load_values(i, pages, 2);
-                            if (seen != ALL) clear_unseen(seen, 2);
-                        }
-                        // P^T: weight of token t4 (+ 4) for query g, from lane (token, query / 2)
-                        const int from = 4 * t4 + (g >> 1);
-                        const float a = __shfl_sync(FULL, sc[0][s][2 * r], from);
-                        const float b1 = __shfl_sync(FULL, sc[0][s][2 * r + 1], from);
-                        const float a4 = __shfl_sync(FULL, sc[0][s][2 * r], from + 16);
-                        const float b4 = __shfl_sync(FULL, sc[0][s][2 * r + 1], from + 16);
-                        const Split32<> p0(__float_as_uint(g & 1 ? b1 : a)), p1(__float_as_uint(g & 1 ? b4 : a4));
-#pragma unroll
-                        for (int vb = 0; vb < VB; vb++) {
-                            const uint4 x = vr[s][HALVES ? 0 : 2 * r][vb], y = vr[s][HALVES ? 1 : 2 * r + 1][vb];
-                            mma_split32(o[0][vb * MT], x.x, x.y, y.x, y.y, p0, p1);
-                            mma_split32(o[0][vb * MT + 1], x.z, x.w, y.z, y.w, p0, p1);
-                        }
+                for (int vb = 0; vb < VB; vb++) {
+                    float e[4] = {0.f, 0.f, 0.f, 0.f}, f[4] = {0.f, 0.f, 0.f, 0.f};
+                    const uint4 x = vr[0][0][vb], y = vr[0][1][vb];
+                    mma_split32(e, e, x.x, x.y, y.x, y.y, p00, p01);
+                    mma_split32(f, f, x.z, x.w, y.z, y.w, p00, p01);
+                    if constexpr (!HALVES) {
+                        const uint4 z = vr[0][2 % VR][vb], w = vr[0][3 % VR][vb];
+                        mma_split32(e, e, z.x, z.y, w.x, w.y, p10, p11);
+                        mma_split32(f, f, z.z, z.w, w.z, w.w, p10, p11);
                     }
+                    add(o[0][vb * MT], e);
+                    add(o[0][vb * MT + 1], f);
+                }
+                if constexpr (HALVES) {
+                    load_values(i, pages, 2);
+                    if (seen != ALL) clear_unseen(seen, 2);
+#pragma unroll
+                    for (int vb = 0; vb < VB; vb++) {
+                        float e[4] = {0.f, 0.f, 0.f, 0.f}, f[4] = {0.f, 0.f, 0.f, 0.f};
+                        const uint4 z = vr[0][0][vb], w = vr[0][1][vb];
+                        mma_split32(e, e, z.x, z.y, w.x, w.y, p10, p11);
+                        mma_split32(f, f, z.z, z.w, w.z, w.w, p10, p11);
+                        add(o[0][vb * MT], e);
+                        add(o[0][vb * MT + 1], f);
+                    }
+                }
             } else {
 #pragma unroll
                 for (int s = 0; s < NS; s++) {
@@ -502,7 +550,13 @@ struct Stream {
                 if (WIDE) load_keys(i + 1, pages_next, 0);
                 else load_values(i + 1, pages_next, 0);
                 pages = pages_next;
-                if (i + 2 < last) pages_next = pages_at(i + 2);
+                if (AHEAD && i + 2 < last) {
+                    prefetch(i + 2, pages_far);
+                    pages_next = pages_far;
+                    if (i + 3 < last) pages_far = pages_at(i + 3);
+                } else if (i + 2 < last) {
+                    pages_next = pages_at(i + 2);
+                }
             }
         }
 #pragma unroll
