@@ -247,23 +247,10 @@ def read_status(device, reset=True):
     return v
 
 
-# The same for calls that are worth a few microseconds in all (one decoding step makes two per layer): addresses as
-# plain integers, no wrapper objects.
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-
-
-def stream_int(device):
-    if _raw_stream is None or device.index is None:
-        return torch.cuda.current_stream(device).cuda_stream
-    return _raw_stream(device.index)
-
-
 def status_int(device):
-    st = _STATUS.get(device.index)
-    if st is None:
-        p = status_ptr(device)
-        return p.value if p is not None else None
-    return st.data_ptr()
+    """The status word's address as an integer (None: no word)."""
+    p = status_ptr(device)
+    return p.value if p is not None else None
 
 
 def instrumented():

@@ -19,71 +19,40 @@ fp32 and rounded once. What a row's table and length do not cover is never used,
 outside their range, pages outside the pool and an exhausted pool do not fault: the token or row is left out and a flag
 of the device status word is set (SMLM_B200_CHECK=1 turns it into an exception).
 """
-import ctypes
+import importlib.machinery
+import importlib.util
+import os
 
 import torch
 
 from . import _lib as L
 
-
-_I32 = torch.int32
-_CODES = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
-_Strides = ctypes.c_int64 * 6
+_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
-def _int32(what, t, dim):
-    if t.dtype != _I32 or t.dim() != dim or (t.numel() and t.stride(-1) != 1):
-        raise ValueError(f"{what} has to be an int32 tensor of {dim} dimension(s) with contiguous rows")
+def _load():
+    """The native binding (csrc/binding.cpp): checks, outputs, scratch and launch in one call."""
+    path = os.path.join(os.path.dirname(L.LIB_PATH), "_paged.so")
+    if not os.path.exists(path):
+        raise ImportError(f"{path} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'` "
+                          "or `make -C sparse-memory-lm_b200/csrc`")
+    loader = importlib.machinery.ExtensionFileLoader("_paged", path)
+    module = importlib.util.module_from_spec(importlib.machinery.ModuleSpec("_paged", loader, origin=path))
+    loader.exec_module(module)
+    module.init(lambda index: L.status_int(torch.device("cuda", index)))
+    return module
+
+
+_native = _load()
 
 
 def _call(name, launches, device, fn, *args):
-    """fn(*args, status, stream) on the current stream."""
     if not L.instrumented():
-        rc = fn(*args, L.status_int(device), L.stream_int(device))
-        if rc:
-            L.check(rc, name)
-        return
+        return fn(*args)
     with L.timed(name, launches):
-        rc = fn(*args, L.status_int(device), L.stream_int(device))
-    L.check(rc, name)
+        out = fn(*args)
     L.after(device, name)
-
-
-def _cache(what, x, k_pages, v_pages, table, lengths, batch):
-    """Checks a layer's pages against the activations x; returns the pages' shape, both strides and the dtype code."""
-    shape, dtype = k_pages.shape, x.dtype
-    if len(shape) != 4 or shape != v_pages.shape:
-        raise ValueError(f"{what}: k_pages and v_pages have to be (pages, key heads, page_size, head dimension)")
-    if dtype != k_pages.dtype or dtype != v_pages.dtype:
-        raise ValueError(f"{what}: activations and pages have to be of one type, got {x.dtype}, {k_pages.dtype}, "
-                         f"{v_pages.dtype}")
-    code = _CODES.get(dtype)
-    if code is None:
-        raise ValueError(f"{what}: unsupported type {dtype} (fp32, bf16 or fp16)")
-    ks, vs = k_pages.stride(), v_pages.stride()
-    if ks[3] != 1 or vs[3] != 1:
-        raise ValueError(f"{what}: the pages' head dimension has to be contiguous")
-    if table.dtype != _I32 or table.dim() != 2 or table.shape[0] != batch or (batch and table.stride(1) != 1):
-        raise ValueError(f"{what}: the table has to be int32, ({batch} sequences, blocks) with contiguous rows; got "
-                         f"{table.dtype} {tuple(table.shape)}")
-    if lengths.dtype != _I32 or lengths.shape != (batch,) or not lengths.is_contiguous():
-        raise ValueError(f"{what}: lengths has to be a contiguous int32 tensor of {batch} lengths; got "
-                         f"{lengths.dtype} {tuple(lengths.shape)}")
-    if not (x.is_cuda and x.device == k_pages.device == v_pages.device == table.device == lengths.device):
-        L.require_cuda(x, k_pages, v_pages, table, lengths)
-    return shape, _Strides(ks[0], ks[1], ks[2], vs[0], vs[1], vs[2]), code
-
-
-_WORKSPACE = {}
-
-
-def _attention_workspace(*sizes):
-    """smlm_paged_attention_workspace, asked once per sizes and device."""
-    key = (torch.cuda.current_device(), *sizes)
-    n = _WORKSPACE.get(key)
-    if n is None:
-        n = _WORKSPACE[key] = L.lib().smlm_paged_attention_workspace(*sizes)
-    return n
+    return out
 
 
 def paged_attention(q, k_pages, v_pages, table, lengths, *, scale=None, window=0, sinks=0, return_lse=False):
@@ -95,26 +64,8 @@ def paged_attention(q, k_pages, v_pages, table, lengths, *, scale=None, window=0
     entry is not -1; with window > 0 only the last `window` tokens and the first `sinks` are. scale defaults to
     d ** -0.5. A row that sees nothing gives 0. return_lse: also the logarithm of the softmax's sum, fp32 (B, query
     heads), -inf for such a row."""
-    if q.dim() != 3:
-        raise ValueError(f"paged_attention: q has to be (sequences, heads, head dimension), got {tuple(q.shape)}")
-    B, HQ, D = q.shape
-    (P, HKV, page, Dk), strides, code = _cache("paged_attention", q, k_pages, v_pages, table, lengths, B)
-    if D != Dk or HQ % HKV:
-        raise ValueError(f"paged_attention: {HQ} query heads of {D} over {HKV} key heads of {Dk}")
-    if window < 0 or sinks < 0:
-        raise ValueError(f"paged_attention: window {window}, sinks {sinks}")
-    if not q.is_contiguous():
-        q = q.contiguous()
-    dev = q.device
-    out = torch.empty_like(q)
-    lse = torch.empty(B, HQ, dtype=torch.float32, device=dev) if return_lse else None
-    nbytes = _attention_workspace(B, HQ, HKV, D, code)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _call("paged_attention", 2, dev, L.lib().smlm_paged_attention, q.data_ptr(), k_pages.data_ptr(),
-          v_pages.data_ptr(), code, strides, table.data_ptr(), table.stride(0), lengths.data_ptr(), B, HQ, HKV, D, P,
-          page, table.shape[1], D ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(),
-          lse.data_ptr() if return_lse else None, ws.data_ptr(), nbytes)
-    return (out, lse) if return_lse else out
+    return _call("paged_attention", 2, q.device, _native.attention, q, k_pages, v_pages, table, lengths, scale, window,
+                 sinks, return_lse)
 
 
 def paged_append(qkv, k_pages, v_pages, table, lengths, cos=None, sin=None):
@@ -123,117 +74,38 @@ def paged_append(qkv, k_pages, v_pages, table, lengths, cos=None, sin=None):
     before a shorter chunk and is not stored), queries are returned, (B, T, query heads, d). With cos / sin (fp32,
     (positions, d / 2)) queries and keys are turned by the half-split rotary embedding of their position, in fp32,
     rounded once."""
-    if qkv.dim() != 3:
-        raise ValueError(f"paged_append: qkv has to be (sequences, tokens, width), got {tuple(qkv.shape)}")
-    B, T, W = qkv.shape
-    (P, HKV, page, D), strides, code = _cache("paged_append", qkv, k_pages, v_pages, table, lengths, B)
-    HQ = W // D - 2 * HKV
-    if W % D or HQ < 1 or HQ % HKV:
-        raise ValueError(f"paged_append: a projection of {W} values with {HKV} key heads of {D}")
-    dev = qkv.device
-    positions, pcos, psin = 0, None, None
-    if cos is not None or sin is not None:
-        if cos is None or sin is None:
-            raise ValueError("paged_append: cos and sin come together")
-        if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.shape != sin.shape or cos.dim() != 2 or \
-                2 * cos.shape[1] != D or not (cos.is_contiguous() and sin.is_contiguous()):
-            raise ValueError(f"paged_append: cos and sin have to be contiguous fp32 (positions, {D // 2})")
-        if cos.device != dev or sin.device != dev:
-            L.require_cuda(qkv, cos, sin)
-        positions, pcos, psin = cos.shape[0], cos.data_ptr(), sin.data_ptr()
-    if not qkv.is_contiguous():
-        qkv = qkv.contiguous()
-    q = torch.empty((B, T, HQ, D), dtype=qkv.dtype, device=dev)
-    _call("paged_append", 1, dev, L.lib().smlm_paged_append, qkv.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-          code, strides, table.data_ptr(), table.stride(0), lengths.data_ptr(), B, T, HQ, HKV, D, P, page,
-          table.shape[1], pcos, psin, positions, q.data_ptr())
-    return q
+    return _call("paged_append", 1, qkv.device, _native.append, qkv, k_pages, v_pages, table, lengths, cos, sin)
 
 
 # --------------------------------------------------------------------------------------------- the pages
-def _tables(what, table, lengths, refcount, *rows):
-    _int32(f"{what}: table", table, 2)
-    _int32(f"{what}: reference counts", refcount, 1)
-    dev = table.device
-    same = table.is_cuda and refcount.device == dev
-    for r in rows:
-        _int32(f"{what}: row numbers", r, 1)
-        same = same and r.device == dev
-    if lengths is not None:
-        _int32(f"{what}: lengths", lengths, 1)
-        if lengths.shape[0] != table.shape[0]:
-            raise ValueError(f"{what}: {table.shape[0]} table rows, {lengths.shape[0]} lengths")
-        same = same and lengths.device == dev
-    if not same:
-        L.require_cuda(table, lengths, refcount, *rows)
-    return dev
-
-
-def _pool(what, pool, refcount):
-    """(layers, 2, pages, key heads, page_size, d), contiguous -> (planes, heads, bytes of a head's token, page_size)"""
-    if pool.dim() != 6 or pool.shape[1] != 2 or not pool.is_contiguous():
-        raise ValueError(f"{what}: the pool has to be a contiguous (layers, 2, pages, key heads, page_size, head "
-                         f"dimension) tensor, got {tuple(pool.shape)}")
-    if pool.shape[2] != refcount.shape[0]:
-        raise ValueError(f"{what}: {pool.shape[2]} pages, {refcount.shape[0]} reference counts")
-    if pool.device != refcount.device:
-        L.require_cuda(pool, refcount)
-    return 2 * pool.shape[0], pool.shape[3], pool.shape[5] * pool.element_size(), pool.shape[4]
-
-
 def pages_free(table, lengths, refcount, rows):
     """The sequences `rows` (int32) end: their pages are released, their table entries become -1, their lengths 0."""
-    dev = _tables("pages_free", table, lengths, refcount, rows)
-    _call("pages_free", 1, dev, L.lib().smlm_pages_free, table.data_ptr(), table.stride(0), *table.shape,
-          lengths.data_ptr(), refcount.data_ptr(), refcount.shape[0], rows.data_ptr(), rows.shape[0])
+    _call("pages_free", 1, table.device, _native.pages_free, table, lengths, refcount, rows)
 
 
 def pages_trim(table, lengths, refcount, rows, page_size, window, sinks=0):
     """Releases the pages of the sequences `rows` that paged_attention with this window and these sinks no longer reads:
     those that hold only tokens in [sinks, length - window)."""
-    dev = _tables("pages_trim", table, lengths, refcount, rows)
-    _call("pages_trim", 1, dev, L.lib().smlm_pages_trim, table.data_ptr(), table.stride(0), *table.shape,
-          lengths.data_ptr(), refcount.data_ptr(), refcount.shape[0], page_size, rows.data_ptr(), rows.shape[0],
-          window, sinks)
+    _call("pages_trim", 1, table.device, _native.pages_trim, table, lengths, refcount, rows, page_size, window, sinks)
 
 
 def pages_extend(table, lengths, refcount, rows, n_new, page_size):
     """Every sequence in `rows` grows by n_new tokens: lengths[r] += n_new, with the lowest free pages (row by row) where
     its last page is full. A sequence that finds too few keeps its length."""
-    dev = _tables("pages_extend", table, lengths, refcount, rows)
-    lib, n, pages = L.lib(), rows.shape[0], refcount.shape[0]
-    nbytes = lib.smlm_pages_extend_workspace(n, pages)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _call("pages_extend", 1, dev, lib.smlm_pages_extend, table.data_ptr(), table.stride(0), *table.shape,
-          lengths.data_ptr(), refcount.data_ptr(), pages, page_size, rows.data_ptr(), n, n_new, ws.data_ptr(), nbytes)
+    _call("pages_extend", 1, table.device, _native.pages_extend, table, lengths, refcount, rows, n_new, page_size)
 
 
 def pages_fork(pool, table, lengths, refcount, parents, children):
     """Sequence children[i] becomes a copy of sequence parents[i] as it was before the call, for all i at once (a row may
     be a parent and a child: a beam's reordering); what the children held is released. Whole pages are shared, the
     tokens of a partly filled last page are copied in all layers. pool: (layers, 2, pages, key heads, page_size, d)."""
-    dev = _tables("pages_fork", table, lengths, refcount, parents, children)
-    planes, heads, token, page = _pool("pages_fork", pool, refcount)
-    if parents.shape != children.shape:
-        raise ValueError(f"pages_fork: {parents.shape[0]} parents, {children.shape[0]} children")
-    lib, n = L.lib(), parents.shape[0]
-    nbytes = lib.smlm_pages_fork_workspace(n, *table.shape, refcount.shape[0])
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _call("pages_fork", 2, dev, lib.smlm_pages_fork, pool.data_ptr(), planes, heads, token, table.data_ptr(),
-          table.stride(0), *table.shape, lengths.data_ptr(), refcount.data_ptr(), refcount.shape[0], page,
-          parents.data_ptr(), children.data_ptr(), n, ws.data_ptr(), nbytes)
+    _call("pages_fork", 2, table.device, _native.pages_fork, table, lengths, refcount, pool, parents, children)
 
 
 def pages_compact(pool, table, refcount):
     """Moves the pages in use to the lowest numbers, in the pool, the table and the counts: with n in use, the k-th used
     page numbered n or above goes to the k-th free page below n."""
-    dev = _tables("pages_compact", table, None, refcount)
-    planes, heads, token, page = _pool("pages_compact", pool, refcount)
-    lib = L.lib()
-    nbytes = lib.smlm_pages_compact_workspace(refcount.shape[0])
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _call("pages_compact", 2, dev, lib.smlm_pages_compact, pool.data_ptr(), planes, heads, token, table.data_ptr(),
-          table.stride(0), *table.shape, refcount.data_ptr(), refcount.shape[0], page, ws.data_ptr(), nbytes)
+    _call("pages_compact", 2, table.device, _native.pages_compact, table, refcount, pool)
 
 
 # ----------------------------------------------------------------------------------------------- the cache
@@ -249,7 +121,7 @@ class PagedKVCache:
                  device="cuda"):
         if page_size < 1 or page_size > 4096 or page_size & (page_size - 1):
             raise ValueError(f"page_size {page_size} (a power of two up to 4096)")
-        if dtype not in _CODES:
+        if dtype not in _TYPES:
             raise ValueError(f"unsupported type {dtype} (fp32, bf16 or fp16)")
         if head_dim % 16 or not 16 <= head_dim <= 256:
             raise ValueError(f"head dimension {head_dim} (a multiple of 16 up to 256)")
