@@ -5,6 +5,32 @@
 
 namespace smlm {
 
+// Programmatic dependent launch: a kernel that was launched while its predecessor runs waits for that one's end and
+// memory before it touches anything the predecessor wrote; grid_release lets the successor be launched.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;"); }
+
+// Launches while the stream's previous kernel may still run (the kernel calls grid_wait before anything else), in
+// clusters of `cluster` blocks.
+template <typename... P, typename... A>
+inline int launch_dependent(void (*kernel)(P...), const char* what, int cluster, int64_t grid, int threads,
+                            cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(threads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+    return e == cudaSuccess ? SMLM_OK : cuda_status(e, what);
+}
+
 // One layer's pages. Token t of a sequence lies in page table[row][t >> page_shift], slot t & (page - 1); its key of
 // head h starts at k + page * kp + h * kh + slot * kt (64-bit element offsets: a long cache passes 2^31 elements).
 struct PageView {

@@ -26,11 +26,6 @@ constexpr int SPLIT_WARPS = 4, SPLIT_THREADS = SPLIT_WARPS * 32;
 constexpr int JOIN_THREADS = 256;
 constexpr int HEAD = 1;  // what beginning an item costs in the cut, in tiles (measured: 1 and 2 alike, 0 and 4 slower)
 
-// Programmatic dependent launch: a kernel that was launched while its predecessor runs waits for that one's end and
-// memory before it touches anything the predecessor wrote; grid_release lets the successor be launched.
-__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;"); }
-
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -1036,29 +1031,12 @@ static void split_work(W& ws, SplitWork& wk, int64_t batch, int64_t hq, int64_t 
     take(wk.o, slots * wk.rows * dp);
 }
 
-// Launches while the stream's previous kernel may still run: the kernel calls grid_wait.
-template <typename... P, typename... A>
-static int launch_dependent(void (*kernel)(P...), const char* what, int64_t grid, int threads, cudaStream_t st,
-                            A... args) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3(threads);
-    cfg.stream = st;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
-    return e == cudaSuccess ? SMLM_OK : cuda_status(e, what);
-}
-
 template <typename T, int DP, int NT, bool PART, bool SMALL>
 static int launch_split(const PageView& pv, const void* q, float scale, int window, int sinks, void* out, float* lse,
                         const SplitWork& wk, int* status, cudaStream_t st) {
     using S = SplitShape<T, DP, NT>;
     const int blocks = sm_count() * S::BLOCKS;
-    int rc = launch_dependent(paged_split_kernel<T, DP, NT, PART, SMALL>, "paged_attention", blocks, SPLIT_THREADS, st, pv,
+    int rc = launch_dependent(paged_split_kernel<T, DP, NT, PART, SMALL>, "paged_attention", 1, blocks, SPLIT_THREADS, st, pv,
                               static_cast<const T*>(q), scale * 1.4426950408889634074f, window, sinks,
                               static_cast<T*>(out), lse, wk, status);
     if (rc != SMLM_OK) return rc;
@@ -1067,7 +1045,7 @@ static int launch_split(const PageView& pv, const void* q, float scale, int wind
     const int64_t items = (int64_t)pv.batch * pv.hkv * ((pv.hq / pv.hkv + S::QT - 1) / S::QT);
     const bool shared = (int64_t)blocks * SPLIT_WARPS > 32 * items;  // over 32 pieces an item: a block for each
     return launch_dependent(shared ? paged_join_kernel<T, S::TT, S::QT, 8> : paged_join_kernel<T, S::TT, S::QT, 1>,
-                            "paged_attention: join", shared ? units : (units + 7) / 8, JOIN_THREADS, st, pv, window, sinks,
+                            "paged_attention: join", 1, shared ? units : (units + 7) / 8, JOIN_THREADS, st, pv, window, sinks,
                             columns, static_cast<T*>(out), lse, wk);
 }
 
@@ -1164,7 +1142,7 @@ extern "C" int smlm_paged_append(const void* qkv, void* k_pages, void* v_pages, 
     const auto reciprocal = [](int64_t n) { return (uint32_t)(((int64_t(1) << 32) + n - 1) / n); };  // unused for 1
     return by_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        return launch_dependent(paged_append_kernel<T>, "paged_append", grid, APPEND_THREADS, as_stream(stream), pv,
+        return launch_dependent(paged_append_kernel<T>, "paged_append", 1, grid, APPEND_THREADS, as_stream(stream), pv,
                                 static_cast<const T*>(qkv), (int)tokens, cos, sin,
                                 (int)std::min<int64_t>(max_pos, INT32_MAX), static_cast<T*>(q_out), per_block,
                                 reciprocal(pairs), reciprocal(pairs / (hq + 2 * hkv)), status);

@@ -42,6 +42,8 @@ __device__ __forceinline__ void drop_entry(const Pages& pg, int32_t* entry) {
 }
 
 __global__ void __launch_bounds__(256) pages_free_kernel(Pages pg, const int32_t* rows) {
+    grid_wait();
+    grid_release();
     const int r = rows[blockIdx.x];
     if (!row_ok(pg, r)) return;
     for (int j = threadIdx.x; j < pg.max_blocks; j += blockDim.x) drop_entry(pg, pg.table + r * pg.table_stride + j);
@@ -51,6 +53,8 @@ __global__ void __launch_bounds__(256) pages_free_kernel(Pages pg, const int32_t
 // Releases the pages that hold only tokens in [sinks, length - window).
 __global__ void __launch_bounds__(256) pages_trim_kernel(Pages pg, const int32_t* rows, int shift, int window,
                                                          int sinks) {
+    grid_wait();
+    grid_release();
     const int r = rows[blockIdx.x];
     if (!row_ok(pg, r)) return;
     const int64_t first = (((int64_t)sinks + (1 << shift) - 1) >> shift);
@@ -170,6 +174,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) pages_extend_kernel(Pages pg, co
                                                                     int shift, int32_t* offset, int32_t* len_of,
                                                                     int32_t* list, int32_t* totals) {
     constexpr int TAKEN = INT32_MIN;
+    grid_wait();
+    grid_release();
     const Team team;
     const int64_t cap = (int64_t)pg.max_blocks << shift;
     auto blocks = [&](int64_t len) { return (int)((len + (1 << shift) - 1) >> shift); };
@@ -221,6 +227,8 @@ struct CopyList {
 __global__ void __launch_bounds__(PLAN_THREADS)
     pages_fork_kernel(Pages pg, const int32_t* parents, const int32_t* children, int n, int shift, int32_t* claim,
                       int32_t* snap, int32_t* snap_len, int32_t* offset, int32_t* list, int32_t* totals, CopyList cl) {
+    grid_wait();
+    grid_release();
     const Team team;
     const int mb = pg.max_blocks, lane = lane_id();
     const int warp0 = team.thread() >> 5, warps = team.threads() >> 5;
@@ -310,6 +318,8 @@ __global__ void __launch_bounds__(PLAN_THREADS)
 // where page p went. Each thread has a contiguous piece of the pages; two scans give L and the ranks.
 __global__ void __launch_bounds__(PLAN_THREADS) pages_compact_kernel(Pages pg, int32_t* to, int32_t* live_out,
                                                                      int32_t* totals, CopyList cl) {
+    grid_wait();
+    grid_release();
     const Team team;
     const int per = (pg.n_pages + team.threads() - 1) / team.threads();
     const int a = min(pg.n_pages, team.thread() * per), e = min(pg.n_pages, a + per);
@@ -350,6 +360,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) pages_compact_kernel(Pages pg, i
 __global__ void __launch_bounds__(256) pages_copy_kernel(char* pool, CopyList cl, int planes, int heads, int n_pages,
                                                          int page_size, int token_bytes, Pages pg, const int32_t* to,
                                                          const int32_t* live) {
+    grid_wait();
+    grid_release();
     const int64_t thread = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (to) {
         const int first = *live;
@@ -420,18 +432,7 @@ template <typename... P, typename... A>
 static int launch_plan(void (*kernel)(P...), const char* what, int64_t entries, cudaStream_t st, A... args) {
     int size = 1;
     while (size < MAX_TEAM && (int64_t)size * PLAN_THREADS < entries) size *= 2;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(size);
-    cfg.blockDim = dim3(PLAN_THREADS);
-    cfg.stream = st;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = size;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
-    return e == cudaSuccess ? SMLM_OK : cuda_status(e, what);
+    return launch_dependent(kernel, what, size, size, PLAN_THREADS, st, args...);
 }
 
 static int copy_grid(int64_t most_units) {
@@ -451,9 +452,7 @@ extern "C" int smlm_pages_free(int32_t* table, int64_t table_stride, int64_t tab
                                n_pages, 1, status);
     if (rc != SMLM_OK) return rc;
     SMLM_CHECK_ARG(rows && lengths && n > 0 && n <= INT32_MAX, "pages_free: %lld rows", (long long)n);
-    pages_free_kernel<<<(unsigned)n, 256, 0, as_stream(stream)>>>(pg, rows);
-    SMLM_LAUNCHED("pages_free");
-    return SMLM_OK;
+    return launch_dependent(pages_free_kernel, "pages_free", 1, n, 256, as_stream(stream), pg, rows);
 }
 
 extern "C" int smlm_pages_trim(int32_t* table, int64_t table_stride, int64_t table_rows, int64_t max_blocks,
@@ -468,11 +467,8 @@ extern "C" int smlm_pages_trim(int32_t* table, int64_t table_stride, int64_t tab
     SMLM_CHECK_ARG(rows && lengths && n > 0 && n <= INT32_MAX, "pages_trim: %lld rows", (long long)n);
     SMLM_CHECK_ARG(window >= 1 && sinks >= 0, "pages_trim: window %lld (at least 1), sinks %lld", (long long)window,
                    (long long)sinks);
-    pages_trim_kernel<<<(unsigned)n, 256, 0, as_stream(stream)>>>(pg, rows, log2_of(page_size),
-                                                                  (int)std::min<int64_t>(window, INT32_MAX),
-                                                                  (int)std::min<int64_t>(sinks, INT32_MAX));
-    SMLM_LAUNCHED("pages_trim");
-    return SMLM_OK;
+    return launch_dependent(pages_trim_kernel, "pages_trim", 1, n, 256, as_stream(stream), pg, rows, log2_of(page_size),
+                            (int)std::min<int64_t>(window, INT32_MAX), (int)std::min<int64_t>(sinks, INT32_MAX));
 }
 
 extern "C" size_t smlm_pages_extend_workspace(int64_t n, int64_t n_pages) {
@@ -504,7 +500,7 @@ extern "C" int smlm_pages_extend(int32_t* table, int64_t table_stride, int64_t t
         set_error("pages_extend: workspace of %zu bytes, %zu needed", workspace_bytes, ws.used);
         return SMLM_ERR_WORKSPACE;
     }
-    return launch_plan(pages_extend_kernel, "pages_extend", std::max(n, n_pages / 4), as_stream(stream), pg, rows, (int)n,
+    return launch_plan(pages_extend_kernel, "pages_extend", std::max(n, n_pages), as_stream(stream), pg, rows, (int)n,
                        (int)n_new, log2_of(page_size), offset, len_of, list, totals);
 }
 
@@ -547,14 +543,12 @@ extern "C" int smlm_pages_fork(void* pool, int64_t planes, int64_t heads, int64_
         set_error("pages_fork: workspace of %zu bytes, %zu needed", workspace_bytes, ws.used);
         return SMLM_ERR_WORKSPACE;
     }
-    rc = launch_plan(pages_fork_kernel, "pages_fork: plan", std::max(32 * n, n_pages / 4), as_stream(stream), pg,
+    rc = launch_plan(pages_fork_kernel, "pages_fork: plan", std::max(32 * n, n_pages), as_stream(stream), pg,
                      parents, children, (int)n, log2_of(page_size), claim, snap, snap_len, offset, list, totals, cl);
     if (rc != SMLM_OK) return rc;
-    pages_copy_kernel<<<copy_grid(n * planes * heads), 256, 0, as_stream(stream)>>>(
-        static_cast<char*>(pool), cl, (int)planes, (int)heads, (int)n_pages, (int)page_size, (int)token_bytes, pg,
-        nullptr, nullptr);
-    SMLM_LAUNCHED("pages_fork: copy");
-    return SMLM_OK;
+    return launch_dependent(pages_copy_kernel, "pages_fork: copy", 1, copy_grid(n * planes * heads), 256,
+                            as_stream(stream), static_cast<char*>(pool), cl, (int)planes, (int)heads, (int)n_pages,
+                            (int)page_size, (int)token_bytes, pg, nullptr, nullptr);
 }
 
 extern "C" size_t smlm_pages_compact_workspace(int64_t n_pages) {
@@ -585,12 +579,10 @@ extern "C" int smlm_pages_compact(void* pool, int64_t planes, int64_t heads, int
         set_error("pages_compact: workspace of %zu bytes, %zu needed", workspace_bytes, ws.used);
         return SMLM_ERR_WORKSPACE;
     }
-    rc = launch_plan(pages_compact_kernel, "pages_compact: plan", n_pages / 4, as_stream(stream), pg, to, cl.count + 1,
+    rc = launch_plan(pages_compact_kernel, "pages_compact: plan", n_pages, as_stream(stream), pg, to, cl.count + 1,
                      totals, cl);
     if (rc != SMLM_OK) return rc;
-    pages_copy_kernel<<<copy_grid(n_pages / 2 * planes * heads), 256, 0, as_stream(stream)>>>(
-        static_cast<char*>(pool), cl, (int)planes, (int)heads, (int)n_pages, (int)page_size, (int)token_bytes, pg, to,
-        cl.count + 1);
-    SMLM_LAUNCHED("pages_compact: copy");
-    return SMLM_OK;
+    return launch_dependent(pages_copy_kernel, "pages_compact: copy", 1, copy_grid(n_pages / 2 * planes * heads), 256,
+                            as_stream(stream), static_cast<char*>(pool), cl, (int)planes, (int)heads, (int)n_pages,
+                            (int)page_size, (int)token_bytes, pg, to, cl.count + 1);
 }
