@@ -10,6 +10,11 @@ namespace smlm {
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;"); }
 
+// Barrier of the blocks of a cluster; what a block wrote before it is seen by the others after it.
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 // Launches while the stream's previous kernel may still run (the kernel calls grid_wait before anything else), in
 // clusters of `cluster` blocks.
 template <typename... P, typename... A>

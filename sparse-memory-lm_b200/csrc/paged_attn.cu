@@ -1,4 +1,6 @@
 // Attention of one new token per sequence over a paged key-value cache, and the append that fills it.
+#include <atomic>
+
 #include "paged.cuh"
 
 namespace smlm {
@@ -128,6 +130,20 @@ __device__ __forceinline__ uint4 narrow16(const float (&f)[16 / sizeof(T)]) {
         else w[i] = pack16<T>(f[2 * i], f[2 * i + 1]);
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// A value in the same place of another block's shared memory (rank in the cluster).
+template <typename V>
+__device__ __forceinline__ V of_block(const V* p, int rank) {
+    uint32_t at;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    V v;
+    if constexpr (sizeof(V) == 16)
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at));
+    else
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at));
+    return v;
 }
 
 // The tiles of one sequence: all of [0, n), or with a window those of the first tokens and of [lo, n).
@@ -735,6 +751,100 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP, NT>::BLOCKS)
     }
 }
 
+// Few short sequences: one cluster of blocks per item, its tiles divided among the cluster's warps and joined through
+// the blocks' shared memory, so that the call is one launch and nothing goes through global memory in between.
+template <typename T, int DP, int NT, bool PART, bool SMALL>
+__global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP, NT>::BLOCKS)
+    paged_cluster_kernel(PageView pv, const T* __restrict__ q, float c, int window, int sinks, T* __restrict__ out,
+                         float* __restrict__ lse, int* status) {
+    using S = SplitShape<T, DP, NT>;
+    constexpr int CH = S::CH, TT = S::TT, VB = S::VB, QT = S::QT, FOURS = DP / 4;
+    __shared__ float4 so[SPLIT_WARPS][QT][FOURS];  // before it a warp's queries, in the wide shapes
+    static_assert(!S::WIDE || sizeof(so[0]) >= NT * S::KJ * 32 * sizeof(uint4), "a warp's queries fit its results' place");
+    __shared__ float2 sml[SPLIT_WARPS][QT], joined[QT];
+    grid_wait();
+    grid_release();
+    const int lane = lane_id(), warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
+    const int group = pv.hq / pv.hkv, gt = (group + QT - 1) / QT, items = pv.hkv * gt;
+    uint32_t rank, size;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
+    const int unit = blockIdx.x / size, b = unit / items, h = unit % items / gt, q0 = unit % items % gt * QT;
+    const int cols = min(QT, group - q0);
+    const Span span(row_length(pv, b, rank == 0 ? status : nullptr), window, sinks, TT);
+    const int workers = size * SPLIT_WARPS, worker = rank * SPLIT_WARPS + warp;
+    const int first = span.tiles * worker / workers, last = span.tiles * (worker + 1) / workers;
+    if (first < last) {
+        Stream<T, DP, NT, PART, SMALL> st;
+        st.run(pv, q, c, span, b, h, q0, first, last, reinterpret_cast<uint4*>(so[warp]), status);
+        __syncwarp();
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const int col = 8 * n + 2 * t4 + x;
+                if (col >= cols) continue;
+                if (g == 0) sml[warp][col] = make_float2(st.m[n][x], st.l[n][x]);
+#pragma unroll
+                for (int vb = 0; vb < VB; vb++) {
+                    if (DP < 8 * CH && g * CH >= DP) continue;
+                    float v[CH];
+                    st.values(n, x, vb, 1.f, v);
+#pragma unroll
+                    for (int k = 0; k < CH; k += 4)
+                        so[warp][col][((g + 8 * vb) * CH + k) / 4] = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                }
+            }
+    } else if (lane < QT) {
+        sml[warp][lane] = make_float2(-INFINITY, 0.f);
+    }
+    __syncthreads();
+    // pieces (maximum and sum ml(i), values o(i)) added up; those that saw nothing are not read
+    auto add_up = [](int n, auto ml, auto o, float4& acc) {
+        float m = -INFINITY, l = 0.f;
+        acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = 0; i < n; i++) m = fmaxf(m, ml(i).x);
+        const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll 8
+        for (int i = 0; i < n; i++) {
+            const float2 p = ml(i);
+            if (p.x == -INFINITY && p.y == 0.f) continue;
+            const float e = ex2(p.x - base);
+            const float4 v = o(i);
+            l = fmaf(p.y, e, l);
+            acc.x = fmaf(v.x, e, acc.x);
+            acc.y = fmaf(v.y, e, acc.y);
+            acc.z = fmaf(v.z, e, acc.z);
+            acc.w = fmaf(v.w, e, acc.w);
+        }
+        return make_float2(m, l);
+    };
+    float4 acc;
+    for (int e = threadIdx.x; e < cols * FOURS; e += SPLIT_THREADS) {
+        const int col = e / FOURS, f = e % FOURS;
+        const float2 ml = add_up(SPLIT_WARPS, [&](int w) { return sml[w][col]; }, [&](int w) { return so[w][col][f]; }, acc);
+        so[0][col][f] = acc;
+        if (f == 0) joined[col] = ml;
+    }
+    cluster_sync();
+    for (int e = rank * SPLIT_THREADS + threadIdx.x; e < cols * FOURS; e += size * SPLIT_THREADS) {
+        const int col = e / FOURS, f = e % FOURS;
+        const float2 ml = add_up((int)size, [&](int r) { return of_block(&joined[col], r); },
+                                 [&](int r) { return of_block(&so[0][col][f], r); }, acc);
+        const int64_t head = (int64_t)b * pv.hq + h * group + q0 + col;
+        const float inv = ml.y == 0.f ? 0.f : 1.f / ml.y;
+        if (4 * f < pv.d) {
+            T* dst = out + head * pv.d + 4 * f;
+            dst[0] = narrow<T>(acc.x * inv);
+            dst[1] = narrow<T>(acc.y * inv);
+            dst[2] = narrow<T>(acc.z * inv);
+            dst[3] = narrow<T>(acc.w * inv);
+        }
+        if (lse && f == 0) lse[head] = ml.y == 0.f ? -INFINITY : (ml.x + log2f(ml.y)) * 0.69314718055994530942f;
+    }
+    cluster_sync();  // no block leaves while another reads its memory
+}
+
 // For each 32 columns of each (sequence, query head): the pieces of an item that was cut, each scaled to the largest
 // maximum, in an order that only the lengths decide (the same sums on every run); rows that see nothing become 0.
 // Eight lanes take a piece's 128 bytes, four pieces a warp go at a time and every lane has eight of them in flight:
@@ -1031,10 +1141,45 @@ static void split_work(W& ws, SplitWork& wk, int64_t batch, int64_t hq, int64_t 
     take(wk.o, slots * wk.rows * dp);
 }
 
+// The blocks per item of paged_cluster_kernel, 0: the list and the join. A cluster is faster while its warps have up to
+// four tiles each and all clusters run at once (blocks alone, without a partner, up to twice as many). Measured, list
+// and join against clusters: 6 heads x 64, 1 x 64 tokens 6.3 -> 3.5 us, 1 x 1024 7.1 -> 4.9, 16 x 256 7.2 -> 5.3; 32 / 8
+// heads x 128, 4 x 2048 15.5 -> 12.0 (four tiles a warp); with eight tiles a warp 15.4 -> 16.3 (16 x 2304), with twice
+// the clusters that fit 22.7 -> 38.9 (64 x 1024). Sixteen blocks find room slowly where several share an SM (fp32,
+// 4 x 2048: 11.7 -> 17.5), so they are for calls of at most a block per SM (1 x 2304: 7.3 -> 6.8).
+static int64_t cluster_size(const PageView& pv, int qt, int tt, int64_t resident, int64_t window, int64_t sinks) {
+    int64_t most = (int64_t)pv.max_blocks << pv.page_shift;  // tokens that any sequence can see
+    if (window) most = std::min(most, window + sinks + 2 * tt);
+    const int64_t tiles = (most + tt - 1) / tt, items = (int64_t)pv.batch * pv.hkv * ((pv.hq / pv.hkv + qt - 1) / qt);
+    int64_t size = 1;
+    while (size < 16 && size * SPLIT_WARPS < tiles) size *= 2;
+    if (size == 16 && (items * size > sm_count() || tiles > size * SPLIT_WARPS * 2)) size = 8;
+    while (size > 1 && items * size > resident) size /= 2;
+    if (size == 1 && tiles <= SPLIT_WARPS) return items <= 2 * resident;
+    return items * size <= resident && tiles <= size * SPLIT_WARPS * 4 ? size : 0;
+}
+
 template <typename T, int DP, int NT, bool PART, bool SMALL>
 static int launch_split(const PageView& pv, const void* q, float scale, int window, int sinks, void* out, float* lse,
                         const SplitWork& wk, int* status, cudaStream_t st) {
     using S = SplitShape<T, DP, NT>;
+    const int64_t size = cluster_size(pv, S::QT, S::TT, (int64_t)sm_count() * S::BLOCKS, window, sinks);
+    if (size) {
+        const auto kernel = paged_cluster_kernel<T, DP, NT, PART, SMALL>;
+        if (size > 8) {  // more than the portable eight, allowed once per device
+            static std::atomic<uint64_t> allowed{0};
+            int dev = 0;
+            SMLM_CUDA(cudaGetDevice(&dev));
+            if (dev >= 64 || !(allowed.load() >> dev & 1)) {
+                SMLM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+                if (dev < 64) allowed.fetch_or(uint64_t(1) << dev);
+            }
+        }
+        const int64_t items = (int64_t)pv.batch * pv.hkv * ((pv.hq / pv.hkv + S::QT - 1) / S::QT);
+        return launch_dependent(kernel, "paged_attention", (int)size, size * items, SPLIT_THREADS, st, pv,
+                                static_cast<const T*>(q), scale * 1.4426950408889634074f, window, sinks,
+                                static_cast<T*>(out), lse, status);
+    }
     const int blocks = sm_count() * S::BLOCKS;
     int rc = launch_dependent(paged_split_kernel<T, DP, NT, PART, SMALL>, "paged_attention", 1, blocks, SPLIT_THREADS, st, pv,
                               static_cast<const T*>(q), scale * 1.4426950408889634074f, window, sinks,

@@ -100,10 +100,8 @@ struct Team {
         asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
     }
     __device__ __forceinline__ void sync() const {
-        if (size > 1)
-            asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-        else
-            __syncthreads();
+        if (size > 1) cluster_sync();
+        else __syncthreads();
     }
     __device__ __forceinline__ int thread() const { return rank * PLAN_THREADS + threadIdx.x; }
     __device__ __forceinline__ int threads() const { return size * PLAN_THREADS; }
