@@ -1141,48 +1141,74 @@ static void split_work(W& ws, SplitWork& wk, int64_t batch, int64_t hq, int64_t 
     take(wk.o, slots * wk.rows * dp);
 }
 
-// The blocks per item of paged_cluster_kernel, 0: the list and the join. A cluster is faster while its warps have up to
-// four tiles each and all clusters run at once (blocks alone, without a partner, up to twice as many). Measured, list
-// and join against clusters: 6 heads x 64, 1 x 64 tokens 6.3 -> 3.5 us, 1 x 1024 7.1 -> 4.9, 16 x 256 7.2 -> 5.3; 32 / 8
-// heads x 128, 4 x 2048 15.5 -> 12.0 (four tiles a warp); with eight tiles a warp 15.4 -> 16.3 (16 x 2304), with twice
-// the clusters that fit 22.7 -> 38.9 (64 x 1024). Sixteen blocks find room slowly where several share an SM (fp32,
-// 4 x 2048: 11.7 -> 17.5), so they are for calls of at most a block per SM (1 x 2304: 7.3 -> 6.8).
-static int64_t cluster_size(const PageView& pv, int qt, int tt, int64_t resident, int64_t window, int64_t sinks) {
+// How many clusters of `size` blocks of the kernel run at once on this card (asked once per kernel and size): fewer than
+// the blocks that fit, because a cluster lies in one part of the card.
+template <auto kernel>
+static int64_t clusters_at_once(int size) {
+    static std::atomic<int> known[17];  // the answer + 1
+    int n = known[size].load();
+    if (n) return n - 1;
+    if (size > 8 && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(size);
+    cfg.blockDim = dim3(SPLIT_THREADS);
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = size;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    known[size].store(n + 1);
+    return n;
+}
+
+// The blocks per item of paged_cluster_kernel, 0: the list and the join. A cluster is faster while its warps have a few
+// tiles each and all clusters run at once. Measured, list and join -> clusters:
+//   6 heads x 64: 1 x 64 tokens 6.3 -> 3.5 us, 1 x 1024 7.1 -> 4.9, 16 x 256 7.2 -> 5.3;
+//   32 / 8 heads x 128: 4 x 2048 15.5 -> 12.0 (eight blocks, four tiles a warp), 16 x 512 13.0 -> 10.4 (three, 2.7);
+//   in fives with 3.6 tiles 15.4 -> 15.2 for even sequences and 8.9 -> 10.6 for uneven ones (16 x up to 2304, 6 x 64):
+//   the list evens out what the table could hold and the sequences do not;
+//   more clusters than run at once 15.4 -> 22.5 (16 x 2304 in sixes).
+// Up to six tiles a warp with a window, under which long sequences do the same work (64 x 1028 seen: 20.3 -> 17.3).
+// Sixteen blocks find room slowly where several share an SM (fp32, 4 x 2048: 11.7 -> 17.5), so they are for calls of at
+// most a block per SM (1 x 2304: 7.3 -> 6.8).
+template <auto kernel>
+static int cluster_size(const PageView& pv, int qt, int tt, int64_t window, int64_t sinks) {
     int64_t most = (int64_t)pv.max_blocks << pv.page_shift;  // tokens that any sequence can see
     if (window) most = std::min(most, window + sinks + 2 * tt);
     const int64_t tiles = (most + tt - 1) / tt, items = (int64_t)pv.batch * pv.hkv * ((pv.hq / pv.hkv + qt - 1) / qt);
-    int64_t size = 1;
-    while (size < 16 && size * SPLIT_WARPS < tiles) size *= 2;
-    if (size == 16 && (items * size > sm_count() || tiles > size * SPLIT_WARPS * 2)) size = 8;
-    while (size > 1 && items * size > resident) size /= 2;
-    if (size == 1 && tiles <= SPLIT_WARPS) return items <= 2 * resident;
-    return items * size <= resident && tiles <= size * SPLIT_WARPS * 4 ? size : 0;
+    if (tiles <= SPLIT_WARPS) return items <= 2 * clusters_at_once<kernel>(1);  // blocks alone: two rounds are as fast
+    if (tiles > 8 * SPLIT_WARPS && tiles <= 16 * SPLIT_WARPS * 2 && items * 16 <= sm_count() &&
+        items <= clusters_at_once<kernel>(16))
+        return 16;
+    for (int size = (int)std::min<int64_t>(8, (tiles + SPLIT_WARPS - 1) / SPLIT_WARPS); size >= 1; size--) {
+        if (tiles > size * SPLIT_WARPS * (window ? 6 : size == 8 ? 4 : 3)) break;
+        if (items <= clusters_at_once<kernel>(size)) return size;
+    }
+    return 0;
 }
 
 template <typename T, int DP, int NT, bool PART, bool SMALL>
 static int launch_split(const PageView& pv, const void* q, float scale, int window, int sinks, void* out, float* lse,
                         const SplitWork& wk, int* status, cudaStream_t st) {
     using S = SplitShape<T, DP, NT>;
-    const int64_t size = cluster_size(pv, S::QT, S::TT, (int64_t)sm_count() * S::BLOCKS, window, sinks);
-    if (size) {
-        const auto kernel = paged_cluster_kernel<T, DP, NT, PART, SMALL>;
-        if (size > 8) {  // more than the portable eight, allowed once per device
-            static std::atomic<uint64_t> allowed{0};
-            int dev = 0;
-            SMLM_CUDA(cudaGetDevice(&dev));
-            if (dev >= 64 || !(allowed.load() >> dev & 1)) {
-                SMLM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-                if (dev < 64) allowed.fetch_or(uint64_t(1) << dev);
-            }
-        }
+    constexpr auto clustered = paged_cluster_kernel<T, DP, NT, PART, SMALL>;
+    if (const int size = cluster_size<clustered>(pv, S::QT, S::TT, window, sinks)) {
         const int64_t items = (int64_t)pv.batch * pv.hkv * ((pv.hq / pv.hkv + S::QT - 1) / S::QT);
-        return launch_dependent(kernel, "paged_attention", (int)size, size * items, SPLIT_THREADS, st, pv,
+        return launch_dependent(clustered, "paged_attention", size, size * items, SPLIT_THREADS, st, pv,
                                 static_cast<const T*>(q), scale * 1.4426950408889634074f, window, sinks,
                                 static_cast<T*>(out), lse, status);
     }
     const int blocks = sm_count() * S::BLOCKS;
-    int rc = launch_dependent(paged_split_kernel<T, DP, NT, PART, SMALL>, "paged_attention", 1, blocks, SPLIT_THREADS, st, pv,
-                              static_cast<const T*>(q), scale * 1.4426950408889634074f, window, sinks,
+    int rc = launch_dependent(paged_split_kernel<T, DP, NT, PART, SMALL>, "paged_attention", 1, blocks, SPLIT_THREADS, st,
+                              pv, static_cast<const T*>(q), scale * 1.4426950408889634074f, window, sinks,
                               static_cast<T*>(out), lse, wk, status);
     if (rc != SMLM_OK) return rc;
     const int columns = (pv.d + 31) / 32;
