@@ -51,7 +51,7 @@ def test_append_and_page_refusals():
                                      positions, P, None, None)
     for args, text in [({"cos": None}, b"together"), ({"positions": 0}, b"together"), ({"tokens": -1}, b"tokens"),
                        ({"qkv": ctypes.c_void_p(0x1004)}, b"aligned"), ({"cos": ctypes.c_void_p(0x1004)}, b"aligned"),
-                       ({"hq": 4096, "d": 256}, b"MiB")]:
+                       ({"hq": 4096, "d": 256}, b"2^20")]:
         assert append(**args) == L.ERR_INVALID and text in lib.smlm_last_error(), args
     assert append(tokens=0) == L.OK
     assert lib.smlm_pages_free(None, 4, 4, 4, P, P, 8, P, 2, None, None) == L.ERR_INVALID
