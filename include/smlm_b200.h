@@ -492,7 +492,9 @@ SMLM_API size_t smlm_paged_attention_workspace(int64_t batch, int64_t hq, int64_
  * j >= lengths[b] - window or j < sinks. out = sum_j p_j v_j with p the softmax over the visible tokens of
  * scale * <q, k_j> (scores, sums and the output's sum in fp32); a row with no visible token (or only scores of
  * -inf) gives 0. lse: NULL, or fp32 (batch, hq) for the logarithm of the softmax's sum (-inf for such a row).
- * Nothing of a token that is not visible enters, whatever its bits. */
+ * Nothing of a token that is not visible enters, whatever its bits. (An infinite value of a visible token makes its
+ * column infinite or NaN.) At most 65535 sequences; page and token strides below 4 GiB. Every cut and every sum follows
+ * from the arguments and lengths alone, so a call's result is the same on every run. */
 SMLM_API int smlm_paged_attention(const void *q, const void *k_pages, const void *v_pages, int dtype,
                                   const int64_t *strides, const int32_t *table, int64_t table_stride,
                                   const int32_t *lengths, int64_t batch, int64_t hq, int64_t hkv, int64_t d,
@@ -505,7 +507,8 @@ SMLM_API int smlm_paged_attention(const void *q, const void *k_pages, const void
  * the half-split rotary embedding with cos / sin (fp32, max_pos x d / 2; both NULL: not turned), computed in fp32 and
  * rounded once; keys and values go to their pages, queries to q_out (batch, tokens, hq, d). A negative position is
  * padding before a shorter chunk: its queries are 0 and it is not stored. A token whose page is missing sets
- * SMLM_FLAG_NO_PAGES, a position beyond max_pos SMLM_FLAG_INDEX_RANGE; both are skipped. */
+ * SMLM_FLAG_NO_PAGES and is not stored; a position beyond max_pos sets SMLM_FLAG_INDEX_RANGE, is not stored and has
+ * queries of 0. */
 SMLM_API int smlm_paged_append(const void *qkv, void *k_pages, void *v_pages, int dtype, const int64_t *strides,
                                const int32_t *table, int64_t table_stride, const int32_t *lengths, int64_t batch,
                                int64_t tokens, int64_t hq, int64_t hkv, int64_t d, int64_t n_pages, int64_t page_size,

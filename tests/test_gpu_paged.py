@@ -62,6 +62,46 @@ def test_attention_head_layouts_and_types(dtype, hq, hkv, d, page):
     check(*make([1, 37, 0, 300, page, page + 1], hq, hkv, d, page, dtype, seed=hq + d))
 
 
+def roomy(table, page):
+    """The table with room for sequences of 100000 tokens: how the work is cut follows from what the table could hold
+    (one cluster per item while that is little, a list over the whole card else)."""
+    out = torch.full((table.shape[0], 100000 // page), -1, dtype=torch.int32, device=DEV)
+    out[:, :table.shape[1]] = table
+    return out
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("hq,hkv,d,page", [(6, 6, 64, 16), (8, 1, 128, 32), (32, 8, 128, 16), (4, 4, 16, 8),
+                                           (7, 7, 80, 64), (20, 2, 96, 128), (6, 3, 256, 16), (3, 1, 48, 1),
+                                           (17, 1, 32, 4), (40, 2, 64, 256)])
+def test_attention_in_tables_with_room(dtype, hq, hkv, d, page):
+    q, k, v, table, lengths = make([1, 37, 0, 300, 0, page, 700], hq, hkv, d, page, dtype, seed=hq + d)
+    check(q, k, v, roomy(table, page), lengths)
+    check(q, k, v, roomy(table, page), lengths, window=50, sinks=5)
+
+
+@pytest.mark.parametrize("batch", [1, 2, 31, 33, 128, 129, 500])
+def test_attention_batches_in_tables_with_room(batch):
+    """The list's cut for batches of less and more rows than a warp has lanes and a block has threads; empty rows among
+    them, alone and last."""
+    r = random.Random(batch)
+    lens = [r.choice([0, 0, 1, 16, 33, 90, 400]) for _ in range(batch)]
+    lens[-1] = 0 if batch > 1 else 5
+    q, k, v, table, lengths = make(lens, 4, 2, 32, 16, BF16, seed=batch)
+    check(q, k, v, roomy(table, 16), lengths)
+    lengths.zero_()
+    out = paged.paged_attention(q, k, v, roomy(table, 16), lengths)
+    assert not bool(out.any())
+
+
+@pytest.mark.parametrize("room", [False, True])
+@pytest.mark.parametrize("n", [300, 1100, 2300])
+def test_attention_clusters_of_every_size(n, room):
+    for batch in (1, 3, 9, 24, 40):
+        q, k, v, table, lengths = make([n - 7 * i for i in range(batch)], 6, 6, 64, 16, BF16, seed=n + batch)
+        check(q, k, v, roomy(table, 16) if room else table, lengths)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("n", [1, 2, 7, 8, 9, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 129, 1000, 5003])
 def test_attention_every_small_length_and_long_ones(dtype, n):
