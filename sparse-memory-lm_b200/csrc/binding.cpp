@@ -4,6 +4,9 @@
 // Python checks, of which 6 are the two launches).
 #include <Python.h>
 
+#include <cmath>
+#include <cstdlib>
+
 #include <ATen/Context.h>
 #include <ATen/ops/empty.h>
 #include <c10/cuda/CUDACachingAllocator.h>
@@ -366,8 +369,15 @@ PyObject* init(PyObject*, PyObject* f) {
     Py_RETURN_NONE;
 }
 
+// Whether SMLM_B200_CHECK=1 is set now (os.environ.get costs ten times as much as this call).
+PyObject* checking(PyObject*, PyObject*) {
+    const char* v = std::getenv("SMLM_B200_CHECK");
+    return PyBool_FromLong(v && v[0] == '1' && !v[1]);
+}
+
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {{"init", init, METH_O, nullptr},
+                         {"checking", checking, METH_NOARGS, nullptr},
                          FAST(attention),
                          FAST(append),
                          FAST(pages_free),

@@ -221,7 +221,7 @@ class timed:
 
 
 def checked():
-    return os.environb.get(b"SMLM_B200_CHECK") == b"1"
+    return os.environ.get("SMLM_B200_CHECK", "0") == "1"
 
 
 def status_ptr(device):
@@ -251,11 +251,6 @@ def status_int(device):
     """The status word's address as an integer (None: no word)."""
     p = status_ptr(device)
     return p.value if p is not None else None
-
-
-def instrumented():
-    """Whether calls are timed, ranged or checked (timed / after do something)."""
-    return PROFILE is not None or NVTX or checked()
 
 
 def after(device, what):

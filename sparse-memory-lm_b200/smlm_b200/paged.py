@@ -46,9 +46,16 @@ def _load():
 _native = _load()
 
 
+_checking = _native.checking
+
+
+def _instrumented():
+    """Whether calls are timed, ranged or checked."""
+    return L.PROFILE is not None or L.NVTX or _checking()
+
+
 def _call(name, launches, device, fn, *args):
-    if not L.instrumented():
-        return fn(*args)
+    """A call that is timed, ranged or checked."""
     with L.timed(name, launches):
         out = fn(*args)
     L.after(device, name)
@@ -64,8 +71,10 @@ def paged_attention(q, k_pages, v_pages, table, lengths, *, scale=None, window=0
     entry is not -1; with window > 0 only the last `window` tokens and the first `sinks` are. scale defaults to
     d ** -0.5. A row that sees nothing gives 0. return_lse: also the logarithm of the softmax's sum, fp32 (B, query
     heads), -inf for such a row."""
-    return _call("paged_attention", 2, q.device, _native.attention, q, k_pages, v_pages, table, lengths, scale, window,
-                 sinks, return_lse)
+    if not _instrumented():
+        return _native.attention(q, k_pages, v_pages, table, lengths, scale, window, sinks, return_lse)
+    return _call("paged_attention", 2, q.device, _native.attention, q, k_pages, v_pages, table, lengths, scale,
+                 window, sinks, return_lse)
 
 
 def paged_append(qkv, k_pages, v_pages, table, lengths, cos=None, sin=None):
@@ -74,38 +83,52 @@ def paged_append(qkv, k_pages, v_pages, table, lengths, cos=None, sin=None):
     before a shorter chunk and is not stored), queries are returned, (B, T, query heads, d). With cos / sin (fp32,
     (positions, d / 2)) queries and keys are turned by the half-split rotary embedding of their position, in fp32,
     rounded once."""
+    if not _instrumented():
+        return _native.append(qkv, k_pages, v_pages, table, lengths, cos, sin)
     return _call("paged_append", 1, qkv.device, _native.append, qkv, k_pages, v_pages, table, lengths, cos, sin)
 
 
 # --------------------------------------------------------------------------------------------- the pages
 def pages_free(table, lengths, refcount, rows):
     """The sequences `rows` (int32) end: their pages are released, their table entries become -1, their lengths 0."""
-    _call("pages_free", 1, table.device, _native.pages_free, table, lengths, refcount, rows)
+    if not _instrumented():
+        return _native.pages_free(table, lengths, refcount, rows)
+    return _call("pages_free", 1, table.device, _native.pages_free, table, lengths, refcount, rows)
 
 
 def pages_trim(table, lengths, refcount, rows, page_size, window, sinks=0):
     """Releases the pages of the sequences `rows` that paged_attention with this window and these sinks no longer reads:
     those that hold only tokens in [sinks, length - window)."""
-    _call("pages_trim", 1, table.device, _native.pages_trim, table, lengths, refcount, rows, page_size, window, sinks)
+    if not _instrumented():
+        return _native.pages_trim(table, lengths, refcount, rows, page_size, window, sinks)
+    return _call("pages_trim", 1, table.device, _native.pages_trim, table, lengths, refcount, rows, page_size,
+                 window, sinks)
 
 
 def pages_extend(table, lengths, refcount, rows, n_new, page_size):
     """Every sequence in `rows` grows by n_new tokens: lengths[r] += n_new, with the lowest free pages (row by row) where
     its last page is full. A sequence that finds too few keeps its length."""
-    _call("pages_extend", 1, table.device, _native.pages_extend, table, lengths, refcount, rows, n_new, page_size)
+    if not _instrumented():
+        return _native.pages_extend(table, lengths, refcount, rows, n_new, page_size)
+    return _call("pages_extend", 1, table.device, _native.pages_extend, table, lengths, refcount, rows, n_new,
+                 page_size)
 
 
 def pages_fork(pool, table, lengths, refcount, parents, children):
     """Sequence children[i] becomes a copy of sequence parents[i] as it was before the call, for all i at once (a row may
     be a parent and a child: a beam's reordering); what the children held is released. Whole pages are shared, the
     tokens of a partly filled last page are copied in all layers. pool: (layers, 2, pages, key heads, page_size, d)."""
-    _call("pages_fork", 2, table.device, _native.pages_fork, table, lengths, refcount, pool, parents, children)
+    if not _instrumented():
+        return _native.pages_fork(table, lengths, refcount, pool, parents, children)
+    return _call("pages_fork", 2, table.device, _native.pages_fork, table, lengths, refcount, pool, parents, children)
 
 
 def pages_compact(pool, table, refcount):
     """Moves the pages in use to the lowest numbers, in the pool, the table and the counts: with n in use, the k-th used
     page numbered n or above goes to the k-th free page below n."""
-    _call("pages_compact", 2, table.device, _native.pages_compact, table, refcount, pool)
+    if not _instrumented():
+        return _native.pages_compact(table, refcount, pool)
+    return _call("pages_compact", 2, table.device, _native.pages_compact, table, refcount, pool)
 
 
 # ----------------------------------------------------------------------------------------------- the cache
