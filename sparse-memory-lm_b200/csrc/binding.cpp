@@ -1,7 +1,7 @@
 // Python functions over the paged cache's C entry points, for tensors of torch: argument checks, outputs, scratch from
 // torch's caching allocator, the current stream. A decoding step makes two of these calls per layer, and each is a few
-// microseconds of device time, so what the host spends on one counts (attention of one token: 20 us through ctypes and
-// Python checks, of which 6 are the two launches).
+// microseconds of device time, so what the host spends on one counts: attention of one token took 17.6 us through ctypes
+// and checks in Python and takes 5 through this (one launch; 7 with two).
 #include <Python.h>
 
 #include <cmath>
