@@ -129,22 +129,79 @@ __device__ __forceinline__ int team_scan(const Team& team, int v, int32_t* total
     return before + x;
 }
 
-// The free pages in increasing order: list[k] = the k-th free page, for k < most. Returns how many there are. Each
-// thread counts a contiguous piece, one scan gives its first rank. Ends with a barrier.
-__device__ int list_free(const Team& team, const Pages& pg, int32_t* list, int most, int32_t* totals) {
-    const int per = (pg.n_pages + team.threads() - 1) / team.threads();
-    const int a = min(pg.n_pages, team.thread() * per), e = min(pg.n_pages, a + per);
-    uint32_t bits = 0;  // the first 32 of the piece, not to read them twice
-    int count = 0, total;
-    for (int p = a; p < e; p++)
-        if (__ldcg(pg.refcount + p) == 0) {
-            count++;
-            if (p - a < 32) bits |= 1u << (p - a);
+// A warp's contiguous piece of the pages, 32 at a time: which of them are in use. The first 32 words stay in registers
+// (lane i has word i), so up to 32768 pages a block are read once. (A thread with pages of its own, one after the other:
+// compacting 100000 pages 24 us instead of 13, 10^6 pages 266 instead of 85.)
+struct Piece {
+    const int32_t* refcount;
+    int n_pages, first, words;  // words of 32 pages from word `first` on
+    uint32_t kept = 0;
+    __device__ __forceinline__ Piece(const Team& team, const Pages& pg) : refcount(pg.refcount), n_pages(pg.n_pages) {
+        const int all = (n_pages + 31) / 32, warps = team.threads() / 32, each = (all + warps - 1) / warps;
+        first = min(all, team.thread() / 32 * each);
+        words = min(all - first, each);
+    }
+    // f(first page of the word, its bits) for every word, several loads in flight; pages past the end are not in use
+    template <typename F>
+    __device__ __forceinline__ void read(F f) {
+        constexpr int U = 4;
+        const int lane = lane_id();
+#pragma unroll 1
+        for (int w0 = 0; w0 < words; w0 += U) {
+            int v[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int p = (first + w0 + u) * 32 + lane;
+                v[u] = w0 + u < words && p < n_pages ? __ldcg(refcount + p) : 0;
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (w0 + u >= words) break;
+                const uint32_t used = __ballot_sync(FULL, v[u] > 0);
+                if (w0 + u == lane) kept = used;
+                f((first + w0 + u) * 32, used);
+            }
         }
-    int k = team_scan(team, count, totals, &total);
-    for (; bits && k < most; bits &= bits - 1) list[k++] = a + __ffs(bits) - 1;
-    for (int p = a + 32; p < e && k < most; p++)
-        if (__ldcg(pg.refcount + p) == 0) list[k++] = p;
+    }
+    // the same again, the first 32 words from the registers
+    template <typename F>
+    __device__ __forceinline__ void again(F f) {
+        const int lane = lane_id();
+#pragma unroll 1
+        for (int w = 0; w < words; w++) {
+            const int p = (first + w) * 32;
+            uint32_t used = __shfl_sync(FULL, kept, w & 31);
+            if (w >= 32) used = __ballot_sync(FULL, p + lane < n_pages && __ldcg(refcount + p + lane) > 0);
+            f(p, used);
+        }
+    }
+    // the bits of pages below n in the word that begins at page p
+    static __device__ __forceinline__ uint32_t below(int p, int n) {
+        return p + 32 <= n ? FULL : p >= n ? 0u : (1u << (n - p)) - 1;
+    }
+};
+
+// The sum of one value per warp (the same in its lanes) over the warps before this one; *total: of all.
+__device__ __forceinline__ int team_scan_warps(const Team& team, int v, int32_t* totals, int* total) {
+    return __shfl_sync(FULL, team_scan(team, lane_id() == 0 ? v : 0, totals, total), 0);
+}
+
+// The free pages in increasing order: list[k] = the k-th free page, for k < most. Returns how many there are. Ends with
+// a barrier.
+__device__ int list_free(const Team& team, const Pages& pg, int32_t* list, int most, int32_t* totals) {
+    Piece piece(team, pg);
+    const int lane = lane_id();
+    const uint32_t lower = (1u << lane) - 1;
+    int count = 0, total;
+    piece.read([&](int p, uint32_t used) { count += __popc(~used & Piece::below(p, pg.n_pages)); });
+    int rank = team_scan_warps(team, count, totals, &total);
+    if (rank < most)
+        piece.again([&](int p, uint32_t used) {
+            const uint32_t free = ~used & Piece::below(p, pg.n_pages);
+            const int k = rank + __popc(free & lower);
+            if (free >> lane & 1 && k < most) list[k] = p + lane;
+            rank += __popc(free);
+        });
     team.sync();
     return total;
 }
@@ -314,33 +371,33 @@ __global__ void __launch_bounds__(PLAN_THREADS)
 }
 
 // With L pages in use: the k-th used page numbered L or above moves to the k-th free page below L. to[p] (p >= L) is
-// where page p went. Each thread has a contiguous piece of the pages; two scans give L and the ranks. 6480 pages: 7 us,
-// three dependent reads of the counts and the barriers between them.
+// where page p went. Two scans give L and the ranks. 6480 pages: 7 us, a chain of reads and barriers.
 __global__ void __launch_bounds__(PLAN_THREADS) pages_compact_kernel(Pages pg, int32_t* to, int32_t* live_out,
                                                                      int32_t* totals, CopyList cl) {
     grid_wait();
     grid_release();
     const Team team;
-    const int per = (pg.n_pages + team.threads() - 1) / team.threads();
-    const int a = min(pg.n_pages, team.thread() * per), e = min(pg.n_pages, a + per);
+    Piece piece(team, pg);
+    const int lane = lane_id();
+    const uint32_t lower = (1u << lane) - 1;
     int count = 0, live, below;
-    for (int p = a; p < e; p++) count += __ldcg(pg.refcount + p) > 0;
-    const int before = team_scan(team, count, totals, &live);
+    piece.read([&](int, uint32_t used) { count += __popc(used); });
+    int rank = team_scan_warps(team, count, totals, &live);  // used pages before the word
     count = 0;  // of them below L
-    for (int p = a; p < min(e, live); p++) count += __ldcg(pg.refcount + p) > 0;
-    team_scan(team, count, totals + MAX_TEAM, &below);
+    piece.again([&](int p, uint32_t used) { count += __popc(used & Piece::below(p, live)); });
+    team_scan_warps(team, count, totals + MAX_TEAM, &below);
     const int moves = live - below;
-    int used = before;
-    for (int p = a; p < e; p++) {
-        const bool u = __ldcg(pg.refcount + p) > 0;
-        if (p < live) {
-            if (!u) cl.dst[p - used] = p;
-        } else {
-            if (u) cl.src[used - below] = p;
-            else to[p] = p;
+    piece.again([&](int p, uint32_t used) {
+        const int page = p + lane, before = rank + __popc(used & lower);
+        const bool u = used >> lane & 1;
+        if (page < live) {
+            if (!u) cl.dst[page - before] = page;
+        } else if (page < pg.n_pages) {
+            if (u) cl.src[before - below] = page;
+            else to[page] = page;
         }
-        used += u;
-    }
+        rank += __popc(used);
+    });
     if (team.thread() == 0) {
         *cl.count = moves;
         *live_out = live;
