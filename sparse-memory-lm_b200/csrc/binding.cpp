@@ -122,9 +122,9 @@ Layer layer(const char* what, const at::Tensor& x, const at::Tensor& k, const at
     l.hkv = k.size(1);
     l.page = k.size(2);
     l.d = k.size(3);
-    for (int i = 0; i < 3; i++) {
-        l.strides[i] = k.stride(i);
-        l.strides[3 + i] = v.stride(i);
+    for (int i = 0; i < 3; i++) {  // a dimension of one element may have any stride: it is not used
+        l.strides[i] = k.size(i) > 1 ? k.stride(i) : 0;
+        l.strides[3 + i] = v.size(i) > 1 ? v.stride(i) : 0;
     }
     return l;
 }

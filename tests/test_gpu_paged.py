@@ -152,6 +152,20 @@ def test_attention_strides(order):
     check(full[:, ::2], wide[:, 1], other, broad[:, :table.shape[1]], lengths)
 
 
+def test_strides_of_dimensions_with_one_element_do_not_matter():
+    q, k, v, table, lengths = make([40, 7], 4, 1, 64, 16, BF16, seed=6)
+    odd = k.as_strided(k.shape, (k.stride(0), 7, k.stride(2), 1))
+    want = paged.paged_attention(q, k, v, table, lengths)
+    assert torch.equal(paged.paged_attention(q, odd, v, table, lengths), want)
+    one = table[:1].as_strided((1, table.shape[1]), (3, 1))
+    assert torch.equal(paged.paged_attention(q[:1], k, v, one, lengths[:1]),
+                       paged.paged_attention(q[:1], k, v, table[:1], lengths[:1]))
+    k1 = k[int(table[1, 0]):int(table[1, 0]) + 1]
+    v1 = v[int(table[1, 0]):int(table[1, 0]) + 1]
+    single = torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    check(q[1:], k1.as_strided(k1.shape, (5, 3, k1.stride(2), 1)), v1, single, lengths[1:])
+
+
 def test_attention_scores_of_infinity_and_large_scores():
     """Visible keys may give scores of -inf (weight 0); scores of thousands do not overflow."""
     q, k, v, table, lengths = make([40, 20], 2, 2, 64, 16, F32, seed=8)
