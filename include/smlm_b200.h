@@ -484,8 +484,9 @@ SMLM_API int smlm_ngram_rows(const int64_t *c, int64_t batch, int64_t t_len, int
  * F16, the same for the cache and the activations. Page numbers outside the pool and lengths outside the table set
  * SMLM_FLAG_INDEX_RANGE and are left out. */
 
-/* Scratch bytes of smlm_paged_attention. */
-SMLM_API size_t smlm_paged_attention_workspace(int64_t batch, int64_t hq, int64_t hkv, int64_t d, int dtype);
+/* Scratch bytes of smlm_paged_attention with these arguments on the current device; 0 where it needs none. */
+SMLM_API size_t smlm_paged_attention_workspace(int64_t batch, int64_t hq, int64_t hkv, int64_t d, int dtype,
+                                               int64_t page_size, int64_t max_blocks, int64_t window, int64_t sinks);
 
 /* Attention of one new token per sequence: q and out (batch, hq, d); query head i reads key head i / (hq / hkv).
  * Token j of sequence b is visible if j < lengths[b], its table entry is not -1, and, with window > 0, if

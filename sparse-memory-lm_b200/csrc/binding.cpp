@@ -8,7 +8,7 @@
 #include <cstdlib>
 
 #include <ATen/Context.h>
-#include <ATen/ops/empty.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -80,10 +80,16 @@ struct Call {
         stream = c10::cuda::getCurrentCUDAStream(t.device().index()).stream();
     }
     void* workspace(size_t bytes) {
-        scratch = c10::cuda::CUDACachingAllocator::get()->allocate(bytes ? bytes : 1);
+        if (!bytes) return nullptr;
+        scratch = c10::cuda::CUDACachingAllocator::get()->allocate(bytes);
         return scratch.get();
     }
 };
+
+// An uninitialised tensor beside `like`.
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
+    return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+}
 
 void checked(const char* what, int rc) {
     if (rc == SMLM_OK) return;
@@ -174,9 +180,10 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (!q.is_contiguous()) q = q.contiguous();
         const bool with_lse = PyObject_IsTrue(a[8]) == 1;
         Call c(q);
-        at::Tensor out = at::empty(q.sizes(), q.options());
-        at::Tensor lse = with_lse ? at::empty({batch, hq}, q.options().dtype(at::kFloat)) : at::Tensor();
-        const size_t bytes = smlm_paged_attention_workspace(batch, hq, l.hkv, l.d, l.code);
+        at::Tensor out = fresh(q.sizes(), q.scalar_type(), q);
+        at::Tensor lse = with_lse ? fresh({batch, hq}, at::kFloat, q) : at::Tensor();
+        const size_t bytes = smlm_paged_attention_workspace(batch, hq, l.hkv, l.d, l.code, l.page, table.size(1), window,
+                                                            sinks);
         checked(what, smlm_paged_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), l.code, l.strides,
                                            static_cast<const int32_t*>(table.data_ptr()), row_stride(table),
                                            static_cast<const int32_t*>(lengths.data_ptr()), batch, hq, l.hkv, l.d,
@@ -218,7 +225,7 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
         }
         if (!x.is_contiguous()) x = x.contiguous();
         Call c(x);
-        at::Tensor q = at::empty({batch, tokens, hq, l.d}, x.options());
+        at::Tensor q = fresh({batch, tokens, hq, l.d}, x.scalar_type(), x);
         checked(what, smlm_paged_append(x.data_ptr(), k.data_ptr(), v.data_ptr(), l.code, l.strides,
                                         static_cast<const int32_t*>(table.data_ptr()), row_stride(table),
                                         static_cast<const int32_t*>(lengths.data_ptr()), batch, tokens, hq, l.hkv, l.d,

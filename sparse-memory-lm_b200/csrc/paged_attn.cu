@@ -1190,62 +1190,102 @@ static int cluster_size(const PageView& pv, int qt, int tt, int64_t window, int6
     return 0;
 }
 
-template <typename T, int DP, int NT, bool PART, bool SMALL>
-static int launch_split(const PageView& pv, const void* q, float scale, int window, int sinks, void* out, float* lse,
-                        const SplitWork& wk, int* status, cudaStream_t st) {
-    using S = SplitShape<T, DP, NT>;
-    constexpr auto clustered = paged_cluster_kernel<T, DP, NT, PART, SMALL>;
-    if (const int size = cluster_size<clustered>(pv, S::QT, S::TT, window, sinks)) {
-        const int64_t items = (int64_t)pv.batch * pv.hkv * ((pv.hq / pv.hkv + S::QT - 1) / S::QT);
-        return launch_dependent(clustered, "paged_attention", size, size * items, SPLIT_THREADS, st, pv,
-                                static_cast<const T*>(q), scale * 1.4426950408889634074f, window, sinks,
-                                static_cast<T*>(out), lse, status);
-    }
+// The kernels' template arguments for a call.
+template <typename T_, int DP_, int NT_, bool PART_, bool SMALL_>
+struct Variant {
+    using T = T_;
+    using S = SplitShape<T_, DP_, NT_>;
+    static constexpr int DP = DP_, NT = NT_;
+    static constexpr auto cluster = paged_cluster_kernel<T_, DP_, NT_, PART_, SMALL_>;
+    static constexpr auto split = paged_split_kernel<T_, DP_, NT_, PART_, SMALL_>;
+};
+
+template <typename F>
+static int with_variant(const PageView& pv, int dtype, F f) {
+    return by_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        const auto of = [&](auto dp, auto nt) {
+            constexpr int DP = decltype(dp)::value, NT = decltype(nt)::value;
+            if (pv.page_shift < 4) return f(Variant<T, DP, NT, true, true>());
+            if (pv.d < DP) return f(Variant<T, DP, NT, true, false>());
+            return f(Variant<T, DP, NT, false, false>());
+        };
+        const auto go = [&](auto dp) {
+            if constexpr (sizeof(T) == 2 && decltype(dp)::value <= 128)
+                if (eights(pv.hq / pv.hkv, decltype(dp)::value, sizeof(T)) == 2)
+                    return of(dp, std::integral_constant<int, 2>());
+            return of(dp, std::integral_constant<int, 1>());
+        };
+        if (pv.d <= 32) return go(std::integral_constant<int, 32>());
+        if (pv.d <= 64) return go(std::integral_constant<int, 64>());
+        if (pv.d <= 128) return go(std::integral_constant<int, 128>());
+        return go(std::integral_constant<int, 256>());
+    });
+}
+
+struct AttentionArgs {
+    const void* q;
+    float scale;
+    int window, sinks;
+    void* out;
+    float* lse;
+    int* status;
+    cudaStream_t st;
+};
+
+template <typename V>
+static int launch_cluster(V, const PageView& pv, int size, const AttentionArgs& a) {
+    using T = typename V::T;
+    const int64_t items = (int64_t)pv.batch * pv.hkv * ((pv.hq / pv.hkv + V::S::QT - 1) / V::S::QT);
+    return launch_dependent(V::cluster, "paged_attention", size, size * items, SPLIT_THREADS, a.st, pv,
+                            static_cast<const T*>(a.q), a.scale * 1.4426950408889634074f, a.window, a.sinks,
+                            static_cast<T*>(a.out), a.lse, a.status);
+}
+
+template <typename V>
+static int launch_list(V, const PageView& pv, const SplitWork& wk, const AttentionArgs& a) {
+    using T = typename V::T;
+    using S = typename V::S;
     const int blocks = sm_count() * S::BLOCKS;
-    int rc = launch_dependent(paged_split_kernel<T, DP, NT, PART, SMALL>, "paged_attention", 1, blocks, SPLIT_THREADS, st,
-                              pv, static_cast<const T*>(q), scale * 1.4426950408889634074f, window, sinks,
-                              static_cast<T*>(out), lse, wk, status);
+    const int rc = launch_dependent(V::split, "paged_attention", 1, blocks, SPLIT_THREADS, a.st, pv,
+                                    static_cast<const T*>(a.q), a.scale * 1.4426950408889634074f, a.window, a.sinks,
+                                    static_cast<T*>(a.out), a.lse, wk, a.status);
     if (rc != SMLM_OK) return rc;
     const int columns = (pv.d + 31) / 32;
     const int64_t units = (int64_t)pv.batch * pv.hq * columns;
     const int64_t items = (int64_t)pv.batch * pv.hkv * ((pv.hq / pv.hkv + S::QT - 1) / S::QT);
     const bool shared = (int64_t)blocks * SPLIT_WARPS > 32 * items;  // over 32 pieces an item: a block for each
     return launch_dependent(shared ? paged_join_kernel<T, S::TT, S::QT, 8> : paged_join_kernel<T, S::TT, S::QT, 1>,
-                            "paged_attention: join", 1, shared ? units : (units + 7) / 8, JOIN_THREADS, st, pv, window, sinks,
-                            columns, static_cast<T*>(out), lse, wk);
+                            "paged_attention: join", 1, shared ? units : (units + 7) / 8, JOIN_THREADS, a.st, pv,
+                            a.window, a.sinks, columns, static_cast<T*>(a.out), a.lse, wk);
 }
 
-template <typename T>
-static int launch_attention(const PageView& pv, const void* q, float scale, int window, int sinks, void* out,
-                            float* lse, const SplitWork& wk, int* status, cudaStream_t st) {
-    const auto of = [&](auto dp, auto nt) {
-        constexpr int DP = decltype(dp)::value, NT = decltype(nt)::value;
-        if (pv.page_shift < 4)
-            return launch_split<T, DP, NT, true, true>(pv, q, scale, window, sinks, out, lse, wk, status, st);
-        if (pv.d < DP)
-            return launch_split<T, DP, NT, true, false>(pv, q, scale, window, sinks, out, lse, wk, status, st);
-        return launch_split<T, DP, NT, false, false>(pv, q, scale, window, sinks, out, lse, wk, status, st);
-    };
-    const auto go = [&](auto dp) {
-        if constexpr (sizeof(T) == 2 && decltype(dp)::value <= 128)
-            if (eights(pv.hq / pv.hkv, decltype(dp)::value, sizeof(T)) == 2)
-                return of(dp, std::integral_constant<int, 2>());
-        return of(dp, std::integral_constant<int, 1>());
-    };
-    if (pv.d <= 32) return go(std::integral_constant<int, 32>());
-    if (pv.d <= 64) return go(std::integral_constant<int, 64>());
-    if (pv.d <= 128) return go(std::integral_constant<int, 128>());
-    return go(std::integral_constant<int, 256>());
-}
+static int clamp_window(int64_t window) { return (int)std::min<int64_t>(window, INT32_MAX); }
+static int clamp_sinks(int64_t sinks) { return (int)std::min<int64_t>(sinks, INT32_MAX / 2); }
 
 }  // namespace smlm
 
 using namespace smlm;
 
-extern "C" size_t smlm_paged_attention_workspace(int64_t batch, int64_t hq, int64_t hkv, int64_t d, int dtype) {
+extern "C" size_t smlm_paged_attention_workspace(int64_t batch, int64_t hq, int64_t hkv, int64_t d, int dtype,
+                                                 int64_t page_size, int64_t max_blocks, int64_t window, int64_t sinks) {
+    // (any addresses: the checks look at them, nothing is read)
+    static const int64_t strides[6] = {};
+    void* some = reinterpret_cast<void*>(uintptr_t(16));
+    PageView pv;
+    if (batch <= 0 || window < 0 || sinks < 0 ||
+        fill_view(pv, "paged_attention", some, some, dtype, strides, static_cast<int32_t*>(some), max_blocks,
+                  static_cast<int32_t*>(some), batch, hq, hkv, d, 1, page_size, max_blocks) != SMLM_OK)
+        return 0;
+    const int win = clamp_window(window), snk = clamp_sinks(sinks);
+    if (with_variant(pv, dtype, [&](auto v) {
+            using V = decltype(v);
+            return cluster_size<V::cluster>(pv, V::S::QT, V::S::TT, win, snk);
+        }))
+        return 0;
     WorkspaceSize ws;
     SplitWork wk;
-    split_work(ws, wk, std::max<int64_t>(batch, 0), hq, hkv, d, element_bytes(dtype));
+    split_work(ws, wk, batch, hq, hkv, d, element_bytes(dtype));
     return ws.used;
 }
 
@@ -1268,16 +1308,19 @@ extern "C" int smlm_paged_attention(const void* q, const void* k_pages, const vo
     SMLM_CHECK_ARG((double)batch * hq * ((double)max_blocks * page_size / 16 + HEAD + 1) < 2147483648.0,
                    "paged_attention: %lld sequences x %lld heads x up to %lld tokens: fewer rows a call",
                    (long long)batch, (long long)hq, (long long)(max_blocks * page_size));
-    const int win = (int)std::min<int64_t>(window, INT32_MAX), snk = (int)std::min<int64_t>(sinks, INT32_MAX / 2);
-    Workspace ws(workspace, workspace_bytes);
-    SplitWork wk;
-    split_work(ws, wk, batch, hq, hkv, d, element_bytes(dtype));
-    if (!workspace || !ws.ok()) {
-        set_error("paged_attention: workspace of %zu bytes, %zu needed", workspace_bytes, ws.used);
-        return SMLM_ERR_WORKSPACE;
-    }
-    return by_dtype(dtype, [&](auto t) {
-        return launch_attention<decltype(t)>(pv, q, scale, win, snk, out, lse, wk, status, as_stream(stream));
+    const AttentionArgs args{q, scale, clamp_window(window), clamp_sinks(sinks), out, lse, status, as_stream(stream)};
+    return with_variant(pv, dtype, [&](auto v) {
+        using V = decltype(v);
+        if (const int size = cluster_size<V::cluster>(pv, V::S::QT, V::S::TT, args.window, args.sinks))
+            return launch_cluster(v, pv, size, args);
+        Workspace ws(workspace, workspace_bytes);
+        SplitWork wk;
+        split_work(ws, wk, batch, hq, hkv, d, element_bytes(dtype));
+        if (!workspace || !ws.ok()) {
+            set_error("paged_attention: workspace of %zu bytes, %zu needed", workspace_bytes, ws.used);
+            return SMLM_ERR_WORKSPACE;
+        }
+        return launch_list(v, pv, wk, args);
     });
 }
 

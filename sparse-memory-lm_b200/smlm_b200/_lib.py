@@ -100,7 +100,7 @@ SIGNATURES = {
     "smlm_host_rows_add": (_i32, [_p, _p, _p, _i64, _p, _p, _p, _i64, _i64, _p, _p]),
     "smlm_rows_rowwise_step": (_i32, [_p, _i64, _p, _p, _p, _i64, _i64, _p, _p, _i32, _f32, _f32, _f32, _p, _f32,
                                       _i32, _p, _p]),
-    "smlm_paged_attention_workspace": (_sz, [_i64, _i64, _i64, _i64, _i32]),
+    "smlm_paged_attention_workspace": (_sz, [_i64, _i64, _i64, _i64, _i32, _i64, _i64, _i64, _i64]),
     "smlm_paged_attention": (_i32, [_p, _p, _p, _i32, _p, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                                     _f32, _i64, _i64, _p, _p, _p, _sz, _p, _p]),
     "smlm_paged_append": (_i32, [_p, _p, _p, _i32, _p, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,

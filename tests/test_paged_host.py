@@ -32,9 +32,11 @@ def test_attention_refusals(args, text):
 
 
 def test_workspaces():
-    assert attention(nbytes=16) == L.ERR_WORKSPACE and attention(ws=None) == L.ERR_WORKSPACE
+    roomy = {"blocks": 60000, "stride": 60000}       # so much that it is not one launch without scratch
+    assert attention(nbytes=16, **roomy) == L.ERR_WORKSPACE and attention(ws=None, **roomy) == L.ERR_WORKSPACE
     lib = L.lib()
-    assert lib.smlm_paged_attention_workspace(4, 8, 2, 64, L.BF16) > 0
+    assert lib.smlm_paged_attention_workspace(4, 8, 2, 64, L.BF16, 16, 60000, 0, 0) > 0
+    assert lib.smlm_paged_attention_workspace(4, 8, 3, 64, L.BF16, 16, 60000, 0, 0) == 0      # refused arguments
     assert lib.smlm_pages_extend(P, 4, 4, 4, P, P, 8, 16, P, 2, 1, P, 8, None, None) == L.ERR_WORKSPACE
     assert lib.smlm_pages_fork(P, 2, 2, 128, P, 4, 4, 4, P, P, 8, 16, P, P, 2, P, 8, None, None) == L.ERR_WORKSPACE
     assert lib.smlm_pages_compact(P, 2, 2, 128, P, 4, 4, 4, P, 8, 16, P, 8, None, None) == L.ERR_WORKSPACE
