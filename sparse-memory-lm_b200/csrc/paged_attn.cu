@@ -28,7 +28,7 @@ namespace smlm {
 // Device time per call, share of the measured copy rate (6570 GB/s) for the bytes of the visible keys and values:
 //   64 x 2175 tokens, 6 heads x 64, bf16: 40.2 us, 81%; 1 x 131071, 32 / 8 heads x 128, fp16: 86.1 us, 95%;
 //   96 x 0-8191, 32 / 8 x 128, bf16: 67.0 us, 85%; 64 x 1028 seen, 16 / 2 x 128, fp16: 17.3 us (cluster), 59%;
-//   1 x 2304, 6 x 64, bf16: 6.9 us (cluster); 32 x 2048 x 8 heads, fp32, d 64 / 128: 54 / 53 us, 76%.
+//   1 x 2304, 6 x 64, bf16: 5.9 us (cluster); 32 x 2048 x 8 heads, fp32, d 64 / 128: 54 / 53 us, 76%.
 // While all warps run, memory delivers 93% of the copy rate; the rest is the start (2.5 us to the first tiles), the
 // spread of the last warps (4 us) and the join (3 us).
 
@@ -193,6 +193,8 @@ struct SplitShape {
     static constexpr bool WIDE = DP * ES > 256, HALVES = DP * ES > 512;
     static constexpr int KK = HALVES ? KJ / 2 : KJ, VR = HALVES ? 2 : 4;
     static constexpr int BLOCKS = DP * ES * NT <= 128 ? 4 : DP * ES * NT <= 256 ? 3 : 2;  // per SM (registers)
+    // the larger blocks of paged_cluster_kernel: eight warps up to d 64 (at d 128 they lose: 1 x 2048 tokens 8.3 -> 8.5 us)
+    static constexpr int MORE_WARPS = QT * DP <= 512 ? 8 : 4;
 };
 
 // Tiles first .. last - 1 of one item by one warp: the sums of its columns. PART: d < DP; SMALL: pages of fewer than
@@ -767,15 +769,15 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP, NT>::BLOCKS)
 // the blocks' shared memory, so that the call is one launch and nothing goes through global memory in between. One
 // sequence of 64 / 1024 tokens (6 heads x 64): 3.5 / 4.9 us, a launch and a chain of four dependent loads (cluster_size
 // says when, with the list's times).
-template <typename T, int DP, int NT, bool PART, bool SMALL>
-__global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP, NT>::BLOCKS)
+template <typename T, int DP, int NT, bool PART, bool SMALL, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, SplitShape<T, DP, NT>::BLOCKS * 4 / WARPS)
     paged_cluster_kernel(PageView pv, const T* __restrict__ q, float c, int window, int sinks, T* __restrict__ out,
                          float* __restrict__ lse, int* status) {
     using S = SplitShape<T, DP, NT>;
     constexpr int CH = S::CH, TT = S::TT, VB = S::VB, QT = S::QT, FOURS = DP / 4;
-    __shared__ float4 so[SPLIT_WARPS][QT][FOURS];  // before it a warp's queries, in the wide shapes
+    __shared__ float4 so[WARPS][QT][FOURS];  // before it a warp's queries, in the wide shapes
     static_assert(!S::WIDE || sizeof(so[0]) >= NT * S::KJ * 32 * sizeof(uint4), "a warp's queries fit in its results");
-    __shared__ float2 sml[SPLIT_WARPS][QT], joined[QT];
+    __shared__ float2 sml[WARPS][QT], joined[QT];
     grid_wait();
     grid_release();
     const int lane = lane_id(), warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
@@ -786,7 +788,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP, NT>::BLOCKS)
     const int unit = blockIdx.x / size, b = unit / items, h = unit % items / gt, q0 = unit % items % gt * QT;
     const int cols = min(QT, group - q0);
     const Span span(row_length(pv, b, rank == 0 ? status : nullptr), window, sinks, TT);
-    const int workers = size * SPLIT_WARPS, worker = rank * SPLIT_WARPS + warp;
+    const int workers = size * WARPS, worker = rank * WARPS + warp;
     const int first = span.tiles * worker / workers, last = span.tiles * (worker + 1) / workers;
     if (first < last) {
         Stream<T, DP, NT, PART, SMALL> st;
@@ -834,15 +836,15 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP, NT>::BLOCKS)
         return make_float2(m, l);
     };
     float4 acc;
-    for (int e = threadIdx.x; e < cols * FOURS; e += SPLIT_THREADS) {
+    for (int e = threadIdx.x; e < cols * FOURS; e += WARPS * 32) {
         const int col = e / FOURS, f = e % FOURS;
         const float2 ml =
-            add_up(SPLIT_WARPS, [&](int w) { return sml[w][col]; }, [&](int w) { return so[w][col][f]; }, acc);
+            add_up(WARPS, [&](int w) { return sml[w][col]; }, [&](int w) { return so[w][col][f]; }, acc);
         so[0][col][f] = acc;
         if (f == 0) joined[col] = ml;
     }
     cluster_sync();
-    for (int e = rank * SPLIT_THREADS + threadIdx.x; e < cols * FOURS; e += size * SPLIT_THREADS) {
+    for (int e = rank * WARPS * 32 + threadIdx.x; e < cols * FOURS; e += size * WARPS * 32) {
         const int col = e / FOURS, f = e % FOURS;
         const float2 ml = add_up((int)size, [&](int r) { return of_block(&joined[col], r); },
                                  [&](int r) { return of_block(&so[0][col][f], r); }, acc);
@@ -1138,7 +1140,7 @@ static void split_work(W& ws, SplitWork& wk, int64_t batch, int64_t hq, int64_t 
 
 // How many clusters of `size` blocks of the kernel run at once on this card (asked once per kernel and size): fewer than
 // the blocks that fit, because a cluster lies in one part of the card.
-template <auto kernel>
+template <auto kernel, int WARPS>
 static int64_t clusters_at_once(int size) {
     static std::atomic<int> known[17];  // the answer + 1
     int n = known[size].load();
@@ -1149,7 +1151,7 @@ static int64_t clusters_at_once(int size) {
     }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(size);
-    cfg.blockDim = dim3(SPLIT_THREADS);
+    cfg.blockDim = dim3(WARPS * 32);
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = size;
@@ -1173,21 +1175,28 @@ static int64_t clusters_at_once(int size) {
 //   more clusters than run at once 15.4 -> 22.5 (16 x 2304 in sixes).
 // Up to six tiles a warp with a window, under which long sequences do the same work (64 x 1028 seen: 20.3 -> 17.3).
 // Sixteen blocks find room slowly where several share an SM (fp32, 4 x 2048: 11.7 -> 17.5), so they are for calls of at
-// most a block per SM (1 x 2304: 7.3 -> 6.8).
-template <auto kernel>
-static int cluster_size(const PageView& pv, int qt, int tt, int64_t window, int64_t sinks) {
+// most a block per SM, and then of eight warps for more tiles than 64 (1 x 2304: list 7.3, sixteen blocks of four warps
+// 6.9, of eight 5.9; eight warps everywhere would cost 5% on average: 1 x 1024 4.9 -> 5.9).
+struct Cluster {
+    int size, warps;  // blocks per item (0: the list), warps of a block
+};
+template <typename V>
+static Cluster cluster_size(const PageView& pv, int64_t window, int64_t sinks) {
+    constexpr int QT = V::S::QT, TT = V::S::TT, MORE = V::S::MORE_WARPS, W = 4;
     int64_t most = (int64_t)pv.max_blocks << pv.page_shift;  // tokens that any sequence can see
-    if (window) most = std::min(most, window + sinks + 2 * tt);
-    const int64_t tiles = (most + tt - 1) / tt, items = (int64_t)pv.batch * pv.hkv * ((pv.hq / pv.hkv + qt - 1) / qt);
-    if (tiles <= SPLIT_WARPS) return items <= 2 * clusters_at_once<kernel>(1);  // blocks alone: two rounds are as fast
-    if (tiles > 8 * SPLIT_WARPS && tiles <= 16 * SPLIT_WARPS * 2 && items * 16 <= sm_count() &&
-        items <= clusters_at_once<kernel>(16))
-        return 16;
-    for (int size = (int)std::min<int64_t>(8, (tiles + SPLIT_WARPS - 1) / SPLIT_WARPS); size >= 1; size--) {
-        if (tiles > size * SPLIT_WARPS * (window ? 6 : size == 8 ? 4 : 3)) break;
-        if (items <= clusters_at_once<kernel>(size)) return size;
+    if (window) most = std::min(most, window + sinks + 2 * TT);
+    const int64_t tiles = (most + TT - 1) / TT, items = (int64_t)pv.batch * pv.hkv * ((pv.hq / pv.hkv + QT - 1) / QT);
+    const auto at_once = [](int size) { return clusters_at_once<V::cluster, W>(size); };
+    if (tiles <= W) return {items <= 2 * at_once(1), W};  // blocks alone: two rounds are as fast
+    if (tiles > 8 * W && items * 16 <= sm_count()) {
+        if (tiles <= 16 * W && items <= at_once(16)) return {16, W};
+        if (tiles <= 16 * MORE * 2 && items <= clusters_at_once<V::cluster_more, MORE>(16)) return {16, MORE};
     }
-    return 0;
+    for (int size = (int)std::min<int64_t>(8, (tiles + W - 1) / W); size >= 1; size--) {
+        if (tiles > size * W * (window ? 6 : size == 8 ? 4 : 3)) break;
+        if (items <= at_once(size)) return {size, W};
+    }
+    return {0, W};
 }
 
 // The kernels' template arguments for a call.
@@ -1196,7 +1205,8 @@ struct Variant {
     using T = T_;
     using S = SplitShape<T_, DP_, NT_>;
     static constexpr int DP = DP_, NT = NT_;
-    static constexpr auto cluster = paged_cluster_kernel<T_, DP_, NT_, PART_, SMALL_>;
+    static constexpr auto cluster = paged_cluster_kernel<T_, DP_, NT_, PART_, SMALL_, 4>;
+    static constexpr auto cluster_more = paged_cluster_kernel<T_, DP_, NT_, PART_, SMALL_, S::MORE_WARPS>;
     static constexpr auto split = paged_split_kernel<T_, DP_, NT_, PART_, SMALL_>;
 };
 
@@ -1234,10 +1244,11 @@ struct AttentionArgs {
 };
 
 template <typename V>
-static int launch_cluster(V, const PageView& pv, int size, const AttentionArgs& a) {
+static int launch_cluster(V, const PageView& pv, const Cluster& c, const AttentionArgs& a) {
     using T = typename V::T;
     const int64_t items = (int64_t)pv.batch * pv.hkv * ((pv.hq / pv.hkv + V::S::QT - 1) / V::S::QT);
-    return launch_dependent(V::cluster, "paged_attention", size, size * items, SPLIT_THREADS, a.st, pv,
+    return launch_dependent(c.warps == 4 ? V::cluster : V::cluster_more, "paged_attention", c.size, c.size * items,
+                            c.warps * 32, a.st, pv,
                             static_cast<const T*>(a.q), a.scale * 1.4426950408889634074f, a.window, a.sinks,
                             static_cast<T*>(a.out), a.lse, a.status);
 }
@@ -1280,7 +1291,7 @@ extern "C" size_t smlm_paged_attention_workspace(int64_t batch, int64_t hq, int6
     const int win = clamp_window(window), snk = clamp_sinks(sinks);
     if (with_variant(pv, dtype, [&](auto v) {
             using V = decltype(v);
-            return cluster_size<V::cluster>(pv, V::S::QT, V::S::TT, win, snk);
+            return cluster_size<V>(pv, win, snk).size;
         }))
         return 0;
     WorkspaceSize ws;
@@ -1311,8 +1322,8 @@ extern "C" int smlm_paged_attention(const void* q, const void* k_pages, const vo
     const AttentionArgs args{q, scale, clamp_window(window), clamp_sinks(sinks), out, lse, status, as_stream(stream)};
     return with_variant(pv, dtype, [&](auto v) {
         using V = decltype(v);
-        if (const int size = cluster_size<V::cluster>(pv, V::S::QT, V::S::TT, args.window, args.sinks))
-            return launch_cluster(v, pv, size, args);
+        const Cluster c = cluster_size<V>(pv, args.window, args.sinks);
+        if (c.size) return launch_cluster(v, pv, c, args);
         Workspace ws(workspace, workspace_bytes);
         SplitWork wk;
         split_work(ws, wk, batch, hq, hkv, d, element_bytes(dtype));
