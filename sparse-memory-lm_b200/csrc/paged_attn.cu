@@ -1138,12 +1138,18 @@ static void split_work(W& ws, SplitWork& wk, int64_t batch, int64_t hq, int64_t 
     take(wk.o, slots * wk.rows * dp);
 }
 
-// How many clusters of `size` blocks of the kernel run at once on this card (asked once per kernel and size): fewer than
-// the blocks that fit, because a cluster lies in one part of the card.
+// How many clusters of `size` blocks of the kernel run at once on the current device (asked once per kernel, size and
+// device, and more than the portable eight blocks allowed then): fewer than the blocks that fit, because a cluster lies
+// in one part of the card.
 template <auto kernel, int WARPS>
 static int64_t clusters_at_once(int size) {
-    static std::atomic<int> known[17];  // the answer + 1
-    int n = known[size].load();
+    static std::atomic<int> known[64][17];  // the answer + 1
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    if (dev < 64) n = known[dev][size].load();
     if (n) return n - 1;
     if (size > 8 && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
         cudaGetLastError();
@@ -1162,7 +1168,7 @@ static int64_t clusters_at_once(int size) {
         cudaGetLastError();
         return 0;
     }
-    known[size].store(n + 1);
+    if (dev < 64) known[dev][size].store(n + 1);
     return n;
 }
 
