@@ -414,8 +414,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) pages_compact_kernel(Pages pg, i
 // --------------------------------------------------------------------------------------------------- moving
 // The listed pages' tokens in every (layer, k / v) plane: one warp per (entry, plane, head), 16 bytes a lane and four
 // loads in flight before the first store. With `to`, the table's entries follow their pages. Memory bounds it: 1583 pages
-// of 147 KB in 72 us, 99% of the measured copy rate; one load at a time
-// took 91 us.
+// of 147 KB in 72 us, 99% of the measured copy rate; one load at a time took 91 us.
 __global__ void __launch_bounds__(256) pages_copy_kernel(char* pool, CopyList cl, int planes, int heads, int n_pages,
                                                          int page_size, int token_bytes, Pages pg, const int32_t* to,
                                                          const int32_t* live) {
