@@ -18,7 +18,9 @@ namespace smlm {
 // With queries as the 8 columns, up to 8 query heads of one key head cost the same as one. (mma.sync is enough: the
 // tile of queries is 8 wide, and tcgen05's 128-row tiles would be 1/16 full or less.) Running maxima and sums are
 // fp32, one per column; the weights enter the second product as a sum of two 16-bit values (hi + lo), so they carry
-// 16 bits or more and rounding the output is the only loss that shows.
+// 16 bits or more and rounding the output is the only loss that shows. fp16 ends at 2^-24, which weights of at most 1
+// pass 17 nats below the maximum, while their fp32 sum keeps them: they are taken 2^15 times as large there (WEIGHT) and
+// carry 16 bits down to 2^-24 of the largest weight; what is below 2^-40 of it adds nothing.
 // fp32 caches use the same shape with tf32 fragments, each operand split in two and three products kept (2^-21).
 //
 // The tiles of all (sequence, key head, 8 or 16 query heads) items form one list, cut evenly over all warps of the grid,
@@ -204,6 +206,8 @@ struct Stream {
     using S = SplitShape<T, DP, NT>;
     static constexpr int CH = S::CH, TT = S::TT, NS = S::NS, KJ = S::KJ, KK = S::KK, VB = S::VB, VR = S::VR, MT = S::MT;
     static constexpr bool WIDE = S::WIDE, HALVES = S::HALVES, F = S::ES == 4;
+    // a weight in the second product, and so o, is WEIGHT times what l counts; an exact factor, taken out in values()
+    static constexpr float WEIGHT = std::is_same_v<T, __half> ? 32768.f : 1.f;
     // The tile after next goes to L2 where few bytes are in flight otherwise (two eights of queries: 8 warps an SM; d
     // well below DP): 64 x 8192 tokens, 32 heads on one: 107 -> 96 us, d 80: 70 -> 66, fp32 d 128: 58 -> 56. Where the
     // loads alone fill the memory's queues it costs: d 64 40.3 -> 41.9, one of 131071 tokens 86.8 -> 91.9.
@@ -543,7 +547,7 @@ struct Stream {
                     for (int n = 0; n < NT; n++)
 #pragma unroll
                         for (int r = 0; r < 2; r++) {
-                            const float x = sc[n][s][2 * r], y = sc[n][s][2 * r + 1];
+                            const float x = sc[n][s][2 * r] * WEIGHT, y = sc[n][s][2 * r + 1] * WEIGHT;
                             const uint32_t w = pack16<T>(x, y);
                             const float2 u = unpack16<T>(w);
                             hi[n][r] = transpose8x8(w);
@@ -593,6 +597,7 @@ struct Stream {
 
     // CH consecutive values, (g + 8 vb) CH and on, of column 2 t4 + x of eight n
     __device__ __forceinline__ void values(int n, int x, int vb, float scale, float (&v)[CH]) const {
+        scale *= 1.f / WEIGHT;
 #pragma unroll
         for (int k = 0; k < MT; k++) {
             v[2 * k] = o[n][vb * MT + k][x] * scale;
