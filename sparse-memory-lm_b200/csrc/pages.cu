@@ -65,23 +65,24 @@ __global__ void __launch_bounds__(256) pages_trim_kernel(Pages pg, const int32_t
 
 // ------------------------------------------------------------------------------------------------- planning
 // Exclusive sum over the block, in thread order; *total receives the sum of all.
-__device__ __forceinline__ int block_scan(int v, int* total) {
-    __shared__ int part[PLAN_THREADS / 32];
+template <typename V>
+__device__ __forceinline__ V block_scan(V v, V* total) {
+    __shared__ V part[PLAN_THREADS / 32];
     const int lane = lane_id(), warp = threadIdx.x >> 5;
-    int x = v;
+    V x = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(FULL, x, o);
+        const V y = __shfl_up_sync(FULL, x, o);
         if (lane >= o) x += y;
     }
     __syncthreads();
     if (lane == 31) part[warp] = x;
     __syncthreads();
     if (warp == 0) {
-        int p = part[lane];
+        V p = part[lane];
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(FULL, p, o);
+            const V y = __shfl_up_sync(FULL, p, o);
             if (lane >= o) p += y;
         }
         part[lane] = p;
@@ -206,19 +207,20 @@ __device__ int list_free(const Team& team, const Pages& pg, int32_t* list, int m
     return total;
 }
 
-// offset[i] = sum of need(0 .. i-1); returns the sum of all. need(i) is called once for each i < n. One block.
+// offset[i] = sum of need(0 .. i-1); returns the sum of all; both at most `most` (the pages there are: more cannot be
+// handed out). need(i) is called once for each i < n. One block. The sums are 64-bit: 65535 rows may want 2^30 pages each.
 template <typename F>
-__device__ int scan_needs(int n, int32_t* offset, F need) {
-    int sum = 0;
+__device__ int scan_needs(int n, int32_t* offset, int most, F need) {
+    int64_t sum = 0;
     for (int base = 0; base < n; base += PLAN_THREADS) {
         const int i = base + threadIdx.x;
-        int total;
-        const int off = block_scan(i < n ? need(i) : 0, &total);
-        if (i < n) offset[i] = sum + off;
+        int64_t total;
+        const int64_t off = block_scan<int64_t>(i < n ? need(i) : 0, &total);
+        if (i < n) offset[i] = (int32_t)min(sum + off, (int64_t)most);
         sum += total;
         __syncthreads();
     }
-    return sum;
+    return (int)min(sum, (int64_t)most);
 }
 
 // lengths[r] += n_new for every listed row, with the pages that takes: rows in order, lowest free pages first. A row
@@ -236,7 +238,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) pages_extend_kernel(Pages pg, co
     auto blocks = [&](int64_t len) { return (int)((len + (1 << shift) - 1) >> shift); };
     auto fits = [&](int len) { return len >= 0 && (int64_t)len + n_new <= cap; };
     if (team.rank == 0) {
-        const int wanted = scan_needs(n, offset, [&](int i) {
+        const int wanted = scan_needs(n, offset, pg.n_pages, [&](int i) {
             const int r = rows[i];
             const bool ok = row_ok(pg, r);
             const int len = ok ? atomicExch(pg.lengths + r, TAKEN) : TAKEN;
@@ -254,7 +256,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) pages_extend_kernel(Pages pg, co
         if (len == TAKEN) continue;
         bool grow = fits(len);
         const int b0 = blocks(len), need = grow ? blocks((int64_t)len + n_new) - b0 : 0, off = __ldcg(offset + i);
-        if (need && off + need > have) {
+        if (need && (int64_t)off + need > have) {
             flag(pg.status, SMLM_FLAG_NO_PAGES);
             grow = false;
         }
@@ -330,7 +332,7 @@ __global__ void __launch_bounds__(PLAN_THREADS)
     }
     team.sync();
     if (team.rank == 0) {
-        const int wanted = scan_needs(n, offset, [&](int i) { return __ldcg(cl.tokens + i) ? 1 : 0; });
+        const int wanted = scan_needs(n, offset, pg.n_pages, [&](int i) { return __ldcg(cl.tokens + i) ? 1 : 0; });
         if (threadIdx.x == 0) totals[MAX_TEAM] = wanted;
     }
     for (int i = warp0; i < n; i += warps) {
