@@ -6,7 +6,8 @@
 namespace smlm {
 
 // Programmatic dependent launch: a kernel that was launched while its predecessor runs waits for that one's end and
-// memory before it touches anything the predecessor wrote; grid_release lets the successor be launched.
+// memory before it touches anything the predecessor wrote; grid_release lets the successor be launched. What a kernel
+// reads may thus be written while it already runs (before grid_wait returns), so no load here is a non-coherent one.
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;"); }
 
@@ -61,7 +62,7 @@ __device__ __forceinline__ int row_length(const PageView& pv, int b, int* status
 
 // The page that holds token t of row b, or -1: a hole (entry -1) or an entry outside the pool (flagged).
 __device__ __forceinline__ int page_of(const PageView& pv, int b, int t, int* status) {
-    const int p = __ldg(pv.table + b * pv.table_stride + (t >> pv.page_shift));
+    const int p = pv.table[b * pv.table_stride + (t >> pv.page_shift)];
     if (p >= pv.n_pages) {
         flag(status, SMLM_FLAG_INDEX_RANGE);
         return -1;

@@ -45,7 +45,7 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ uint4 load16(const void* p) {
     uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                  : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                  : "l"(p));
     return v;
@@ -265,7 +265,7 @@ struct Stream {
         auto entry = [&](int t) {  // the page of token t, or -1 past the end, in a hole or outside the pool
             int p = -1;
             if (t < span.n) {
-                p = __ldg(row + (t >> shift));
+                p = row[t >> shift];
                 if (p >= pv.n_pages) {
                     flag(status, SMLM_FLAG_INDEX_RANGE);
                     p = -1;
@@ -610,8 +610,8 @@ struct Stream {
 // last pieces of cut items go to the workspace, whole items straight to the output.
 template <typename T, int DP, int NT, bool PART, bool SMALL>
 __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP, NT>::BLOCKS)
-    paged_split_kernel(PageView pv, const T* __restrict__ q, float c, int window, int sinks, T* __restrict__ out,
-                       float* __restrict__ lse, SplitWork wk, int* status) {
+    paged_split_kernel(PageView pv, const T* q, float c, int window, int sinks, T* __restrict__ out, float* __restrict__ lse,
+                       SplitWork wk, int* status) {
     using S = SplitShape<T, DP, NT>;
     constexpr int CH = S::CH, TT = S::TT, VB = S::VB, QT = S::QT;
     __shared__ int4 pre[SPLIT_THREADS / 4];
@@ -776,7 +776,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, SplitShape<T, DP, NT>::BLOCKS)
 // says when, with the list's times).
 template <typename T, int DP, int NT, bool PART, bool SMALL, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32, SplitShape<T, DP, NT>::BLOCKS * 4 / WARPS)
-    paged_cluster_kernel(PageView pv, const T* __restrict__ q, float c, int window, int sinks, T* __restrict__ out,
+    paged_cluster_kernel(PageView pv, const T* q, float c, int window, int sinks, T* __restrict__ out,
                          float* __restrict__ lse, int* status) {
     using S = SplitShape<T, DP, NT>;
     constexpr int CH = S::CH, TT = S::TT, VB = S::VB, QT = S::QT, FOURS = DP / 4;
@@ -994,9 +994,8 @@ constexpr int APPEND_THREADS = 128, APPEND_HEADS = 3;
 
 template <typename T, int U>
 __global__ void __launch_bounds__(APPEND_THREADS)
-    paged_append_kernel(PageView pv, const T* __restrict__ qkv, int tokens, const float* __restrict__ cosb,
-                        const float* __restrict__ sinb, int max_pos, T* __restrict__ q_out, int groups,
-                        int per_block, uint32_t all, int* status) {
+    paged_append_kernel(PageView pv, const T* qkv, int tokens, const float* cosb, const float* sinb, int max_pos,
+                        T* __restrict__ q_out, int groups, int per_block, uint32_t all, int* status) {
     constexpr int CH = 16 / sizeof(T);
     grid_wait();
     grid_release();
@@ -1028,8 +1027,8 @@ __global__ void __launch_bounds__(APPEND_THREADS)
                     const float* sp = sinb + (int64_t)pos * half + c;
 #pragma unroll
                     for (int k = 0; k < CH; k += 4) {
-                        const float4 x = __ldg(reinterpret_cast<const float4*>(cp + k));
-                        const float4 y = __ldg(reinterpret_cast<const float4*>(sp + k));
+                        const float4 x = *reinterpret_cast<const float4*>(cp + k);
+                        const float4 y = *reinterpret_cast<const float4*>(sp + k);
                         cs[k] = x.x, cs[k + 1] = x.y, cs[k + 2] = x.z, cs[k + 3] = x.w;
                         sn[k] = y.x, sn[k + 1] = y.y, sn[k + 2] = y.z, sn[k + 3] = y.w;
                     }
