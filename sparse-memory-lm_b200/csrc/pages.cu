@@ -208,25 +208,27 @@ __device__ int list_free(const Team& team, const Pages& pg, int32_t* list, int m
 }
 
 // offset[i] = sum of need(0 .. i-1); returns the sum of all; both at most `most` (the pages there are: more cannot be
-// handed out). need(i) is called once for each i < n. One block. The sums are 64-bit: 65535 rows may want 2^30 pages each.
-template <typename F>
+// handed out). need(i) is called once for each i < n. One block. V holds the sum of all (65535 rows may want 2^30 each).
+template <typename V, typename F>
 __device__ int scan_needs(int n, int32_t* offset, int most, F need) {
-    int64_t sum = 0;
+    V sum = 0;
     for (int base = 0; base < n; base += PLAN_THREADS) {
         const int i = base + threadIdx.x;
-        int64_t total;
-        const int64_t off = block_scan<int64_t>(i < n ? need(i) : 0, &total);
-        if (i < n) offset[i] = (int32_t)min(sum + off, (int64_t)most);
+        V total;
+        const V off = block_scan<V>(i < n ? need(i) : 0, &total);
+        if (i < n) offset[i] = (int32_t)min(sum + off, (V)most);
         sum += total;
         __syncthreads();
     }
-    return (int)min(sum, (int64_t)most);
+    return (int)min(sum, (V)most);
 }
 
 // lengths[r] += n_new for every listed row, with the pages that takes: rows in order, lowest free pages first. A row
 // whose pages are not there, or whose table is too narrow, stays as it is and raises a flag. The lengths are taken by
 // an exchange and put back at the end, which finds rows listed twice (the second does nothing). Without a page to
 // hand out (most decoding steps) the counts are not read. Eight rows: 4 us, a launch and four dependent accesses.
+// V: what the wanted pages are summed in; the host takes 32 bits where they cannot pass them (64: 0.2 us more).
+template <typename V>
 __global__ void __launch_bounds__(PLAN_THREADS) pages_extend_kernel(Pages pg, const int32_t* rows, int n, int n_new,
                                                                     int shift, int32_t* offset, int32_t* len_of,
                                                                     int32_t* list, int32_t* totals) {
@@ -238,7 +240,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) pages_extend_kernel(Pages pg, co
     auto blocks = [&](int64_t len) { return (int)((len + (1 << shift) - 1) >> shift); };
     auto fits = [&](int len) { return len >= 0 && (int64_t)len + n_new <= cap; };
     if (team.rank == 0) {
-        const int wanted = scan_needs(n, offset, pg.n_pages, [&](int i) {
+        const int wanted = scan_needs<V>(n, offset, pg.n_pages, [&](int i) {
             const int r = rows[i];
             const bool ok = row_ok(pg, r);
             const int len = ok ? atomicExch(pg.lengths + r, TAKEN) : TAKEN;
@@ -332,7 +334,7 @@ __global__ void __launch_bounds__(PLAN_THREADS)
     }
     team.sync();
     if (team.rank == 0) {
-        const int wanted = scan_needs(n, offset, pg.n_pages, [&](int i) { return __ldcg(cl.tokens + i) ? 1 : 0; });
+        const int wanted = scan_needs<int>(n, offset, pg.n_pages, [&](int i) { return __ldcg(cl.tokens + i) ? 1 : 0; });
         if (threadIdx.x == 0) totals[MAX_TEAM] = wanted;
     }
     for (int i = warp0; i < n; i += warps) {
@@ -560,8 +562,10 @@ extern "C" int smlm_pages_extend(int32_t* table, int64_t table_stride, int64_t t
         set_error("pages_extend: workspace of %zu bytes, %zu needed", workspace_bytes, ws.used);
         return SMLM_ERR_WORKSPACE;
     }
-    return launch_plan(pages_extend_kernel, "pages_extend", std::max(n, n_pages), as_stream(stream), pg, rows, (int)n,
-                       (int)n_new, log2_of(page_size), offset, len_of, list, totals);
+    const bool fits = n * (n_new / page_size + 1) <= INT32_MAX;  // a row's need is at most that
+    return launch_plan(fits ? pages_extend_kernel<int32_t> : pages_extend_kernel<int64_t>, "pages_extend",
+                       std::max(n, n_pages), as_stream(stream), pg, rows, (int)n, (int)n_new, log2_of(page_size), offset,
+                       len_of, list, totals);
 }
 
 extern "C" size_t smlm_pages_fork_workspace(int64_t n, int64_t table_rows, int64_t max_blocks, int64_t n_pages) {
