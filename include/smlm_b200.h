@@ -481,8 +481,9 @@ SMLM_API int smlm_ngram_rows(const int64_t *c, int64_t batch, int64_t t_len, int
  * order, -1 where it has none, and lengths[b] (int32) counts its tokens. strides: six host integers, the elements
  * between pages, heads and tokens of k_pages and then of v_pages (multiples of 16 bytes; the head dimension d, a
  * multiple of 16 up to 256, is contiguous), so that any order of pages, heads and tokens serves. dtype: F32, BF16 or
- * F16, the same for the cache and the activations. Page numbers outside the pool and lengths outside the table set
- * SMLM_FLAG_INDEX_RANGE and are left out. */
+ * F16, the same for the cache and the activations. Page numbers outside the pool and lengths outside the table (below 0
+ * or beyond max_blocks * page_size) set SMLM_FLAG_INDEX_RANGE and are left out: such an entry is as one of -1, such a row
+ * as an empty one (its outputs are 0, nothing of it is stored). */
 
 /* Scratch bytes of smlm_paged_attention with these arguments on the current device; 0 where it needs none. */
 SMLM_API size_t smlm_paged_attention_workspace(int64_t batch, int64_t hq, int64_t hkv, int64_t d, int dtype,

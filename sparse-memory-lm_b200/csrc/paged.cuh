@@ -49,13 +49,13 @@ struct PageView {
     int batch, hq, hkv, d, n_pages, page_shift, max_blocks;
 };
 
-// Tokens of row b that the table can hold at all (a length beyond the table is cut and flagged).
+// Tokens of row b. A length outside the table is flagged and the row left out, as if it were empty: a length cut to the
+// table's end would place an append on the tokens that are there.
 __device__ __forceinline__ int row_length(const PageView& pv, int b, int* status) {
     const int n = pv.lengths[b];
-    const int64_t cap = (int64_t)pv.max_blocks << pv.page_shift;
-    if (n < 0 || n > cap) {
+    if (n < 0 || n > (int64_t)pv.max_blocks << pv.page_shift) {
         flag(status, SMLM_FLAG_INDEX_RANGE);
-        return n < 0 ? 0 : (int)cap;
+        return 0;
     }
     return n;
 }

@@ -1,11 +1,25 @@
 """Lengths outside the table, pools that cannot hold what is asked for: what a call leaves out stays as it was."""
+import math
+
 import pytest
 import torch
 
+import paged_ref as R
+from smlm_b200 import _lib as L
 from smlm_b200 import paged
-from test_gpu_paged import DEV
+from test_gpu_paged import BF16, DEV, F32, make, roomy
 
 pytestmark = pytest.mark.gpu
+
+
+def unchecked(monkeypatch):
+    """Calls return although flags are raised, as they do in use."""
+    monkeypatch.setenv("SMLM_B200_CHECK", "0")
+
+
+def flags():
+    torch.cuda.synchronize()
+    return L.read_status(torch.device(DEV, torch.cuda.current_device()))
 
 
 def test_extend_by_more_pages_than_31_bits_count():
@@ -19,3 +33,44 @@ def test_extend_by_more_pages_than_31_bits_count():
     assert lengths[0] == blocks and not bool(lengths[1:].any())
     assert torch.equal(table[0], torch.arange(blocks, dtype=torch.int32, device=DEV))
     assert bool((table[1:] == -1).all()) and ref.tolist() == [1] * blocks + [0] * 5
+
+
+@pytest.mark.parametrize("bad", [10 ** 6, 49, -1, -10 ** 6])
+@pytest.mark.parametrize("tokens", [1, 5])
+def test_append_leaves_out_rows_whose_length_is_outside_the_table(monkeypatch, bad, tokens):
+    """The table has room for 48 tokens: a row of 49 is left out whole, with queries of 0."""
+    unchecked(monkeypatch)
+    _, k, v, table, lengths = make([20, 30], 4, 2, 32, 16, BF16, stale=1.0)
+    table[0] = table[0].clamp(min=0)                      # every entry is a page
+    lengths[0] = bad
+    qkv = torch.randn(2, tokens, 8 * 32, device=DEV).to(BF16)
+    cos, sin = (x.to(DEV) for x in R.rotary(32, 64))
+    ok = torch.tensor([0, 30], dtype=torch.int32, device=DEV)
+    rq, rk, rv = R.append(qkv, k, v, table, ok, cos, sin)
+    flags()
+    q = paged.paged_append(qkv, k, v, table, lengths, cos, sin)
+    assert flags() & L.FLAG_INDEX_RANGE
+    assert not bool(q[0].any()) and bool(q[1].any())
+    for got, ref in ((k, rk), (v, rv)):
+        assert bool(((got.double().cpu() - ref).abs() <= 2.0 ** -7 * ref.abs() + 2.0 ** -20).all())
+
+
+@pytest.mark.parametrize("bad", [10 ** 6, 49, -1])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("room", [False, True])
+@pytest.mark.parametrize("window", [0, 10])
+def test_attention_leaves_out_rows_whose_length_is_outside_the_table(monkeypatch, bad, dtype, room, window):
+    unchecked(monkeypatch)
+    q, k, v, table, lengths = make([20, 30, 3], 4, 2, 32, 16, dtype, stale=1.0)
+    if room:
+        table = roomy(table, 16)
+        bad = bad if bad < 49 else 100000 // 16 * 16 + 1
+    want, wlse = paged.paged_attention(q, k, v, table, lengths, window=window, return_lse=True)
+    lengths[0] = bad
+    flags()
+    out, lse = paged.paged_attention(q, k, v, table, lengths, window=window, return_lse=True)
+    assert flags() & L.FLAG_INDEX_RANGE
+    assert not bool(out[0].any()) and bool((lse[0] == -math.inf).all())
+    # (the work is cut by the lengths, so the other rows' sums may be split elsewhere)
+    torch.testing.assert_close(out[1:].float(), want[1:].float(), rtol=2.0 ** -7, atol=1e-5)
+    torch.testing.assert_close(lse[1:], wlse[1:], rtol=1e-5, atol=1e-5)
