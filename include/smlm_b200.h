@@ -520,10 +520,11 @@ SMLM_API int smlm_paged_append(const void *qkv, void *k_pages, void *v_pages, in
 /* ------------------------------------------------------------------------------- pages of a paged cache
  * No counterpart in the reference. refcount (int32, n_pages): how many table entries hold each page, 0 = free; this
  * is the whole state of the allocator, and the lowest free page is always taken first. rows, parents, children:
- * device int32 row numbers; negative ones are left out (so that lists can have a fixed length), rows listed twice and
- * rows past the table set SMLM_FLAG_INDEX_RANGE. A sequence of n
- * tokens has ceil(n / page_size) entries, the later ones of its row being -1 (entries that smlm_pages_trim dropped
- * are -1 too). */
+ * device int32 row numbers; negative ones are left out (so that lists can have a fixed length), rows past the table are
+ * too and set SMLM_FLAG_INDEX_RANGE. A row listed twice is freed or trimmed once; in rows to extend or children it acts
+ * once and sets the flag. A sequence of n tokens has ceil(n / page_size) entries, the later ones of its row being -1
+ * (entries that smlm_pages_trim dropped are -1 too). A row whose length is outside the table (below 0 or beyond
+ * max_blocks * page_size) is not extended, forked or trimmed and sets SMLM_FLAG_INDEX_RANGE; freeing it ends that. */
 
 /* The rows' pages are released, their entries become -1 and their lengths 0. */
 SMLM_API int smlm_pages_free(int32_t *table, int64_t table_stride, int64_t table_rows, int64_t max_blocks,

@@ -34,6 +34,13 @@ __device__ __forceinline__ bool row_ok(const Pages& pg, int r) {
     return false;
 }
 
+// Whether a row's length is one that the table can hold (flagged if not).
+__device__ __forceinline__ bool length_ok(const Pages& pg, int len, int shift) {
+    if (len >= 0 && len <= (int64_t)pg.max_blocks << shift) return true;
+    flag(pg.status, SMLM_FLAG_INDEX_RANGE);
+    return false;
+}
+
 // Takes the entry out of the table (an exchange, so that a row listed twice is released once) and drops the page.
 __device__ __forceinline__ void drop_entry(const Pages& pg, int32_t* entry) {
     if (*entry < 0) return;
@@ -56,7 +63,7 @@ __global__ void __launch_bounds__(256) pages_trim_kernel(Pages pg, const int32_t
     grid_wait();
     grid_release();
     const int r = rows[blockIdx.x];
-    if (!row_ok(pg, r)) return;
+    if (!row_ok(pg, r) || !length_ok(pg, pg.lengths[r], shift)) return;
     const int64_t first = (((int64_t)sinks + (1 << shift) - 1) >> shift);
     const int64_t last = max((int64_t)pg.lengths[r] - window, (int64_t)0) >> shift;
     for (int64_t j = first + threadIdx.x; j < min(last, (int64_t)pg.max_blocks); j += blockDim.x)
@@ -308,8 +315,8 @@ __global__ void __launch_bounds__(PLAN_THREADS)
             const int head = lane < mb ? row[lane] : -1;  // not waiting for the length
             if (owner != i) {
                 if (lane == 0) flag(pg.status, SMLM_FLAG_INDEX_RANGE);
-            } else if (c != p) {
-                len = min(max(held, 0), mb << shift);
+            } else if (c != p && length_ok(pg, held, shift)) {
+                len = held;
                 const int used = (len + (1 << shift) - 1) >> shift, rest = len & ((1 << shift) - 1);
                 for (int j = lane; j < used; j += 32) {
                     int e = j < 32 ? head : row[j];

@@ -74,3 +74,22 @@ def test_attention_leaves_out_rows_whose_length_is_outside_the_table(monkeypatch
     # (the work is cut by the lengths, so the other rows' sums may be split elsewhere)
     torch.testing.assert_close(out[1:].float(), want[1:].float(), rtol=2.0 ** -7, atol=1e-5)
     torch.testing.assert_close(lse[1:], wlse[1:], rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.parametrize("bad", [25, 10 ** 9, -1])
+def test_fork_and_trim_leave_out_rows_whose_length_is_outside_the_table(monkeypatch, bad):
+    """Three blocks of 8 tokens: a row of 25 is neither copied nor trimmed, the other rows of the call are."""
+    unchecked(monkeypatch)
+    t = lambda *r: torch.tensor(r, dtype=torch.int32, device=DEV)  # noqa: E731
+    table = torch.tensor([[0, 1, 2], [3, 4, -1], [5, -1, -1], [-1, -1, -1]], dtype=torch.int32, device=DEV)
+    lengths, ref = t(bad, 16, 8, 0), t(1, 1, 1, 1, 1, 1, 0)
+    pool = torch.zeros(1, 2, 7, 1, 8, 16, dtype=BF16, device=DEV)
+    flags()
+    paged.pages_fork(pool, table, lengths, ref, t(0, 1), t(2, 3))
+    assert flags() & L.FLAG_INDEX_RANGE
+    assert table.tolist() == [[0, 1, 2], [3, 4, -1], [5, -1, -1], [3, 4, -1]]
+    assert lengths.tolist() == [bad, 16, 8, 16] and ref.tolist() == [1, 1, 1, 2, 2, 1, 0]
+    paged.pages_trim(table, lengths, ref, t(0, 1), 8, 2)
+    assert flags() & L.FLAG_INDEX_RANGE
+    assert table.tolist() == [[0, 1, 2], [-1, 4, -1], [5, -1, -1], [3, 4, -1]]
+    assert ref.tolist() == [1, 1, 1, 1, 2, 1, 0]
