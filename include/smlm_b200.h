@@ -517,6 +517,16 @@ SMLM_API int smlm_paged_append(const void *qkv, void *k_pages, void *v_pages, in
                                int64_t max_blocks, const float *cos, const float *sin, int64_t max_pos, void *q_out,
                                int *status, void *stream);
 
+/* The same (no counterpart in the reference) with the tokens each sequence really grew by: grown NULL, or int32 (batch);
+ * of sequence b only the last grown[b] tokens of the chunk are taken, the ones before are as padding. A sequence that
+ * smlm_pages_extend_grown could not extend has 0 there and keeps its last tokens, which its chunk would overwrite
+ * otherwise (positions are counted back from the length). */
+SMLM_API int smlm_paged_append_grown(const void *qkv, void *k_pages, void *v_pages, int dtype, const int64_t *strides,
+                                     const int32_t *table, int64_t table_stride, const int32_t *lengths, int64_t batch,
+                                     int64_t tokens, int64_t hq, int64_t hkv, int64_t d, int64_t n_pages,
+                                     int64_t page_size, int64_t max_blocks, const float *cos, const float *sin,
+                                     int64_t max_pos, const int32_t *grown, void *q_out, int *status, void *stream);
+
 /* ------------------------------------------------------------------------------- pages of a paged cache
  * No counterpart in the reference. refcount (int32, n_pages): how many table entries hold each page, 0 = free; this
  * is the whole state of the allocator, and the lowest free page is always taken first. rows, parents, children:
@@ -544,6 +554,14 @@ SMLM_API int smlm_pages_extend(int32_t *table, int64_t table_stride, int64_t tab
                                int32_t *lengths, int32_t *refcount, int64_t n_pages, int64_t page_size,
                                const int32_t *rows, int64_t n, int64_t n_new, void *workspace, size_t workspace_bytes,
                                int *status, void *stream);
+
+/* The same (no counterpart in the reference); grown: NULL, or int32 (table_rows) that receives n_new at the rows that
+ * grew and 0 at the listed ones that did not (other rows' entries stay). An append for rows that may have failed takes
+ * it (smlm_paged_append_grown). Scratch as smlm_pages_extend. */
+SMLM_API int smlm_pages_extend_grown(int32_t *table, int64_t table_stride, int64_t table_rows, int64_t max_blocks,
+                                     int32_t *lengths, int32_t *refcount, int64_t n_pages, int64_t page_size,
+                                     const int32_t *rows, int64_t n, int64_t n_new, int32_t *grown, void *workspace,
+                                     size_t workspace_bytes, int *status, void *stream);
 
 /* Row children[i] becomes a copy of row parents[i] as it was before the call, for all i at once (a row may be both);
  * what the children held is released. Whole pages are shared, the tokens of a partly filled last page are copied to a

@@ -139,6 +139,16 @@ Layer layer(const char* what, const at::Tensor& x, const at::Tensor& k, const at
 // columns.
 int64_t row_stride(const at::Tensor& table) { return table.size(0) > 1 ? table.stride(0) : table.size(1); }
 
+// A contiguous int32 tensor of n numbers on like's device, or None.
+int32_t* optional_ints(const char* what, const char* name, PyObject* o, int64_t n, const at::Tensor& like) {
+    if (o == Py_None) return nullptr;
+    const at::Tensor& t = tensor(o, what, name);
+    if (t.scalar_type() != at::kInt || t.dim() != 1 || t.size(0) != n || !t.is_contiguous())
+        refuse("%s: %s has to be a contiguous int32 tensor of %lld numbers", what, name, (long long)n);
+    same_device(what, {&like, &t});
+    return static_cast<int32_t*>(t.data_ptr());
+}
+
 template <typename F>
 PyObject* guarded(F f) {
     try {
@@ -195,10 +205,10 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
-// (qkv, k_pages, v_pages, table, lengths, cos, sin)
+// (qkv, k_pages, v_pages, table, lengths, cos, sin, grown)
 PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const char* what = "paged_append";
-    if (!arity(what, n, 7)) return nullptr;
+    if (!arity(what, n, 8)) return nullptr;
     return guarded([&]() -> PyObject* {
         at::Tensor x = tensor(a[0], what, "qkv");
         const at::Tensor &k = tensor(a[1], what, "k_pages"), &v = tensor(a[2], what, "v_pages");
@@ -223,14 +233,15 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
             sin = static_cast<const float*>(s.data_ptr());
             positions = c.size(0);
         }
+        const int32_t* grown = optional_ints(what, "grown", a[7], batch, x);
         if (!x.is_contiguous()) x = x.contiguous();
         Call c(x);
         at::Tensor q = fresh({batch, tokens, hq, l.d}, x.scalar_type(), x);
-        checked(what, smlm_paged_append(x.data_ptr(), k.data_ptr(), v.data_ptr(), l.code, l.strides,
-                                        static_cast<const int32_t*>(table.data_ptr()), row_stride(table),
-                                        static_cast<const int32_t*>(lengths.data_ptr()), batch, tokens, hq, l.hkv, l.d,
-                                        l.pages, l.page, table.size(1), cos, sin, positions, q.data_ptr(), c.st,
-                                        c.stream));
+        checked(what, smlm_paged_append_grown(x.data_ptr(), k.data_ptr(), v.data_ptr(), l.code, l.strides,
+                                              static_cast<const int32_t*>(table.data_ptr()), row_stride(table),
+                                              static_cast<const int32_t*>(lengths.data_ptr()), batch, tokens, hq, l.hkv,
+                                              l.d, l.pages, l.page, table.size(1), cos, sin, positions, grown,
+                                              q.data_ptr(), c.st, c.stream));
         return THPVariable_Wrap(std::move(q));
     });
 }
@@ -311,20 +322,21 @@ PyObject* pages_trim(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
-// (table, lengths, refcount, rows, n_new, page_size)
+// (table, lengths, refcount, rows, n_new, page_size, grown)
 PyObject* pages_extend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const char* what = "pages_extend";
-    if (!arity(what, n, 6)) return nullptr;
+    if (!arity(what, n, 7)) return nullptr;
     return guarded([&]() -> PyObject* {
         const Tables t(what, a);
         const at::Tensor& rows = tensor(a[3], what, "rows");
         const int32_t* r = ints(what, "row numbers", rows, 1);
         const int64_t fresh = integer(a[4]), page = integer(a[5]);
         same_device(what, {&t.table, &t.lengths, &t.refcount, &rows});
+        int32_t* grown = optional_ints(what, "grown", a[6], t.rows, t.table);
         Call c(t.table);
         const size_t bytes = smlm_pages_extend_workspace(rows.size(0), t.pages);
-        checked(what, smlm_pages_extend(t.t, t.stride, t.rows, t.blocks, t.l, t.r, t.pages, page, r, rows.size(0), fresh,
-                                        c.workspace(bytes), bytes, c.st, c.stream));
+        checked(what, smlm_pages_extend_grown(t.t, t.stride, t.rows, t.blocks, t.l, t.r, t.pages, page, r, rows.size(0),
+                                              fresh, grown, c.workspace(bytes), bytes, c.st, c.stream));
         Py_RETURN_NONE;
     });
 }

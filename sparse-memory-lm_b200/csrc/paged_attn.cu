@@ -986,7 +986,8 @@ __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(PageView pv, i
 // once and written once. A thread handles 16 bytes of a head's first half and the 16 bytes they are paired with in its
 // second half (value i with i + d / 2), for U of a token's heads: those loads go out first, then the position, and
 // from it the page and the cos and sin that the heads share. Nothing is exchanged between threads.
-// Token t of row b is at position lengths[b] - T + t; a negative one is the padding before a shorter chunk.
+// Token t of row b is at position lengths[b] - T + t; a negative one is the padding before a shorter chunk, and with
+// grown (or NULL) so are all but the row's last grown[b] tokens.
 // Memory bounds it. 16 x 2048 tokens of 18 heads x 64, bf16: 29.7 us, 82% of the copy rate (heads a thread: two 31.3,
 // three 30.3, four 35.2, six 30.8; blocks of 256 threads 30.6; a thread for each pair, with the block's positions looked
 // up once into shared memory behind a barrier, 34.2); 3 x 777 tokens of 48 heads x 128, fp32: 17.4 us, 97%.
@@ -995,7 +996,8 @@ constexpr int APPEND_THREADS = 128, APPEND_HEADS = 3;
 template <typename T, int U>
 __global__ void __launch_bounds__(APPEND_THREADS)
     paged_append_kernel(PageView pv, const T* qkv, int tokens, const float* cosb, const float* sinb, int max_pos,
-                        T* __restrict__ q_out, int groups, int per_block, uint32_t all, int* status) {
+                        const int32_t* grown, T* __restrict__ q_out, int groups, int per_block, uint32_t all,
+                        int* status) {
     constexpr int CH = 16 / sizeof(T);
     grid_wait();
     grid_release();
@@ -1020,6 +1022,7 @@ __global__ void __launch_bounds__(APPEND_THREADS)
         if (h0 == g) {
             const int b = token / (uint32_t)tokens, t = token - (uint32_t)b * tokens;
             pos = row_length(pv, b, status) - tokens + t;
+            if (grown && tokens - t > grown[b]) pos = -1;
             if (pos >= 0) {
                 const int page = page_of(pv, b, pos, status);
                 if (cosb && pos < max_pos) {
@@ -1345,11 +1348,11 @@ extern "C" int smlm_paged_attention(const void* q, const void* k_pages, const vo
     });
 }
 
-extern "C" int smlm_paged_append(const void* qkv, void* k_pages, void* v_pages, int dtype, const int64_t* strides,
-                                 const int32_t* table, int64_t table_stride, const int32_t* lengths, int64_t batch,
-                                 int64_t tokens, int64_t hq, int64_t hkv, int64_t d, int64_t n_pages, int64_t page_size,
-                                 int64_t max_blocks, const float* cos, const float* sin, int64_t max_pos, void* q_out,
-                                 int* status, void* stream) {
+extern "C" int smlm_paged_append_grown(const void* qkv, void* k_pages, void* v_pages, int dtype, const int64_t* strides,
+                                       const int32_t* table, int64_t table_stride, const int32_t* lengths, int64_t batch,
+                                       int64_t tokens, int64_t hq, int64_t hkv, int64_t d, int64_t n_pages,
+                                       int64_t page_size, int64_t max_blocks, const float* cos, const float* sin,
+                                       int64_t max_pos, const int32_t* grown, void* q_out, int* status, void* stream) {
     if (batch == 0 || tokens == 0) return SMLM_OK;
     PageView pv;
     const int rc = fill_view(pv, "paged_append", k_pages, v_pages, dtype, strides, table, table_stride, lengths, batch,
@@ -1377,7 +1380,17 @@ extern "C" int smlm_paged_append(const void* qkv, void* k_pages, void* v_pages, 
         return launch_dependent(each == 1 ? paged_append_kernel<T, 1> : paged_append_kernel<T, APPEND_HEADS>,
                                 "paged_append", 1, grid, APPEND_THREADS, as_stream(stream), pv,
                                 static_cast<const T*>(qkv), (int)tokens, cos, sin,
-                                (int)std::min<int64_t>(max_pos, INT32_MAX), static_cast<T*>(q_out), (int)groups,
+                                (int)std::min<int64_t>(max_pos, INT32_MAX), grown, static_cast<T*>(q_out), (int)groups,
                                 (int)per_block, (uint32_t)all, status);
     });
+}
+
+extern "C" int smlm_paged_append(const void* qkv, void* k_pages, void* v_pages, int dtype, const int64_t* strides,
+                                 const int32_t* table, int64_t table_stride, const int32_t* lengths, int64_t batch,
+                                 int64_t tokens, int64_t hq, int64_t hkv, int64_t d, int64_t n_pages, int64_t page_size,
+                                 int64_t max_blocks, const float* cos, const float* sin, int64_t max_pos, void* q_out,
+                                 int* status, void* stream) {
+    return smlm_paged_append_grown(qkv, k_pages, v_pages, dtype, strides, table, table_stride, lengths, batch, tokens, hq,
+                                   hkv, d, n_pages, page_size, max_blocks, cos, sin, max_pos, nullptr, q_out, status,
+                                   stream);
 }

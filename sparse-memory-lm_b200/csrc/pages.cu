@@ -234,11 +234,12 @@ __device__ int scan_needs(int n, int32_t* offset, int most, F need) {
 // whose pages are not there, or whose table is too narrow, stays as it is and raises a flag. The lengths are taken by
 // an exchange and put back at the end, which finds rows listed twice (the second does nothing). Without a page to
 // hand out (most decoding steps) the counts are not read. Eight rows: 4 us, a launch and four dependent accesses.
+// grown (or NULL): what each listed row of the table grew by, n_new or 0.
 // V: what the wanted pages are summed in; the host takes 32 bits where they cannot pass them (64: 0.2 us more).
 template <typename V>
 __global__ void __launch_bounds__(PLAN_THREADS) pages_extend_kernel(Pages pg, const int32_t* rows, int n, int n_new,
                                                                     int shift, int32_t* offset, int32_t* len_of,
-                                                                    int32_t* list, int32_t* totals) {
+                                                                    int32_t* list, int32_t* totals, int32_t* grown) {
     constexpr int TAKEN = INT32_MIN;
     grid_wait();
     grid_release();
@@ -276,6 +277,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) pages_extend_kernel(Pages pg, co
                 pg.refcount[page] = 1;
             }
         pg.lengths[rows[i]] = grow ? len + n_new : len;
+        if (grown) grown[rows[i]] = grow ? n_new : 0;
     }
 }
 
@@ -549,17 +551,17 @@ extern "C" size_t smlm_pages_extend_workspace(int64_t n, int64_t n_pages) {
     return ws.used;
 }
 
-extern "C" int smlm_pages_extend(int32_t* table, int64_t table_stride, int64_t table_rows, int64_t max_blocks,
-                                 int32_t* lengths, int32_t* refcount, int64_t n_pages, int64_t page_size,
-                                 const int32_t* rows, int64_t n, int64_t n_new, void* workspace, size_t workspace_bytes,
-                                 int* status, void* stream) {
-    if (n == 0 || n_new == 0) return SMLM_OK;
+extern "C" int smlm_pages_extend_grown(int32_t* table, int64_t table_stride, int64_t table_rows, int64_t max_blocks,
+                                       int32_t* lengths, int32_t* refcount, int64_t n_pages, int64_t page_size,
+                                       const int32_t* rows, int64_t n, int64_t n_new, int32_t* grown, void* workspace,
+                                       size_t workspace_bytes, int* status, void* stream) {
+    if (n == 0 || (n_new == 0 && !grown)) return SMLM_OK;
     Pages pg;
     const int rc = check_pages(pg, "pages_extend", table, table_stride, table_rows, max_blocks, lengths, refcount,
                                n_pages, page_size, status);
     if (rc != SMLM_OK) return rc;
     SMLM_CHECK_ARG(rows && lengths && n > 0 && n <= 65535, "pages_extend: %lld rows (at most 65535)", (long long)n);
-    SMLM_CHECK_ARG(n_new > 0 && n_new <= max_blocks * page_size, "pages_extend: %lld new tokens", (long long)n_new);
+    SMLM_CHECK_ARG(n_new >= 0 && n_new <= max_blocks * page_size, "pages_extend: %lld new tokens", (long long)n_new);
     Workspace ws(workspace, workspace_bytes);
     int32_t* offset = ws.take<int32_t>(n);
     int32_t* len_of = ws.take<int32_t>(n);
@@ -572,7 +574,15 @@ extern "C" int smlm_pages_extend(int32_t* table, int64_t table_stride, int64_t t
     const bool fits = n * (n_new / page_size + 1) <= INT32_MAX;  // a row's need is at most that
     return launch_plan(fits ? pages_extend_kernel<int32_t> : pages_extend_kernel<int64_t>, "pages_extend",
                        std::max(n, n_pages), as_stream(stream), pg, rows, (int)n, (int)n_new, log2_of(page_size), offset,
-                       len_of, list, totals);
+                       len_of, list, totals, grown);
+}
+
+extern "C" int smlm_pages_extend(int32_t* table, int64_t table_stride, int64_t table_rows, int64_t max_blocks,
+                                 int32_t* lengths, int32_t* refcount, int64_t n_pages, int64_t page_size,
+                                 const int32_t* rows, int64_t n, int64_t n_new, void* workspace, size_t workspace_bytes,
+                                 int* status, void* stream) {
+    return smlm_pages_extend_grown(table, table_stride, table_rows, max_blocks, lengths, refcount, n_pages, page_size,
+                                   rows, n, n_new, nullptr, workspace, workspace_bytes, status, stream);
 }
 
 extern "C" size_t smlm_pages_fork_workspace(int64_t n, int64_t table_rows, int64_t max_blocks, int64_t n_pages) {

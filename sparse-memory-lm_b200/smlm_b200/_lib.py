@@ -105,10 +105,13 @@ SIGNATURES = {
                                     _f32, _i64, _i64, _p, _p, _p, _sz, _p, _p]),
     "smlm_paged_append": (_i32, [_p, _p, _p, _i32, _p, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                                  _p, _p, _i64, _p, _p, _p]),
+    "smlm_paged_append_grown": (_i32, [_p, _p, _p, _i32, _p, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                                       _i64, _p, _p, _i64, _p, _p, _p, _p]),
     "smlm_pages_free": (_i32, [_p, _i64, _i64, _i64, _p, _p, _i64, _p, _i64, _p, _p]),
     "smlm_pages_trim": (_i32, [_p, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _i64, _i64, _p, _p]),
     "smlm_pages_extend_workspace": (_sz, [_i64, _i64]),
     "smlm_pages_extend": (_i32, [_p, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _i64, _p, _sz, _p, _p]),
+    "smlm_pages_extend_grown": (_i32, [_p, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _sz, _p, _p]),
     "smlm_pages_fork_workspace": (_sz, [_i64, _i64, _i64, _i64]),
     "smlm_pages_fork": (_i32, [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _i64, _p, _sz,
                                _p, _p]),

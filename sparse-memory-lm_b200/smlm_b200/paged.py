@@ -17,7 +17,9 @@ PagedKVCache keeps these tensors together for a model; smlm_b200.decode.PagedDec
 The cache and the activations are fp32, bf16 or fp16, of one type; scores, softmax sums and outputs are accumulated in
 fp32 and rounded once. What a row's table and length do not cover is never used, whatever its bits. Rows of the table
 outside their range, pages outside the pool and an exhausted pool do not fault: the token or row is left out and a flag
-of the device status word is set (SMLM_B200_CHECK=1 turns it into an exception).
+of the device status word is set (SMLM_B200_CHECK=1 turns it into an exception). A sequence that an exhausted pool kept
+from growing is left out by the append that follows if it is given what pages_extend wrote to `grown`; PagedKVCache counts
+pages on the host and never lets it come to that.
 """
 import importlib.machinery
 import importlib.util
@@ -77,15 +79,19 @@ def paged_attention(q, k_pages, v_pages, table, lengths, *, scale=None, window=0
                  window, sinks, return_lse)
 
 
-def paged_append(qkv, k_pages, v_pages, table, lengths, cos=None, sin=None):
+def paged_append(qkv, k_pages, v_pages, table, lengths, cos=None, sin=None, grown=None):
     """The last T tokens of every sequence: qkv (B, T, (query heads + 2 key heads) d), queries, then keys, then values;
     keys and values are written to their pages (positions lengths[b] - T .. lengths[b] - 1; a negative one is padding
     before a shorter chunk and is not stored), queries are returned, (B, T, query heads, d). With cos / sin (fp32,
     (positions, d / 2)) queries and keys are turned by the half-split rotary embedding of their position, in fp32,
-    rounded once."""
+    rounded once.
+
+    grown (int32 (B,), what pages_extend wrote for these rows): only the last grown[b] tokens of the chunk are taken, the
+    others are as padding. Without it, the chunk of a sequence that pages_extend could not extend overwrites the tokens at
+    its end."""
     if not _instrumented():
-        return _native.append(qkv, k_pages, v_pages, table, lengths, cos, sin)
-    return _call("paged_append", 1, qkv.device, _native.append, qkv, k_pages, v_pages, table, lengths, cos, sin)
+        return _native.append(qkv, k_pages, v_pages, table, lengths, cos, sin, grown)
+    return _call("paged_append", 1, qkv.device, _native.append, qkv, k_pages, v_pages, table, lengths, cos, sin, grown)
 
 
 # --------------------------------------------------------------------------------------------- the pages
@@ -105,13 +111,15 @@ def pages_trim(table, lengths, refcount, rows, page_size, window, sinks=0):
                  window, sinks)
 
 
-def pages_extend(table, lengths, refcount, rows, n_new, page_size):
+def pages_extend(table, lengths, refcount, rows, n_new, page_size, grown=None):
     """Every sequence in `rows` grows by n_new tokens: lengths[r] += n_new, with the lowest free pages (row by row) where
-    its last page is full. A sequence that finds too few keeps its length."""
+    its last page is full. A sequence that finds too few keeps its length; an append for it has to know (its positions
+    are counted back from the length): grown, int32 (table rows,), receives n_new at the rows that grew and 0 at the
+    listed ones that did not, and paged_append takes it."""
     if not _instrumented():
-        return _native.pages_extend(table, lengths, refcount, rows, n_new, page_size)
+        return _native.pages_extend(table, lengths, refcount, rows, n_new, page_size, grown)
     return _call("pages_extend", 1, table.device, _native.pages_extend, table, lengths, refcount, rows, n_new,
-                 page_size)
+                 page_size, grown)
 
 
 def pages_fork(pool, table, lengths, refcount, parents, children):

@@ -93,3 +93,48 @@ def test_fork_and_trim_leave_out_rows_whose_length_is_outside_the_table(monkeypa
     assert flags() & L.FLAG_INDEX_RANGE
     assert table.tolist() == [[0, 1, 2], [-1, 4, -1], [5, -1, -1], [3, 4, -1]]
     assert ref.tolist() == [1, 1, 1, 1, 2, 1, 0]
+
+
+def test_a_row_that_could_not_grow_is_left_out_by_the_append(monkeypatch):
+    """Rows 0 and 1 share a full page and one page is free: row 0 grows, row 1 does not, and its token must not land on
+    the shared page's last slot."""
+    unchecked(monkeypatch)
+    t = lambda *r: torch.tensor(r, dtype=torch.int32, device=DEV)  # noqa: E731
+    table = torch.tensor([[0, -1], [0, -1], [-1, -1]], dtype=torch.int32, device=DEV)
+    lengths, ref, grown = t(16, 16, 0), t(2, 0), t(7, 7, 7)
+    k, v = torch.randn(2, 2, 1, 16, 32, device=DEV).to(BF16)
+    k0, v0 = k.clone(), v.clone()
+    flags()
+    paged.pages_extend(table, lengths, ref, t(0, 1, -1), 1, 16, grown=grown)
+    assert flags() & L.FLAG_NO_PAGES
+    assert lengths.tolist() == [17, 16, 0] and grown.tolist() == [1, 0, 7]
+    qkv = torch.randn(3, 1, 3 * 32, device=DEV).to(BF16)
+    q = paged.paged_append(qkv, k, v, table, lengths, grown=grown)
+    assert torch.equal(k[0], k0[0]) and torch.equal(v[0], v0[0])
+    assert torch.equal(k[1, 0, 0], qkv[0, 0, 32:64]) and torch.equal(v[1, 0, 0], qkv[0, 0, 64:])
+    assert torch.equal(q[0, 0, 0], qkv[0, 0, :32]) and not bool(q[1].any())
+    # a chunk of which only the last token is new: the ones before it are as padding
+    chunk = torch.randn(1, 3, 3 * 32, device=DEV).to(BF16)
+    k1 = k.clone()
+    q = paged.paged_append(chunk, k, v, table[:1], lengths[:1], grown=t(1))
+    assert not bool(q[0, :2].any()) and torch.equal(q[0, 2, 0], chunk[0, 2, :32])
+    k1[1, 0, 0] = chunk[0, 2, 32:64]
+    assert torch.equal(k, k1)
+
+
+def test_extend_says_what_each_listed_row_grew_by(monkeypatch):
+    unchecked(monkeypatch)
+    t = lambda *r: torch.tensor(r, dtype=torch.int32, device=DEV)  # noqa: E731
+    table = torch.full((5, 2), -1, dtype=torch.int32, device=DEV)
+    lengths, ref, grown = t(0, 30, 0, 3, -5), torch.zeros(9, dtype=torch.int32, device=DEV), t(-1, -1, -1, -1, -1)
+    paged.pages_extend(table, lengths, ref, t(3, -1, 0, 1, 77, 4), 9, 16, grown=grown)
+    assert grown.tolist() == [9, 0, -1, 9, 0] and lengths.tolist() == [9, 30, 0, 12, -5]
+    flags()
+    for bad in (grown[:4], grown.long(), grown.cpu()):
+        with pytest.raises(ValueError):
+            paged.pages_extend(table, lengths, ref, t(3), 1, 16, grown=bad)
+    qkv = torch.zeros(2, 1, 3 * 32, device=DEV, dtype=BF16)
+    k = torch.zeros(9, 1, 16, 32, device=DEV, dtype=BF16)
+    for bad in (grown[:1], grown[:2].long(), grown[:2].cpu()):
+        with pytest.raises(ValueError):
+            paged.paged_append(qkv, k, k.clone(), table[:2], lengths[:2], grown=bad)
