@@ -306,8 +306,11 @@ class PagedView:
         return paged_attention(q, k, v, self.table, self.lengths, window=self.window, sinks=self.sinks)
 
     def gather(self, layer):
-        """keys and values of the sequences, (B, heads, held, d) each (trimmed pages as page 0: masked by the window)."""
-        out = self.cache.pool[layer][:, self.table.clamp(min=0).long()].transpose(2, 3).flatten(3, 4)
+        """keys and values of the sequences, (B, heads, held, d) each, in trimmed pages 0: a mask keeps their weights out,
+        but not an infinity or NaN times 0 that another sequence's page would bring in."""
+        rows = self.table[:, :-(-self.held // self.cache.page_size)]
+        out = self.cache.pool[layer][:, rows.clamp(min=0).long()].masked_fill_((rows < 0)[..., None, None, None], 0)
+        out = out.transpose(2, 3).flatten(3, 4)
         return out[0, :, :, :self.held], out[1, :, :, :self.held]
 
     def visible(self, tokens):

@@ -1,0 +1,35 @@
+"""PagedKVCache and PagedDecoder between steps: sequences beside one with infinities."""
+import math
+
+import pytest
+import torch
+
+from smlm_b200.decode import PagedDecoder
+from smlm_b200.model import ModelConfig, Transformer
+from test_gpu_paged import DEV
+from test_gpu_paged_decode import ids
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dense():
+    """A model without memory layers."""
+    torch.manual_seed(1)
+    return Transformer(ModelConfig(vocab_size=256, d_model=64, n_layers=2, n_heads=4, ffn_hidden=128, max_seq_len=96,
+                                   mem_layers=[])).to(DEV).eval()
+
+
+def test_a_chunk_after_trimmed_pages_reads_no_other_sequence(dense):
+    """Page 0 belongs to a sequence whose keys and values are infinite and NaN; a chunk prefilled into a sequence that has
+    released pages to its window does not see it."""
+    outs = []
+    for bad in (0.0, math.nan, math.inf):
+        dec = PagedDecoder(dense, 2, page_size=4, window=8, sinks=2)
+        dec.prefill(ids(4, 1), [0])
+        dec.prefill(ids(24, 2), [1])
+        assert int(dec.cache.table[0, 0]) == 0 and -1 in dec.cache.table[1, :6].tolist()
+        dec.cache.pool[:, :, 0] = bad
+        outs.append(dec.prefill(ids(6, 3), [1]))
+    assert bool(outs[0].isfinite().all())
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
