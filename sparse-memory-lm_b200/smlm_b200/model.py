@@ -154,8 +154,10 @@ class Attention(nn.Module):
         """Rotated keys and values into their pages; one token per sequence attends over the pages in place, several
         (a prompt, or a chunk after cached tokens) over the gathered sequence."""
         view, layer = cache["paged"], cache["layer"]
+        T = qkv.shape[1]
+        if T > 1 and view.held is None:      # before anything is written
+            raise ValueError("a pass of several tokens needs the view of sequences of one length, cache.view(rows)")
         q = view.append(layer, qkv, pos.cos, pos.sin)
-        T = q.shape[1]
         if T == 1:
             return view.attend(layer, q[:, 0])
         k, v = view.gather(layer)

@@ -1,12 +1,13 @@
-"""PagedKVCache and PagedDecoder between steps: sequences beside one with infinities."""
+"""PagedKVCache, its views and PagedDecoder between steps."""
 import math
 
 import pytest
 import torch
 
+from smlm_b200 import paged
 from smlm_b200.decode import PagedDecoder
 from smlm_b200.model import ModelConfig, Transformer
-from test_gpu_paged import DEV
+from test_gpu_paged import DEV, F32
 from test_gpu_paged_decode import ids
 
 pytestmark = pytest.mark.gpu
@@ -33,3 +34,14 @@ def test_a_chunk_after_trimmed_pages_reads_no_other_sequence(dense):
         outs.append(dec.prefill(ids(6, 3), [1]))
     assert bool(outs[0].isfinite().all())
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+def test_a_pass_of_several_tokens_over_the_view_of_all_rows_writes_nothing(dense):
+    cache = paged.PagedKVCache.for_model(dense, 2, page_size=4, dtype=F32)
+    cache.extend([0, 1], 5)
+    cache.pool.fill_(2.0)
+    with torch.no_grad():
+        with pytest.raises(ValueError, match="several tokens"):
+            dense(ids(3, 1).expand(2, -1), kv_caches=cache.view().caches())
+        assert bool((cache.pool == 2.0).all())
+        assert dense(ids(5, 1).expand(2, -1), kv_caches=cache.view([0, 1]).caches()).shape == (2, 5, 256)
