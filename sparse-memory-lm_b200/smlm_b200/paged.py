@@ -208,6 +208,8 @@ class PagedKVCache:
 
     def reserve(self, rows, n):
         """Host side of extend: checks and counts n more tokens for each of `rows`."""
+        if n < 0:
+            raise ValueError(f"PagedKVCache.extend: {n} new tokens")
         p = self.page_size
         for r in rows:
             if self._len[r] + n > self.max_len:

@@ -45,3 +45,13 @@ def test_a_pass_of_several_tokens_over_the_view_of_all_rows_writes_nothing(dense
             dense(ids(3, 1).expand(2, -1), kv_caches=cache.view().caches())
         assert bool((cache.pool == 2.0).all())
         assert dense(ids(5, 1).expand(2, -1), kv_caches=cache.view([0, 1]).caches()).shape == (2, 5, 256)
+
+
+def test_extending_by_less_than_nothing_changes_nothing():
+    cache = paged.PagedKVCache(1, 4, 4, 1, 16, 2, 16, F32, DEV)
+    cache.extend([0], 6)
+    with pytest.raises(ValueError, match="-5"):
+        cache.extend([0], -5)
+    assert cache.length(0) == 6 and cache.free_pages() == 2 and cache.lengths.tolist() == [6, 0]
+    cache.extend([0], 0)
+    assert cache.length(0) == 6 and cache.lengths.tolist() == [6, 0]
