@@ -225,20 +225,33 @@ class PagedKVCache:
         pages_extend(self.table, self.lengths, self.refcount, self._device(rows), n, self.page_size)
 
     def fork(self, parents, children):
-        """children[i] becomes a copy of parents[i] (as both were before the call). Needs a free page for every child
-        whose parent's last page is partly filled."""
+        """children[i] becomes a copy of parents[i] (as both were before the call). Needs a page for every child whose
+        parent's last page is partly filled, free before the call or released with what the children held."""
         children, parents = self._rows(children), list(parents)
         for r in parents:
             self._rows([r])
         if len(parents) != len(children):
             raise ValueError(f"{len(parents)} parents, {len(children)} children")
-        need = sum(self._len[p] % self.page_size > 0 for p, c in zip(parents, children) if p != c)
+        pairs = [(p, c) for p, c in zip(parents, children) if p != c]
+        need = sum(self._len[p] % self.page_size > 0 for p, _ in pairs)
         if need > self.free_pages():
-            raise RuntimeError(f"PagedKVCache.fork: {need} pages needed, {self._free} of {self.refcount.shape[0]} free")
+            free = self._free_in_fork(pairs)
+            if need > free:
+                raise RuntimeError(f"PagedKVCache.fork: {need} pages needed, {free} of {self.refcount.shape[0]} free")
         pages_fork(self.pool, self.table, self.lengths, self.refcount, self._device(parents), self._device(children))
         self._free = None
         for c, n in zip(children, [self._len[p] for p in parents]):
             self._len[c] = n
+
+    def _free_in_fork(self, pairs):
+        """The pages a fork of these (parent, child) pairs has to hand out: those that nothing holds once the parents'
+        are held and the children's released (reads the tables)."""
+        table, count = self.table.cpu(), self.refcount.cpu()
+        for p, c in pairs:
+            held, old = table[p, :-(-self._len[p] // self.page_size)], table[c]
+            count += torch.bincount(held[held >= 0], minlength=len(count))
+            count -= torch.bincount(old[old >= 0], minlength=len(count))
+        return int((count == 0).sum())
 
     def free(self, rows):
         """The sequences end; pages that no other sequence shares become free."""

@@ -8,7 +8,7 @@ from smlm_b200 import paged
 from smlm_b200.decode import PagedDecoder
 from smlm_b200.model import ModelConfig, Transformer
 from test_gpu_paged import DEV, F32
-from test_gpu_paged_decode import ids
+from test_gpu_paged_decode import close, growing, ids, model  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +55,26 @@ def test_extending_by_less_than_nothing_changes_nothing():
     assert cache.length(0) == 6 and cache.free_pages() == 2 and cache.lengths.tolist() == [6, 0]
     cache.extend([0], 0)
     assert cache.length(0) == 6 and cache.lengths.tolist() == [6, 0]
+
+
+def test_a_reordering_in_a_full_pool_that_frees_the_pages_it_needs(model):
+    """All 3 x 8 pages are in use. [1, 1, 0] drops row 2's eight pages and copies two partly filled ones: the device
+    completes that, so it must not be refused; one that needs more than is dropped still is."""
+    dec = PagedDecoder(model, 3, page_size=4, max_len=32)
+    prompts = [ids(30, s) for s in (20, 21, 22)]
+    dec.prefill(torch.cat(prompts), range(3))
+    assert dec.cache.free_pages() == 0
+    dec.reorder([1, 1, 0])
+    fed = dec.tokens.clone()
+    dec.step()
+    for r, p in enumerate([1, 1, 0]):
+        close(dec.logits[r], growing(model, prompts[p], fed[r].view(1))[1:])
+    cache = paged.PagedKVCache(1, 4, 4, 1, 16, 4, 16, F32, DEV)
+    cache.extend([0], 6)
+    cache.extend([1, 2], 3)
+    with pytest.raises(RuntimeError, match="pages needed"):
+        cache.fork([0, 0], [1, 3])                    # frees one page, needs two
+    assert cache.lengths.tolist() == [6, 3, 3, 0] and cache.table.tolist()[1:] == [[2, -1, -1, -1], [3, -1, -1, -1],
+                                                                                  [-1] * 4]
+    cache.fork([0], [1])                              # frees one, needs one
+    assert cache.lengths.tolist() == [6, 6, 3, 0] and cache.table.tolist()[:2] == [[0, 1, -1, -1], [0, 2, -1, -1]]
