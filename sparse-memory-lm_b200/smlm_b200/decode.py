@@ -23,7 +23,7 @@ prompt's pages (fork), and with a sliding window the pages that have left it are
         dec.prefill(prompt_ids, rows=[0])   # one prompt
         dec.fork(0, range(1, 8))            # eight continuations of it
         for _ in range(256):
-            dec.step(sample(dec.logits) if dec.logits is not None else None)
+            dec.step(sample(dec.logits))
         dec.free([3])                       # a sequence ends; its pages serve others
 """
 import torch
@@ -155,7 +155,7 @@ class PagedDecoder:
         self.cache = PagedKVCache.for_model(model, max_seqs, max_len, page_size, n_pages, dtype)
         self.tokens = torch.zeros(max_seqs, 1, dtype=torch.long, device=dev)  # the next step's input tokens
         self.live = torch.full((max_seqs,), -1, dtype=torch.int32, device=dev)  # row numbers, -1: idle
-        self.logits = None                                                    # of the last step, (max_seqs, 1, vocab)
+        self.logits = None       # what follows each row's last token, (max_seqs, 1, vocab); None before the first prefill
         self._graph = None
         self._key = None
 
@@ -169,8 +169,8 @@ class PagedDecoder:
 
     @torch.no_grad()
     def prefill(self, ids, rows):
-        """ids (B, P) appended to the sequences `rows` (all of one length: empty ones for prompts); sets their next
-        tokens to the greedy choice. Returns the logits (B, P, vocab)."""
+        """ids (B, P) appended to the sequences `rows` (all of one length: empty ones for prompts); sets their rows of
+        self.logits to the last position's and their next tokens to the greedy choice. Returns the logits (B, P, vocab)."""
         rows = list(rows)
         if ids.dim() != 2 or ids.shape[0] != len(rows) or not ids.shape[1]:
             raise ValueError(f"prefill: ids {tuple(ids.shape)} for {len(rows)} sequences")
@@ -178,18 +178,25 @@ class PagedDecoder:
             raise ValueError("prefill: the sequences have to be of one length (prefill them one by one)")
         self.cache.extend(rows, ids.shape[1])
         logits = self.model(ids, kv_caches=self.cache.view(rows, self.window, self.sinks).caches())
-        self.tokens[torch.tensor(rows, device=ids.device)] = logits[:, -1:].argmax(-1)
+        at = torch.tensor(rows, device=ids.device)
+        self.tokens[at] = logits[:, -1:].argmax(-1)
+        if self.logits is None:
+            self._make_logits(logits)
+        self.logits[at] = logits[:, -1:].to(self.logits.dtype)
         self._trim(rows)
         self._set_live()
         return logits
 
     def fork(self, parent, children):
-        """Every row of `children` becomes a copy of the sequence `parent`, next token included."""
+        """Every row of `children` becomes a copy of the sequence `parent`, logits and next token included."""
         children = [c for c in children if c != parent]
         if not self.cache.length(parent):
             raise ValueError(f"fork: row {parent} holds no sequence")
         self.cache.fork([parent] * len(children), children)
-        self.tokens[torch.tensor(children, dtype=torch.long, device=self.tokens.device)] = self.tokens[parent].clone()
+        at = torch.tensor(children, dtype=torch.long, device=self.tokens.device)
+        self.tokens[at] = self.tokens[parent].clone()
+        if self.logits is not None:
+            self.logits[at] = self.logits[parent].clone()
         self._set_live()
 
     def reorder(self, parents):
@@ -198,7 +205,10 @@ class PagedDecoder:
         if len(parents) != self.cache.max_seqs:
             raise ValueError(f"reorder: {len(parents)} parents for {self.cache.max_seqs} rows")
         self.cache.fork(parents, range(len(parents)))
-        self.tokens.copy_(self.tokens[torch.tensor(parents, device=self.tokens.device)])
+        at = torch.tensor(parents, device=self.tokens.device)
+        self.tokens.copy_(self.tokens[at])
+        if self.logits is not None:
+            self.logits.copy_(self.logits[at])
         self._set_live()
 
     def free(self, rows):
@@ -210,11 +220,19 @@ class PagedDecoder:
         if self.window:
             self.cache.trim(rows, self.window, self.sinks)
 
+    def _make_logits(self, like):
+        # an ordinary tensor in inference mode too, so that prefill and fork can write its rows at any time
+        with torch.inference_mode(False):
+            self.logits = torch.zeros(self.cache.max_seqs, 1, like.shape[-1], dtype=like.dtype, device=like.device)
+
     def _body(self):
         c = self.cache
         pages_extend(c.table, c.lengths, c.refcount, self.live, 1, c.page_size)
-        self.logits = self.model(self.tokens, kv_caches=c.view(None, self.window, self.sinks).caches())
-        self.tokens.copy_(self.logits[:, -1:].argmax(-1))
+        logits = self.model(self.tokens, kv_caches=c.view(None, self.window, self.sinks).caches())
+        if self.logits is None or self.logits.dtype != logits.dtype:       # (in the warm-up: every row is written)
+            self._make_logits(logits)
+        self.logits.copy_(logits)
+        self.tokens.copy_(logits[:, -1:].argmax(-1))
 
     @torch.no_grad()
     def step(self, tokens=None):
@@ -245,6 +263,7 @@ class PagedDecoder:
                else torch.autocast("cuda", enabled=False))
         dev = self.tokens.device
         saved, live, lengths = self.tokens.clone(), self.live.clone(), self.cache.lengths.clone()
+        logits = None if self.logits is None else self.logits.clone()
         try:
             self.live.fill_(-1)
             self.cache.lengths.zero_()
@@ -261,6 +280,8 @@ class PagedDecoder:
             self.tokens.copy_(saved)
             self.live.copy_(live)
             self.cache.lengths.copy_(lengths)
+            if logits is not None:
+                self.logits.copy_(logits)
             for m, f in zip(mems, flags):
                 m.decode_graph = f
         self._graph, self._key = graph, key

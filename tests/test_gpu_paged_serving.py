@@ -78,3 +78,60 @@ def test_a_reordering_in_a_full_pool_that_frees_the_pages_it_needs(model):
                                                                                   [-1] * 4]
     cache.fork([0], [1])                              # frees one, needs one
     assert cache.lengths.tolist() == [6, 6, 3, 0] and cache.table.tolist()[:2] == [[0, 1, -1, -1], [0, 2, -1, -1]]
+
+
+def test_logits_follow_prefills_forks_and_reorderings(model):
+    """Sampling from dec.logits works after every call, on a decoder that has already stepped: row r of the logits belongs
+    to the sequence that row r holds."""
+    dec = PagedDecoder(model, 4, page_size=4)
+    history = {}
+
+    def prefill(row, n, seed):
+        p = ids(n, seed)
+        got = dec.prefill(p, [row])
+        history[row] = p
+        assert torch.equal(dec.logits[row, 0], got[0, -1])
+
+    def agree():
+        for r, h in history.items():
+            with torch.no_grad():
+                close(dec.logits[r], model(h)[0, -1:])
+            assert int(dec.tokens[r]) == int(dec.logits[r, 0].argmax())
+
+    def step():
+        second = dec.logits[:, 0].topk(2).indices[:, 1:]               # the second best token of every row
+        dec.step(second)
+        for r in history:
+            history[r] = torch.cat((history[r], second[r:r + 1]), 1)
+        agree()
+
+    prefill(0, 9, 1)
+    step()
+    prefill(2, 13, 2)                  # a row joins one that has stepped
+    agree()
+    step()
+    dec.fork(0, [1, 3])
+    history[1] = history[3] = history[0]
+    agree()
+    step()
+    dec.reorder([2, 0, 1, 1])
+    history = {0: history[2], 1: history[0], 2: history[1], 3: history[1]}
+    agree()
+    step()
+    dec.free([1])
+    del history[1]
+    prefill(1, 5, 3)
+    agree()
+    step()
+
+
+def test_steps_in_inference_mode_and_forks_outside(model):
+    dec = PagedDecoder(model, 2, page_size=4)
+    with torch.inference_mode():
+        dec.prefill(ids(7, 1), [0])
+        dec.step()
+    dec.fork(0, [1])
+    assert torch.equal(dec.logits[0], dec.logits[1]) and not dec.logits.is_inference()
+    with torch.inference_mode():
+        dec.step()
+    assert torch.equal(dec.tokens[0], dec.tokens[1])
