@@ -12,6 +12,8 @@
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/smlm_b200.h"
@@ -89,6 +91,20 @@ struct Call {
 // An uninitialised tensor beside `like`.
 at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
     return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+}
+
+// These calls have no gradient. Where one would be recorded, the output gets a node that says so in a backward pass (a
+// forward pass outside no_grad is fine by itself).
+void no_gradient(const char* what, std::initializer_list<const at::Tensor*> ins, std::initializer_list<at::Tensor*> outs) {
+    if (!at::GradMode::is_enabled()) return;
+    torch::autograd::edge_list next;
+    for (const at::Tensor* t : ins)
+        if (t->requires_grad()) next.push_back(torch::autograd::impl::gradient_edge(*t));
+    if (next.empty()) return;
+    auto node = std::make_shared<torch::autograd::Error>(std::string(what) + " has no gradient (decoding only)",
+                                                         std::move(next));
+    for (at::Tensor* t : outs)
+        if (t->defined()) torch::autograd::set_history(*t, node);
 }
 
 void checked(const char* what, int rc) {
@@ -200,6 +216,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                            l.pages, l.page, table.size(1), (float)scale, window, sinks, out.data_ptr(),
                                            with_lse ? static_cast<float*>(lse.data_ptr()) : nullptr, c.workspace(bytes),
                                            bytes, c.st, c.stream));
+        no_gradient(what, {&q, &k, &v}, {&out, &lse});
         PyObject* o = THPVariable_Wrap(std::move(out));
         return with_lse ? Py_BuildValue("(NN)", o, THPVariable_Wrap(std::move(lse))) : o;
     });
@@ -242,6 +259,7 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                               static_cast<const int32_t*>(lengths.data_ptr()), batch, tokens, hq, l.hkv,
                                               l.d, l.pages, l.page, table.size(1), cos, sin, positions, grown,
                                               q.data_ptr(), c.st, c.stream));
+        no_gradient(what, {&x}, {&q});
         return THPVariable_Wrap(std::move(q));
     });
 }

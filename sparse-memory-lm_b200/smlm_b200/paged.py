@@ -19,7 +19,7 @@ fp32 and rounded once. What a row's table and length do not cover is never used,
 outside their range, pages outside the pool and an exhausted pool do not fault: the token or row is left out and a flag
 of the device status word is set (SMLM_B200_CHECK=1 turns it into an exception). A sequence that an exhausted pool kept
 from growing is left out by the append that follows if it is given what pages_extend wrote to `grown`; PagedKVCache counts
-pages on the host and never lets it come to that.
+pages on the host and never lets it come to that. There are no gradients: a backward pass through these calls raises.
 """
 import importlib.machinery
 import importlib.util

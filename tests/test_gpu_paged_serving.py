@@ -7,7 +7,7 @@ import torch
 from smlm_b200 import paged
 from smlm_b200.decode import PagedDecoder
 from smlm_b200.model import ModelConfig, Transformer
-from test_gpu_paged import DEV, F32
+from test_gpu_paged import DEV, F32, make
 from test_gpu_paged_decode import close, growing, ids, model  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -135,3 +135,35 @@ def test_steps_in_inference_mode_and_forks_outside(model):
     with torch.inference_mode():
         dec.step()
     assert torch.equal(dec.tokens[0], dec.tokens[1])
+
+
+def test_a_backward_pass_through_the_paged_calls_raises(model):
+    """Forward passes without no_grad work as before; their backward says that there is no gradient."""
+    cache = paged.PagedKVCache.for_model(model, 2, page_size=4, dtype=F32)
+    cache.extend([0, 1], 5)
+    x = ids(5, 1).expand(2, -1)
+    with torch.no_grad():
+        want = model(x, kv_caches=cache.view([0, 1]).caches())
+    out = model(x, kv_caches=cache.view([0, 1]).caches())
+    assert torch.equal(out, want)
+    with pytest.raises(RuntimeError, match="paged_append has no gradient"):
+        out.sum().backward()
+    model.zero_grad(set_to_none=True)
+    q, k, v, table, lengths = make([9], 2, 2, 32, 16, F32)
+    q.requires_grad_()
+    for outs in (paged.paged_attention(q, k, v, table, lengths, return_lse=True),
+                 (paged.paged_attention(q * 2, k, v, table, lengths),)):
+        for o in outs:
+            with pytest.raises(RuntimeError, match="paged_attention has no gradient"):
+                o.sum().backward()
+    assert q.grad is None
+    qkv = torch.randn(1, 1, 6 * 32, device=DEV, requires_grad=True)
+    with pytest.raises(RuntimeError, match="paged_append has no gradient"):
+        paged.paged_append(qkv, k, v, table, lengths).sum().backward()
+    with torch.no_grad():
+        assert not paged.paged_attention(q, k, v, table, lengths).requires_grad
+        assert not paged.paged_append(qkv, k, v, table, lengths).requires_grad
+    assert not paged.paged_attention(q.detach(), k, v, table, lengths).requires_grad
+    # keys and values with a gradient of their own
+    with pytest.raises(RuntimeError, match="paged_attention has no gradient"):
+        paged.paged_attention(q.detach(), k, v.clone().requires_grad_(), table, lengths).sum().backward()
