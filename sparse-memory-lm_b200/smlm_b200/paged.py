@@ -37,7 +37,7 @@ def _load():
     path = os.path.join(os.path.dirname(L.LIB_PATH), "_paged.so")
     if not os.path.exists(path):
         raise ImportError(f"{path} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'` "
-                          "or `make -C sparse-memory-lm_b200/csrc`")
+                          "or `make -C sparse-memory-lm_b200/csrc binding`")
     loader = importlib.machinery.ExtensionFileLoader("_paged", path)
     module = importlib.util.module_from_spec(importlib.machinery.ModuleSpec("_paged", loader, origin=path))
     loader.exec_module(module)
@@ -45,15 +45,21 @@ def _load():
     return module
 
 
-_native = _load()
+class _AtFirstUse:
+    """In the binding's place until a call needs it: modules that import this one work without it."""
+
+    def __getattr__(self, name):
+        global _native
+        _native = _load()
+        return getattr(_native, name)
 
 
-_checking = _native.checking
+_native = _AtFirstUse()
 
 
 def _instrumented():
     """Whether calls are timed, ranged or checked."""
-    return L.PROFILE is not None or L.NVTX or _checking()
+    return L.PROFILE is not None or L.NVTX or _native.checking()
 
 
 def _call(name, launches, device, fn, *args):
