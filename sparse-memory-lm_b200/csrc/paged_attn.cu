@@ -1328,15 +1328,19 @@ extern "C" int smlm_paged_attention(const void* q, const void* k_pages, const vo
                    "paged_attention: q and out have to be 16-byte aligned");
     SMLM_CHECK_ARG(window >= 0 && sinks >= 0, "paged_attention: window %lld, sinks %lld", (long long)window,
                    (long long)sinks);
-    // the list of tiles is counted in 31 bits
-    SMLM_CHECK_ARG((double)batch * hq * ((double)max_blocks * page_size / 16 + HEAD + 1) < 2147483648.0,
-                   "paged_attention: %lld sequences x %lld heads x up to %lld tokens: fewer rows a call",
-                   (long long)batch, (long long)hq, (long long)(max_blocks * page_size));
     const AttentionArgs args{q, scale, clamp_window(window), clamp_sinks(sinks), out, lse, status, as_stream(stream)};
     return with_variant(pv, dtype, [&](auto v) {
         using V = decltype(v);
         const Cluster c = cluster_size<V>(pv, args.window, args.sinks);
         if (c.size) return launch_cluster(v, pv, c, args);
+        // the list of tiles is counted in 31 bits
+        constexpr int TT = V::S::TT, QT = V::S::QT;
+        const int64_t items = batch * hkv * ((hq / hkv + QT - 1) / QT);
+        int64_t tiles = (max_blocks * page_size + TT - 1) / TT;
+        if (args.window) tiles = std::min<int64_t>(tiles, args.window / TT + args.sinks / TT + 3);  // Span's at most
+        SMLM_CHECK_ARG(items * (tiles + HEAD) <= INT32_MAX,
+                       "paged_attention: %lld sequences x %lld heads x up to %lld tokens: fewer rows a call",
+                       (long long)batch, (long long)hq, (long long)(max_blocks * page_size));
         Workspace ws(workspace, workspace_bytes);
         SplitWork wk;
         split_work(ws, wk, batch, hq, hkv, d, element_bytes(dtype));
