@@ -185,6 +185,23 @@ bool arity(const char* what, Py_ssize_t n, Py_ssize_t want) {
     return false;
 }
 
+// (q, k_pages, v_pages, table, lengths, window, sinks): the kernels that the call launches, one where it needs no scratch
+PyObject* attention_launches(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    const char* what = "paged_attention";
+    if (!arity(what, n, 7)) return nullptr;
+    return guarded([&]() -> PyObject* {
+        const at::Tensor& q = tensor(a[0], what, "q");
+        if (q.dim() != 3) refuse("%s: q has to be (sequences, heads, head dimension)", what);
+        const at::Tensor& table = tensor(a[3], what, "table");
+        const Layer l = layer(what, q, tensor(a[1], what, "k_pages"), tensor(a[2], what, "v_pages"), table,
+                              tensor(a[4], what, "lengths"), q.size(0));
+        const c10::cuda::OptionalCUDAGuard guard(q.device());
+        const size_t bytes = smlm_paged_attention_workspace(q.size(0), q.size(1), l.hkv, l.d, l.code, l.page,
+                                                            table.size(1), integer(a[5]), integer(a[6]));
+        return PyLong_FromLong(q.size(0) ? 1 + (bytes > 0) : 0);
+    });
+}
+
 // (q, k_pages, v_pages, table, lengths, scale, window, sinks, return_lse)
 PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const char* what = "paged_attention";
@@ -416,6 +433,7 @@ PyObject* checking(PyObject*, PyObject*) {
 PyMethodDef methods[] = {{"init", init, METH_O, nullptr},
                          {"checking", checking, METH_NOARGS, nullptr},
                          FAST(attention),
+                         FAST(attention_launches),
                          FAST(append),
                          FAST(pages_free),
                          FAST(pages_trim),

@@ -81,7 +81,8 @@ def paged_attention(q, k_pages, v_pages, table, lengths, *, scale=None, window=0
     heads), -inf for such a row."""
     if not _instrumented():
         return _native.attention(q, k_pages, v_pages, table, lengths, scale, window, sinks, return_lse)
-    return _call("paged_attention", 2, q.device, _native.attention, q, k_pages, v_pages, table, lengths, scale,
+    launches = 0 if L.PROFILE is None else _native.attention_launches(q, k_pages, v_pages, table, lengths, window, sinks)
+    return _call("paged_attention", launches, q.device, _native.attention, q, k_pages, v_pages, table, lengths, scale,
                  window, sinks, return_lse)
 
 

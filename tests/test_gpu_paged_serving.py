@@ -1,13 +1,15 @@
 """PagedKVCache, its views and PagedDecoder between steps."""
+import ctypes
 import math
 
 import pytest
 import torch
 
+from smlm_b200 import _lib as L
 from smlm_b200 import paged
 from smlm_b200.decode import PagedDecoder
 from smlm_b200.model import ModelConfig, Transformer
-from test_gpu_paged import DEV, F32, make
+from test_gpu_paged import BF16, DEV, F32, make
 from test_gpu_paged_decode import close, growing, ids, model  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -167,3 +169,30 @@ def test_a_backward_pass_through_the_paged_calls_raises(model):
     # keys and values with a gradient of their own
     with pytest.raises(RuntimeError, match="paged_attention has no gradient"):
         paged.paged_attention(q.detach(), k, v.clone().requires_grad_(), table, lengths).sum().backward()
+
+
+def kernels_of(fn):
+    """How many kernels the call launches: the nodes of its captured graph."""
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        fn()
+    n = ctypes.c_size_t()
+    rc = ctypes.CDLL("libcudart.so.12").cudaGraphGetNodes(ctypes.c_void_p(graph.raw_cuda_graph()), None, ctypes.byref(n))
+    assert rc == 0
+    return n.value
+
+
+@pytest.mark.parametrize("n,batch,launches", [(64, 1, 1), (3000, 40, 2)])
+def test_the_launches_counted_are_those_made(n, batch, launches):
+    """One launch where a cluster takes an item, two with the list and its join."""
+    q, k, v, table, lengths = make([n] * batch, 6, 6, 64, 16, BF16, stale=0.0)
+    call = lambda: paged.paged_attention(q, k, v, table, lengths)  # noqa: E731
+    call()
+    assert kernels_of(call) == launches
+    L.PROFILE = []
+    try:
+        call()
+        counted = [x[3] for x in L.PROFILE]
+    finally:
+        L.PROFILE = None
+    assert counted == [launches]
