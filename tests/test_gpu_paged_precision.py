@@ -38,3 +38,42 @@ def test_weights_far_below_the_largest(dtype, hq, hkv, d, page, gap, room):
     assert bool((err <= bound).all()), float((err / bound).max())
     # the logarithm of a sum of 1 and small weights around the exponent `gap`: both rounded to fp32
     assert bool(((lse.double().cpu() - rlse).abs() <= 2.0 ** -21 * rlse.abs() + 2.0 ** -20).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("hq,hkv,d,n", [(6, 6, 64, 24), (12, 1, 64, 24), (2, 2, 256, 24), (6, 6, 64, 500)])
+def test_rounding_the_output_is_the_only_error_that_shows(dtype, hq, hkv, d, n):
+    """The squared error is that of the float64 result rounded to the type: weights rounded once to the type would add
+    about as much again at 24 tokens."""
+    q, k, v, table, lengths = make([n] * 32, hq, hkv, d, 16, dtype, seed=n + d)
+    out = paged.paged_attention(q, k, v, table, lengths).double().cpu()
+    ref = R.attention(q, k, v, table, lengths, d ** -0.5)[0]
+    rounded = ref.to(dtype).double()
+    assert float((out - ref).square().mean()) <= 1.1 * float((rounded - ref).square().mean())
+
+
+@pytest.mark.parametrize("n", [900, 20000])
+def test_fp32_error_of_long_sums(n):
+    """The root mean square error of fp32 caches is below 2^-20 of the outputs'."""
+    q, k, v, table, lengths = make([n], 6, 2, 64, 16, F32, seed=n)
+    out = paged.paged_attention(q, k, v, table, lengths).double().cpu()
+    ref = R.attention(q, k, v, table, lengths, 0.125)[0]
+    assert float((out - ref).square().mean().sqrt()) <= 2.0 ** -20 * float(ref.square().mean().sqrt())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("room", [False, True])
+def test_peaked_scores_over_values_with_a_common_part(dtype, room):
+    """Scores of tens and values around 4: the weights have to add up to the sum they are divided by. The products are
+    exact in fp32, their sum of 64 terms is off by at most 64 2^-24 of its terms' sizes (fp32 caches: 2^-19)."""
+    q, k, v, table, lengths = make([40, 333, 1500], 8, 2, 64, 16, dtype, seed=11, stale=0.0)
+    q, v = (q.float() * 6).to(dtype), (v.float() * 0.25 + 4).to(dtype)
+    out = paged.paged_attention(q, k, v, roomy(table, 16) if room else table, lengths)
+    ref, _, mag, reach = R.attention(q, k, v, table, lengths, 0.125)
+    score = 2.0 ** -19 if dtype == F32 else 64 * 2.0 ** -24
+    n = lengths.double().cpu().view(-1, 1, 1)
+    bound = R.UNIT[dtype] * ref.abs() + mag * (2 * score * reach + 2.0 ** -15 + n * 2.0 ** -24)
+    if dtype == F16:
+        bound = bound + n * 2.0 ** -40 * float(v.abs().max())
+    err = (out.double().cpu() - ref).abs()
+    assert bool((err <= bound).all()), float((err / bound).max())
