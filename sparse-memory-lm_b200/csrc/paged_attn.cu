@@ -420,10 +420,15 @@ struct Stream {
                 load_keys(i, pages, KK);
                 scores(sc, kr, qf, qs, KK);
             }
-            if constexpr (F) {  // inf - inf in a split operand? Then once more, product by product
-                const bool odd = !(sc[0][0][0] == sc[0][0][0] && sc[0][0][1] == sc[0][0][1] &&
-                                   sc[0][0][2] == sc[0][0][2] && sc[0][0][3] == sc[0][0][3]);
-                if (__any_sync(FULL, odd)) {
+            if constexpr (F) {  // inf - inf in a split operand of a token that is seen? Then once more, product by product
+                const bool odd0 = !(sc[0][0][0] == sc[0][0][0] && sc[0][0][1] == sc[0][0][1]);
+                const bool odd1 = !(sc[0][0][2] == sc[0][0][2] && sc[0][0][3] == sc[0][0][3]);
+                bool again = __any_sync(FULL, odd0 || odd1);
+                if (again) {  // (not for what lies beside the sequence: its bits would decide how the others round)
+                    const unsigned at = seen_of(i, pages) >> g;
+                    again = __any_sync(FULL, (odd0 && at & 1) || (odd1 && at >> 8 & 1));
+                }
+                if (again) {
                     const int t0 = span.token(i, TT);
 #pragma unroll
                     for (int x = 0; x < 4; x++) {

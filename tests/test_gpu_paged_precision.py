@@ -44,7 +44,7 @@ def test_weights_far_below_the_largest(dtype, hq, hkv, d, page, gap, room):
 @pytest.mark.parametrize("hq,hkv,d,n", [(6, 6, 64, 24), (12, 1, 64, 24), (2, 2, 256, 24), (6, 6, 64, 500)])
 def test_rounding_the_output_is_the_only_error_that_shows(dtype, hq, hkv, d, n):
     """The squared error is that of the float64 result rounded to the type: weights rounded once to the type would add
-    about as much again at 24 tokens."""
+    half as much again at 24 tokens."""
     q, k, v, table, lengths = make([n] * 32, hq, hkv, d, 16, dtype, seed=n + d)
     out = paged.paged_attention(q, k, v, table, lengths).double().cpu()
     ref = R.attention(q, k, v, table, lengths, d ** -0.5)[0]
@@ -77,3 +77,23 @@ def test_peaked_scores_over_values_with_a_common_part(dtype, room):
         bound = bound + n * 2.0 ** -40 * float(v.abs().max())
     err = (out.double().cpu() - ref).abs()
     assert bool((err <= bound).all()), float((err / bound).max())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 16), (256, 32), (32, 4)])
+@pytest.mark.parametrize("room", [False, True])
+def test_not_a_bit_follows_from_tokens_that_are_not_seen(dtype, d, page, room):
+    """Whatever lies past a length, in a hole's stand-in and outside the window: the output is the same to the bit."""
+    lens, window, sinks = [5, 40, 333], 70, 3
+    want = None
+    for bad in (0.0, float("nan"), float("inf"), -3e4):
+        q, k, v, table, lengths = make(lens, 4, 2, d, page, dtype, seed=d, stale=bad)
+        rows = table.tolist()
+        for b, n in enumerate(lens):
+            for j in range(sinks, n - window):
+                k[rows[b][j // page], :, j % page] = bad
+                v[rows[b][j // page], :, j % page] = bad
+        got = paged.paged_attention(q, k, v, roomy(table, page) if room else table, lengths, window=window, sinks=sinks,
+                                    return_lse=True)
+        want = want or got
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), bad
