@@ -371,6 +371,9 @@ class Transformer(nn.Module):
         padding (a sequence start)."""
         ids = self.ngram.canon[idx]
         hist = caches[0].get("eng_hist") if caches is not None else None
+        if hist is None and caches is not None and _is_paged(caches[0]) and caches[0]["paged"].held != idx.shape[1]:
+            raise ValueError("a paged cache keeps no n-gram history for Engram memories: a pass over tokens that follow "
+                             "cached ones needs the growing cache")
         if hist is None:
             hist = torch.full((ids.shape[0], self.ngram.history), self.ngram.pad, dtype=ids.dtype, device=ids.device)
         ids = torch.cat((hist, ids), dim=1)

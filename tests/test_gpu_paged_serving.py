@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from smlm_b200 import _lib as L
-from smlm_b200 import paged
+from smlm_b200 import engram, paged
 from smlm_b200.decode import PagedDecoder
 from smlm_b200.model import ModelConfig, Transformer
 from test_gpu_paged import BF16, DEV, F32, make
@@ -196,3 +196,23 @@ def test_the_launches_counted_are_those_made(n, batch, launches):
     finally:
         L.PROFILE = None
     assert counted == [launches]
+
+
+def test_engram_memories_over_a_paged_cache_see_their_history_or_are_refused(monkeypatch):
+    """The n-gram history of a paged sequence is not kept: a pass over whole sequences needs none, a later one is refused
+    (it would look up n-grams of padding)."""
+    # token compression needs the GPT-2 vocabulary, which is not reachable offline
+    monkeypatch.setattr(engram, "canonical_ids", lambda vocab: (torch.arange(vocab, dtype=torch.int64), vocab))
+    torch.manual_seed(3)
+    m = Transformer(ModelConfig(vocab_size=512, d_model=64, n_layers=2, n_heads=4, ffn_hidden=128, max_seq_len=96,
+                                mem_layers=[], eng_layers=[1], eng_heads=2, eng_head_dim=8, eng_rows=101)).to(DEV).eval()
+    cache = paged.PagedKVCache.for_model(m, 1, page_size=4, dtype=F32)
+    x = ids(9, 1)
+    with torch.no_grad():
+        cache.extend([0], 9)
+        close(m(x, kv_caches=cache.view([0]).caches()), m(x))
+        cache.extend([0], 1)
+        with pytest.raises(ValueError, match="Engram"):
+            m(x[:, :1], kv_caches=cache.view([0]).caches())
+        with pytest.raises(ValueError, match="Engram"):
+            m(x[:, :1], kv_caches=cache.view().caches())
