@@ -30,7 +30,8 @@ B-16M model, per-token lookup latency). --case configs times BASELINE configs 1-
 opt separately; config 2 also with the forward reading a bf16 copy of the fp32 table, config 4 with its inputs from a
 uniform + Zipf(1.1) token mix); --case model times BASELINE config 2 as stated, the B-1M model's training step;
 --case scoring and --case inference run one part alone; --case engram times the Engram n-gram memory module;
---case host times the B-16M layer with its table in host RAM against the reference's own host-table path.
+--case host times the B-16M layer with its table in host RAM against the reference's own host-table path; --case paged
+times the paged key-value cache (perf/operators.py's listed cases, and decoding steps over it and over the static cache).
 """
 import argparse
 import json
@@ -69,7 +70,8 @@ def parse():
     ap.add_argument("--no-cpu-baseline", action="store_true")
     ap.add_argument("--cpu-rows-per-half", type=int, default=1024)
     ap.add_argument("--cpu-tokens", type=int, default=4096)
-    ap.add_argument("--case", choices=["layer", "scoring", "inference", "configs", "engram", "model", "host"],
+    ap.add_argument("--case", choices=["layer", "scoring", "inference", "configs", "engram", "model", "host",
+                                       "paged"],
                     default="layer",
                     help="scoring: only the fused sub-key scoring + selection of the workload's layer (a small "
                          "standalone case for profiler captures; prints its time per call); inference: only the "
@@ -1262,6 +1264,82 @@ def run_inference(args, local, world=1):
     return res
 
 
+def run_paged(args):
+    """The paged key-value cache (no counterpart in the reference). operators: the listed cases of perf/operators.py,
+    microseconds a call, eager (calls in a row from Python) and as graph (device time in a captured CUDA graph of 30 calls);
+    both go round three inputs and flush nothing, so what fits L2 stays there. decode: a greedy step of a 12-layer
+    model of 384 with three memory layers (512^2 rows), bf16 autocast, over the static cache (GraphDecoder) and over
+    pages of 16 (PagedDecoder), max_len 2304, milliseconds; window: the same rows of different lengths with and without
+    a window of 512."""
+    import importlib.util
+    from smlm_b200.decode import GraphDecoder, PagedDecoder
+    from smlm_b200.model import ModelConfig, Transformer
+    spec = importlib.util.spec_from_file_location("operators", os.path.join(ROOT, "perf", "operators.py"))
+    ops = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ops)
+    ops.own = True
+    calls = 30
+    res = {"operators": {}, "decode": {}, "window": {}}
+
+    def median_us(fn, n=9, reps=10):
+        for _ in range(3):
+            fn()
+        return round(statistics.median(_event_ms(fn, reps) for _ in range(n)) / (reps * calls) * 1e3, 2)
+
+    for case in ops.listed():
+        states = [ops.prepare(case, seed) for seed in range(3)]
+
+        def many():
+            for i in range(calls):
+                ops.run(states[i % 3])
+        eager = median_us(many)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            many()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            many()
+        res["operators"][case["name"]] = {"eager_us": eager, "graph_us": median_us(graph.replay)}
+        del graph, states
+        torch.cuda.empty_cache()
+
+    cfg = ModelConfig(max_seq_len=2304, mem_layers=[2, 5, 8], mem_n_keys=512, mem_share_values=True,
+                      mem_value_grad="row_sparse")
+    torch.manual_seed(0)
+    with torch.device("cuda"):
+        model = Transformer(cfg).eval()
+
+    def step_ms(dec, reps=64):
+        for _ in range(8):
+            dec.step()
+        return round(_event_ms(dec.step, reps) / reps, 4)
+
+    with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
+        for batch, prompt in ((1, 2048), (64, 1024), (64, 2048)):
+            ids = torch.randint(0, cfg.vocab_size, (batch, prompt), device="cuda")
+            entry = {}
+            for name, cls in (("static", GraphDecoder), ("paged", PagedDecoder)):
+                dec = cls(model, batch, max_len=2304)
+                if name == "static":
+                    dec.prefill(ids)
+                else:
+                    for r in range(batch):
+                        dec.prefill(ids[r:r + 1], [r])
+                entry[name + "_ms"] = step_ms(dec)
+                del dec
+                torch.cuda.empty_cache()
+            res["decode"][f"batch {batch} at {prompt}"] = entry
+        for window in (0, 512):
+            dec = PagedDecoder(model, 64, max_len=2304, window=window, sinks=4 if window else 0)
+            for r in range(64):
+                dec.prefill(ids[r:r + 1, :513 + 20 * r], [r])
+            res["window"][f"{window}_ms" if window else "none_ms"] = step_ms(dec)
+            del dec
+    return res
+
+
 # ----------------------------------------------------------------------------------------- CPU reference
 REF_PKG = os.path.join(ROOT, "baseline", "_ref")
 
@@ -1379,6 +1457,11 @@ def main():
         return
     if args.case == "host":
         print(json.dumps(run_host(args)), flush=True)
+        return
+    if args.case == "paged":
+        with Clocks(0) as clocks:
+            res = run_paged(args)
+        print(json.dumps({"case": "paged", **res, "clocks": clocks.summary()}), flush=True)
         return
     if args.case == "inference":
         print(json.dumps({"case": "inference", **run_inference(args, 0)}), flush=True)
