@@ -28,9 +28,9 @@ namespace smlm {
 // (paged_split_kernel). With few short sequences a cluster of blocks takes an item (paged_cluster_kernel).
 //
 // Device time per call, share of the measured copy rate (6570 GB/s) for the bytes of the visible keys and values:
-//   64 x 2175 tokens, 6 heads x 64, bf16: 40.2 us, 81%; 1 x 131071, 32 / 8 heads x 128, fp16: 86.1 us, 95%;
-//   96 x 0-8191, 32 / 8 x 128, bf16: 67.0 us, 85%; 64 x 1028 seen, 16 / 2 x 128, fp16: 17.3 us (cluster), 59%;
-//   1 x 2304, 6 x 64, bf16: 5.9 us (cluster); 32 x 2048 x 8 heads, fp32, d 64 / 128: 54 / 53 us, 76%.
+//   64 x 2175 tokens, 6 heads x 64, bf16: 41.6 us, 78%; 1 x 131071, 32 / 8 heads x 128, fp16: 86.8 us, 94%;
+//   96 x 0-8191, 32 / 8 x 128, bf16: 67.6 us, 84%; 64 x 1028 seen, 16 / 2 x 128, bf16: 17.3 us (cluster), 59%;
+//   1 x 2304, 6 x 64, bf16: 5.9 us (cluster); 8 heads, fp32, 32 x 2048 x 64: 54.7 us, 75%, 16 x 2048 x 128: 53.6, 76%.
 // While all warps run, memory delivers 93% of the copy rate; the rest is the start (2.5 us to the first tiles), the
 // spread of the last warps (4 us) and the join (3 us).
 
